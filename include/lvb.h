@@ -382,6 +382,132 @@ int lvb_attention_fwd(const lvb_attn_desc* d, const void* Q, const void* K, cons
                       void* O, float* lse, void* stream);
 
 /* ---------------------------------------------------------------------------------------
+ * Position rotation of queries and keys, and its gradient. Pair i of a head (i < pairs) turns
+ * by the angle pos · freqs[i], pos the token's position on the pair's axis:
+ *   (x, y) -> (x·cos - y·sin, y·cos + x·sin),
+ * the rest of the head (head_dim - 2·pairs elements) is copied. The pairs are dealt to the
+ * axes in order: the first sections[0] pairs turn with axis 0, the next sections[1] with
+ * axis 1, and so on (one axis for text; time, height, width for video). The gradient of a
+ * rotation is the rotation by the opposite angle (`inverse`). Angles are taken in 64 bits and
+ * reduced there, cos and sin and the rotation in 32, with one rounding to the tensor's type.
+ * A Lava kernel does this per element between the projection's store and the attention's
+ * loads; it has no counterpart in the reference tree.
+ * ------------------------------------------------------------------------------------- */
+typedef enum lvb_rope_layout {
+  LVB_ROPE_HALVES = 0,  /* pair i = elements i and i + pairs */
+  LVB_ROPE_PAIRS = 1    /* pair i = elements 2i and 2i + 1 */
+} lvb_rope_layout;
+
+#define LVB_ROPE_MAX_AXES 4
+typedef struct lvb_rotation {
+  int32_t pairs;        /* a multiple of 8; 0: nothing turns (lvb_kv_append only) */
+  int32_t layout;       /* lvb_rope_layout */
+  int32_t n_axes;       /* 1..LVB_ROPE_MAX_AXES */
+  int32_t inverse;      /* 1: by the opposite angle */
+  int32_t sections[LVB_ROPE_MAX_AXES]; /* pairs of each axis; their sum is `pairs` */
+} lvb_rotation;
+
+typedef struct lvb_rope_desc {
+  int32_t dtype;        /* LVB_F16, LVB_BF16 or LVB_F32, of every tensor */
+  int32_t reserved;
+  int64_t batch, heads_q, heads_kv, seq, head_dim; /* heads_kv 0: no K */
+  /* element strides of batch, head and seq of Q, K and their results, multiples of 16 bytes;
+   * 0 for all three = packed [batch][head][seq][head_dim] */
+  int64_t q_stride[3], k_stride[3], qo_stride[3], ko_stride[3];
+  int64_t pos_stride[3]; /* element strides of axis, batch and seq in pos; a stride may be 0
+                            (the same positions for every sequence) */
+  lvb_rotation rot;
+} lvb_rope_desc;
+
+int lvb_rope_check(const lvb_rope_desc* d);
+/* Enqueue Qo = rotated Q and Ko = rotated K ([batch][head][seq][head_dim], head_dim contiguous).
+ * A result may be its own input (same pointer and strides); no other overlap. pos: int32 device
+ * array; freqs: `pairs` doubles on the device, radians per unit of position. */
+int lvb_rope(const lvb_rope_desc* d, const void* Q, const void* K, void* Qo, void* Ko,
+             const int32_t* pos, const double* freqs, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Paged KV cache: keys and values live in pages of page_size places, [page][slot][head]
+ * [head_dim] with any strides, and a sequence's pages are the first entries of its row of the
+ * block table. Place p of sequence b is slot p % page_size of page table[b][p / page_size].
+ * The new tokens of all sequences are packed: sequence b's rows are cu_q[b] .. cu_q[b+1]-1 of
+ * K, V, Q and O ([token][head][head_dim]), and they stand at its last places, seq_lens[b] -
+ * q_len .. seq_lens[b] - 1 (seq_lens counts them). Rows behind cu_q[batch] are neither read nor
+ * written. table, seq_lens, cu_q and prefix_table are int32 device arrays read by the kernels
+ * (a captured graph sees what they hold at its replay), so what they hold is checked there and
+ * reported through lvb_device_status as LVB_ERR_INVALID_ARG, with the call's effect limited:
+ * site 81, a length that is negative or beyond the table's row (counts as 0); site 82, a page
+ * number outside the cache (attention reads zeros, the append writes nothing); site 83, query
+ * rows that do not fit in `tokens` or are more than max_q (the sequence is left out).
+ * ------------------------------------------------------------------------------------- */
+typedef struct lvb_paged_desc {
+  int32_t dtype;          /* LVB_F16 or LVB_BF16 */
+  int32_t causal;         /* attention: 1: a query at place p sees places 0..p; 0: all of them */
+  int64_t batch, heads_q, heads_kv, head_dim;
+  int64_t tokens;         /* rows that Q and O (K and V) have */
+  int64_t max_q;          /* no sequence has more query rows; without cu_q each has exactly this
+                             many and tokens == batch·max_q */
+  int64_t page_size;      /* a multiple of 8 */
+  int64_t num_pages;
+  int64_t table_width;    /* entries of a row of the table that may be read */
+  int64_t table_stride;   /* elements between rows (0: table_width) */
+  int64_t prefix_len;     /* keys of the prefix that all sequences share (0: none): their places
+                             come before place 0, every query sees all of them */
+  int64_t kc_stride[3], vc_stride[3]; /* element strides of page, slot and head, multiples of 16
+                                         bytes; 0 for all three = packed */
+  int64_t q_stride[2], o_stride[2];   /* token and head (0 for both = packed) */
+  float scale;            /* attention: usually 1/sqrt(head_dim) */
+  int32_t reserved;
+} lvb_paged_desc;
+
+/* Write new keys and values into their places, the keys rotated on the way, and the queries of
+ * the same tokens rotated beside them. */
+typedef struct lvb_append_desc {
+  lvb_paged_desc paged;   /* q_stride: Q's, o_stride: Qo's; causal and scale unused */
+  int64_t k_stride[2], v_stride[2]; /* token and head of the new K and V (0 for both = packed) */
+  int64_t pos_stride;     /* elements between the axes of pos */
+  lvb_rotation rot;       /* pairs 0: K is stored as it is and Q is not taken */
+} lvb_append_desc;
+
+int lvb_kv_append_check(const lvb_append_desc* d);
+/* Enqueue the append. Q and Qo may be NULL (no queries) or the same tensor (in place). pos
+ * ([axis][token], int32): the positions; NULL (one axis only): prefix_len + the token's place.
+ * freqs as in lvb_rope (NULL when pairs is 0). A token whose place is negative (seq_lens[b] below
+ * its query rows: an idle entry of a padded batch) is left out: nothing of it is written. Two
+ * tokens with the same place in the cache (a page that two sequences list) leave either's values. */
+int lvb_kv_append(const lvb_append_desc* d, void* Kc, void* Vc, const void* K, const void* V,
+                  const void* Q, void* Qo, const int32_t* table, const int32_t* seq_lens,
+                  const int32_t* cu_q, const int32_t* pos, const double* freqs, void* stream);
+
+/* Attention of the packed queries over the paged cache, the same operation as lvb_attention_fwd
+ * per sequence: O = softmax(scale·Q·Kᵀ + mask)·V over the prefix's keys and the sequence's own,
+ * fp32 softmax, P rounded to the cache's type, GQA by head grouping; rows that see no key give
+ * O = 0 and lse = -inf. `lse` (nullable) is fp32 [token][heads_q]. */
+typedef enum lvb_paged_kernel {
+  LVB_PAGED_FLASH = 0,    /* 128-row tiles of (position, head of the group) rows */
+  LVB_PAGED_DECODE = 1    /* group·max_q <= 32: the cache streamed once, its key blocks dealt
+                             evenly to the SMs whatever the lengths */
+} lvb_paged_kernel;
+
+typedef struct lvb_paged_plan {
+  int32_t kernel;         /* lvb_paged_kernel of the sequences' own keys */
+  int32_t splits;         /* LVB_PAGED_FLASH: key-range splits per query tile pair */
+  int32_t prefix_splits;  /* > 0: the prefix is read once for all query rows of a KV head, in
+                             this many key ranges, and joined with the sequences' own part;
+                             0: no prefix, or (LVB_PAGED_FLASH) read by every sequence's tiles */
+  int32_t launches;       /* kernel launches per call */
+  int64_t workspace_bytes;
+} lvb_paged_plan;
+
+int lvb_attention_paged_check(const lvb_paged_desc* d);
+int lvb_attention_paged_plan_for(const lvb_paged_desc* d, int32_t sm_count, lvb_paged_plan* out);
+/* Enqueue it. cu_q may be NULL (max_q rows per sequence). prefix_table: the prefix's pages
+ * ((prefix_len + page_size - 1) / page_size entries; NULL without one). */
+int lvb_attention_paged(const lvb_paged_desc* d, const void* Q, const void* Kc, const void* Vc,
+                        const int32_t* table, const int32_t* seq_lens, const int32_t* cu_q,
+                        const int32_t* prefix_table, void* O, float* lse, void* stream);
+
+/* ---------------------------------------------------------------------------------------
  * Sharding across the GPUs of one box. Lava has no multi-device code; the units of this
  * path are independent (GEMM output rows, attention (batch, kv-head) groups), so each rank
  * computes a contiguous range and no collective is needed on the data path. Host only.
@@ -435,7 +561,8 @@ int lvb_stream_create(void** stream);
 int lvb_stream_destroy(void* stream);
 int lvb_stream_synchronize(void* stream);
 /* Synchronise `stream`, then read and clear the current device's status word. *code is
- * LVB_OK or LVB_ERR_TIMEOUT; *where is the wait site, *block the first CTA that gave up. */
+ * LVB_OK, LVB_ERR_TIMEOUT (*where is the wait site, *block the first CTA that gave up) or
+ * LVB_ERR_INVALID_ARG (bad lengths, rows or pages of the paged cache; *where is the site). */
 int lvb_device_status(void* stream, int32_t* code, int32_t* where, int32_t* block);
 /* Wall-clock limit of every in-kernel wait, in milliseconds (default 2000; also read from
  * the environment variable LVB_WAIT_TIMEOUT_MS at first use). */

@@ -22,8 +22,9 @@ CSRC = HERE / "csrc"
 LIBDIR = HERE / "lib"
 LIB = LIBDIR / "liblvb.so"
 SOURCES = ["abi.cu", "gemm_sm100.cu", "gemv_sm100.cu", "attn_sm100.cu", "attn_decode_sm100.cu",
-           "selftest.cu", "comm.cu"]
-HEADERS = ["sm100.cuh", "epilogue.cuh", "lvb_internal.h"]
+           "selftest.cu", "comm.cu", "abi_paged.cu", "rope_append.cu", "attn_paged_sm100.cu",
+           "attn_paged_decode_sm100.cu"]
+HEADERS = ["sm100.cuh", "epilogue.cuh", "lvb_internal.h", "paged.cuh"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",

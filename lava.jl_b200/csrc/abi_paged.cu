@@ -1,0 +1,381 @@
+// abi_paged.cu — the extern "C" surface of position rotation, the paged KV cache's append and the
+// attention over it: argument validation, planning and launch order.
+#include <cmath>
+#include <cstring>
+
+#include <algorithm>
+
+#include "paged.cuh"
+
+namespace lvb {
+
+PagedLayout paged_layout(const lvb_paged_desc& d) {
+  PagedLayout l;
+  auto two = [&](const int64_t* s, long long* o) {
+    const bool packed = s[0] == 0 && s[1] == 0;
+    o[0] = packed ? d.heads_q * d.head_dim : s[0];
+    o[1] = packed ? d.head_dim : s[1];
+  };
+  auto three = [&](const int64_t* s, long long* o) {
+    const bool packed = s[0] == 0 && s[1] == 0 && s[2] == 0;
+    o[0] = packed ? d.page_size * d.heads_kv * d.head_dim : s[0];
+    o[1] = packed ? d.heads_kv * d.head_dim : s[1];
+    o[2] = packed ? d.head_dim : s[2];
+  };
+  two(d.q_stride, l.q);
+  two(d.o_stride, l.o);
+  three(d.kc_stride, l.kc);
+  three(d.vc_stride, l.vc);
+  return l;
+}
+
+void paged_seqs(PagedSeqs* p, const lvb_paged_desc& d, const int32_t* table,
+                const int32_t* seq_lens, const int32_t* cu_q, const int32_t* prefix_table,
+                DeviceState* dev) {
+  p->table = table;
+  p->lens = seq_lens;
+  p->cu_q = cu_q;
+  p->prefix_table = prefix_table;
+  p->table_stride = d.table_stride ? d.table_stride : d.table_width;
+  p->table_width = (int)d.table_width;
+  p->batch = (int)d.batch;
+  p->max_q = (int)d.max_q;
+  p->tokens = (int)d.tokens;
+  p->page_size = (int)d.page_size;
+  p->num_pages = (int)d.num_pages;
+  p->prefix_len = (int)d.prefix_len;
+  p->status = dev->status;
+}
+
+// 4-D maps over the cache: (64 of head_dim, slots of a page, KV head, page).
+int paged_kv_maps(CUtensorMap* tk, CUtensorMap* tv, const lvb_paged_desc* d, const PagedLayout& lay,
+                  const void* Kc, const void* Vc, const char* op) {
+  const uint64_t dims[4] = {(uint64_t)d->head_dim, (uint64_t)d->page_size, (uint64_t)d->heads_kv,
+                            (uint64_t)d->num_pages};
+  const uint32_t box[4] = {64, (uint32_t)paged_box(d->page_size), 1, 1};
+  const uint64_t sk[3] = {(uint64_t)lay.kc[1], (uint64_t)lay.kc[2], (uint64_t)lay.kc[0]};
+  const uint64_t sv[3] = {(uint64_t)lay.vc[1], (uint64_t)lay.vc[2], (uint64_t)lay.vc[0]};
+  int st = make_tmap_nd(tk, Kc, 2, 4, dims, sk, box, op);
+  if (st) return st;
+  return make_tmap_nd(tv, Vc, 2, 4, dims, sv, box, op);
+}
+
+namespace {
+
+constexpr int64_t kMostKeys = 1LL << 30;   // of a sequence or a prefix
+
+// `n` element strides of a 16-bit or 32-bit tensor whose head_dim is contiguous: all zero
+// (packed), or each a multiple of 16 bytes and at least head_dim where its extent is above 1.
+int check_strides(const char* op, const char* what, const int64_t* s, const int64_t* extent, int n,
+                  int64_t head_dim, int esize) {
+  bool packed = true;
+  for (int i = 0; i < n; ++i) packed = packed && s[i] == 0;
+  if (packed) return LVB_OK;
+  for (int i = 0; i < n; ++i) {
+    if (s[i] < 0 || (extent[i] > 1 && s[i] < head_dim))
+      return fail(LVB_ERR_INVALID_ARG, op, std::string(what) + ": stride below head_dim");
+    if ((s[i] * esize) % 16)
+      return fail(LVB_ERR_UNSUPPORTED, op, std::string(what) + ": strides must be multiples of 16 bytes");
+  }
+  return LVB_OK;
+}
+
+int check_rotation(const char* op, const lvb_rotation& r, int64_t head_dim) {
+  if (r.pairs < 0 || r.pairs % 8 || 2 * (int64_t)r.pairs > head_dim)
+    return fail(LVB_ERR_UNSUPPORTED, op, "pairs must be a multiple of 8 and at most head_dim / 2");
+  if (r.layout != LVB_ROPE_HALVES && r.layout != LVB_ROPE_PAIRS)
+    return fail(LVB_ERR_INVALID_ARG, op, "unknown rotation layout");
+  if (r.n_axes < 1 || r.n_axes > LVB_ROPE_MAX_AXES)
+    return fail(LVB_ERR_INVALID_ARG, op, "n_axes must be 1..4");
+  int64_t sum = 0;
+  for (int a = 0; a < r.n_axes; ++a) {
+    if (r.sections[a] < 0) return fail(LVB_ERR_INVALID_ARG, op, "negative section");
+    sum += r.sections[a];
+  }
+  if (sum != r.pairs)
+    return fail(LVB_ERR_INVALID_ARG, op, "the sections' pairs must add up to `pairs`");
+  return LVB_OK;
+}
+
+// What the append and the attention ask of the cache and the batch.
+int check_paged(const char* op, const lvb_paged_desc* d) {
+  if (!d) return fail(LVB_ERR_INVALID_ARG, op, "descriptor is NULL");
+  if (d->batch < 0 || d->heads_q < 0 || d->heads_kv < 0 || d->tokens < 0 || d->max_q < 0 ||
+      d->table_width < 0 || d->prefix_len < 0)
+    return fail(LVB_ERR_INVALID_ARG, op, "negative extent");
+  if (d->dtype != LVB_F16 && d->dtype != LVB_BF16)
+    return fail(LVB_ERR_UNSUPPORTED, op, std::string("no kernel for ") + dtype_name(d->dtype),
+                "Float16 or BFloat16");
+  if (d->heads_kv == 0 || d->heads_q % d->heads_kv)
+    return fail(LVB_ERR_INVALID_ARG, op, "heads_q must be a multiple of heads_kv");
+  if (d->head_dim != 64 && d->head_dim != 128)
+    return fail(LVB_ERR_UNSUPPORTED, op, "head_dim must be 64 or 128");
+  if (d->page_size <= 0 || d->page_size % 8)
+    return fail(LVB_ERR_UNSUPPORTED, op, "page_size must be a positive multiple of 8");
+  if (d->num_pages < 1) return fail(LVB_ERR_INVALID_ARG, op, "the cache has no page");
+  if (d->table_stride < 0 || (d->table_stride > 0 && d->table_stride < d->table_width))
+    return fail(LVB_ERR_INVALID_ARG, op, "table_stride < table_width");
+  if (d->page_size > kMostKeys || d->table_width > kMostKeys / d->page_size ||
+      d->prefix_len > kMostKeys)
+    return fail(LVB_ERR_UNSUPPORTED, op, "more than 2^30 keys per sequence");
+  if (d->num_pages >= INT32_MAX || d->tokens > INT32_MAX || d->max_q > INT32_MAX ||
+      d->batch > INT32_MAX || d->heads_q > 65535 || d->batch * d->heads_kv > INT32_MAX ||
+      (d->batch > 0 && d->max_q > INT32_MAX / d->batch))
+    return fail(LVB_ERR_UNSUPPORTED, op, "extent above 2^31-1", "split the batch");
+  const int64_t cache[3] = {d->num_pages, d->page_size, d->heads_kv};
+  const int64_t rows[2] = {d->tokens, d->heads_q};
+  int st;
+  if ((st = check_strides(op, "K cache", d->kc_stride, cache, 3, d->head_dim, 2))) return st;
+  if ((st = check_strides(op, "V cache", d->vc_stride, cache, 3, d->head_dim, 2))) return st;
+  if ((st = check_strides(op, "Q", d->q_stride, rows, 2, d->head_dim, 2))) return st;
+  return check_strides(op, "the result", d->o_stride, rows, 2, d->head_dim, 2);
+}
+
+int check_lists(const char* op, const lvb_paged_desc* d, const int32_t* table,
+                const int32_t* seq_lens, const int32_t* cu_q, const int32_t* prefix_table) {
+  if (!seq_lens || (d->table_width > 0 && !table))
+    return fail(LVB_ERR_INVALID_ARG, op, "block table or seq_lens is NULL");
+  if (!cu_q && d->tokens != d->batch * d->max_q)
+    return fail(LVB_ERR_INVALID_ARG, op, "without cu_q, tokens must be batch·max_q");
+  if (((uintptr_t)table | (uintptr_t)seq_lens | (uintptr_t)cu_q | (uintptr_t)prefix_table) % 4)
+    return fail(LVB_ERR_INVALID_ARG, op, "pointer not aligned to its element size");
+  return LVB_OK;
+}
+
+bool use_decode(const lvb_paged_desc* d) {
+  return (d->heads_q / d->heads_kv) * d->max_q <= 32;
+}
+
+size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+
+// Workspace of a planned call: the flash kernel's, then the decoding kernel's.
+size_t flash_bytes(const lvb_paged_desc* d, const lvb_paged_plan& pl) {
+  if (pl.kernel == LVB_PAGED_FLASH)
+    return up256(paged_flash_workspace(d, pl.splits, kFlashOwn | (d->prefix_len ? kFlashPrefix : 0)));
+  return pl.prefix_splits ? up256(paged_flash_workspace(d, pl.prefix_splits, kFlashPrefix)) : 0;
+}
+
+}  // namespace
+}  // namespace lvb
+
+using namespace lvb;
+
+extern "C" {
+
+// ---------------------------------------------------------------------------------------
+// Rotation
+// ---------------------------------------------------------------------------------------
+int lvb_rope_check(const lvb_rope_desc* d) {
+  const char* op = "lvb_rope";
+  if (!d) return fail(LVB_ERR_INVALID_ARG, op, "descriptor is NULL");
+  if (d->batch < 0 || d->heads_q < 0 || d->heads_kv < 0 || d->seq < 0)
+    return fail(LVB_ERR_INVALID_ARG, op, "negative extent");
+  if (d->dtype != LVB_F16 && d->dtype != LVB_BF16 && d->dtype != LVB_F32)
+    return fail(LVB_ERR_UNSUPPORTED, op, std::string("no kernel for ") + dtype_name(d->dtype),
+                "Float16, BFloat16 or Float32");
+  if (d->head_dim <= 0 || d->head_dim % 16 || d->head_dim > 512)
+    return fail(LVB_ERR_UNSUPPORTED, op, "head_dim must be a multiple of 16, at most 512");
+  if (d->seq > INT32_MAX || d->batch > 65535 || d->heads_q > 65535 || d->heads_kv > 65535)
+    return fail(LVB_ERR_UNSUPPORTED, op, "more than 2^31-1 positions, 65535 sequences or heads",
+                "split the batch");
+  int st = check_rotation(op, d->rot, d->head_dim);
+  if (st) return st;
+  if (d->rot.pairs == 0) return fail(LVB_ERR_INVALID_ARG, op, "pairs must be at least 8");
+  const int es = dtype_size(d->dtype);
+  const int64_t eq[3] = {d->batch, d->heads_q, d->seq}, ek[3] = {d->batch, d->heads_kv, d->seq};
+  if ((st = check_strides(op, "Q", d->q_stride, eq, 3, d->head_dim, es))) return st;
+  if ((st = check_strides(op, "K", d->k_stride, ek, 3, d->head_dim, es))) return st;
+  if ((st = check_strides(op, "rotated Q", d->qo_stride, eq, 3, d->head_dim, es))) return st;
+  return check_strides(op, "rotated K", d->ko_stride, ek, 3, d->head_dim, es);
+}
+
+int lvb_rope(const lvb_rope_desc* d, const void* Q, const void* K, void* Qo, void* Ko,
+             const int32_t* pos, const double* freqs, void* stream) {
+  const char* op = "lvb_rope";
+  int st = lvb_rope_check(d);
+  if (st) return st;
+  if (d->batch == 0 || d->seq == 0 || d->heads_q + d->heads_kv == 0) return LVB_OK;
+  if ((d->heads_q && (!Q || !Qo)) || (d->heads_kv && (!K || !Ko)) || !pos || !freqs)
+    return fail(LVB_ERR_INVALID_ARG, op, "a tensor, pos or freqs is NULL");
+  if (((uintptr_t)Q | (uintptr_t)K | (uintptr_t)Qo | (uintptr_t)Ko) % 16)
+    return fail(LVB_ERR_UNSUPPORTED, op, "tensors must start on 16-byte boundaries");
+  if ((uintptr_t)pos % 4 || (uintptr_t)freqs % 8)
+    return fail(LVB_ERR_INVALID_ARG, op, "pointer not aligned to its element size");
+  DeviceState* dev = current_device_state(op);
+  if (!dev) return LVB_ERR_NO_DEVICE;
+  long long s[4][3];
+  const int64_t* given[4] = {d->q_stride, d->k_stride, d->qo_stride, d->ko_stride};
+  for (int t = 0; t < 4; ++t) {
+    const int64_t* g = given[t];
+    const int64_t H = t % 2 ? d->heads_kv : d->heads_q;
+    const bool packed = g[0] == 0 && g[1] == 0 && g[2] == 0;
+    s[t][0] = packed ? H * d->seq * d->head_dim : g[0];
+    s[t][1] = packed ? d->seq * d->head_dim : g[1];
+    s[t][2] = packed ? d->head_dim : g[2];
+  }
+  return rope_launch(d, s[0], s[1], s[2], s[3], Q, K, Qo, Ko, pos, freqs,
+                     reinterpret_cast<cudaStream_t>(stream), dev);
+}
+
+// ---------------------------------------------------------------------------------------
+// Append
+// ---------------------------------------------------------------------------------------
+int lvb_kv_append_check(const lvb_append_desc* d) {
+  const char* op = "lvb_kv_append";
+  if (!d) return fail(LVB_ERR_INVALID_ARG, op, "descriptor is NULL");
+  int st = check_paged(op, &d->paged);
+  if (st) return st;
+  const int64_t rows[2] = {d->paged.tokens, d->paged.heads_kv};
+  if ((st = check_strides(op, "K", d->k_stride, rows, 2, d->paged.head_dim, 2))) return st;
+  if ((st = check_strides(op, "V", d->v_stride, rows, 2, d->paged.head_dim, 2))) return st;
+  return d->rot.pairs == 0 ? LVB_OK : check_rotation(op, d->rot, d->paged.head_dim);
+}
+
+int lvb_kv_append(const lvb_append_desc* d, void* Kc, void* Vc, const void* K, const void* V,
+                  const void* Q, void* Qo, const int32_t* table, const int32_t* seq_lens,
+                  const int32_t* cu_q, const int32_t* pos, const double* freqs, void* stream) {
+  const char* op = "lvb_kv_append";
+  int st = lvb_kv_append_check(d);
+  if (st) return st;
+  const lvb_paged_desc& g = d->paged;
+  if (g.batch == 0 || g.tokens == 0 || g.max_q == 0) return LVB_OK;
+  if (!Kc || !Vc || !K || !V || (!Q != !Qo))
+    return fail(LVB_ERR_INVALID_ARG, op, "K, V, a cache or one of Q and Qo is NULL");
+  if ((st = check_lists(op, &g, table, seq_lens, cu_q, nullptr))) return st;
+  if (d->rot.pairs == 0 && Q)
+    return fail(LVB_ERR_INVALID_ARG, op, "Q without a rotation", "pairs is 0");
+  if (d->rot.pairs > 0 && !freqs) return fail(LVB_ERR_INVALID_ARG, op, "freqs is NULL");
+  if (d->rot.pairs > 0 && !pos && d->rot.n_axes != 1)
+    return fail(LVB_ERR_INVALID_ARG, op, "pos is NULL with several axes",
+                "only one axis can count the places");
+  if (((uintptr_t)Kc | (uintptr_t)Vc | (uintptr_t)K | (uintptr_t)V | (uintptr_t)Q | (uintptr_t)Qo) % 16)
+    return fail(LVB_ERR_UNSUPPORTED, op, "tensors must start on 16-byte boundaries");
+  if ((uintptr_t)pos % 4 || (uintptr_t)freqs % 8)
+    return fail(LVB_ERR_INVALID_ARG, op, "pointer not aligned to its element size");
+  DeviceState* dev = current_device_state(op);
+  if (!dev) return LVB_ERR_NO_DEVICE;
+  long long ks[2], vs[2];
+  for (int t = 0; t < 2; ++t) {
+    const int64_t* s = t ? d->v_stride : d->k_stride;
+    long long* o = t ? vs : ks;
+    const bool packed = s[0] == 0 && s[1] == 0;
+    o[0] = packed ? g.heads_kv * g.head_dim : s[0];
+    o[1] = packed ? g.head_dim : s[1];
+  }
+  return append_launch(d, paged_layout(g), ks, vs, Kc, Vc, K, V, Q, Qo, table, seq_lens, cu_q, pos,
+                       freqs, reinterpret_cast<cudaStream_t>(stream), dev);
+}
+
+// ---------------------------------------------------------------------------------------
+// Attention
+// ---------------------------------------------------------------------------------------
+int lvb_attention_paged_check(const lvb_paged_desc* d) {
+  const char* op = "lvb_attention_paged";
+  int st = check_paged(op, d);
+  if (st) return st;
+  if (!(d->scale > 0.0f) || std::isinf(d->scale))
+    return fail(LVB_ERR_INVALID_ARG, op, "scale must be a positive finite number");
+  if (d->heads_q / d->heads_kv > 128)
+    return fail(LVB_ERR_UNSUPPORTED, op, "more than 128 query heads per KV head");
+  return LVB_OK;
+}
+
+int lvb_attention_paged_plan_for(const lvb_paged_desc* d, int32_t sm_count, lvb_paged_plan* out) {
+  const char* op = "lvb_attention_paged";
+  int st = lvb_attention_paged_check(d);
+  if (st) return st;
+  if (!out) return fail(LVB_ERR_INVALID_ARG, op, "plan is NULL");
+  if (sm_count <= 0) sm_count = 148;
+  std::memset(out, 0, sizeof *out);
+  out->splits = 1;
+  if (d->batch == 0 || d->tokens == 0 || d->max_q == 0 || d->heads_q == 0) return LVB_OK;
+  if (use_decode(d)) {
+    out->kernel = LVB_PAGED_DECODE;
+    out->launches = 2;
+    if (d->prefix_len) {
+      out->prefix_splits = paged_flash_splits(d, sm_count, kFlashPrefix);
+      out->launches = 3;
+    }
+    out->workspace_bytes = (int64_t)(flash_bytes(d, *out) +
+                                     paged_decode_workspace(d, sm_count, d->prefix_len > 0));
+    return LVB_OK;
+  }
+  out->kernel = LVB_PAGED_FLASH;
+  out->splits = paged_flash_splits(d, sm_count, kFlashOwn | (d->prefix_len ? kFlashPrefix : 0));
+  out->launches = out->splits > 1 ? 2 : 1;
+  out->workspace_bytes = (int64_t)flash_bytes(d, *out);
+  return LVB_OK;
+}
+
+int lvb_attention_paged(const lvb_paged_desc* d, const void* Q, const void* Kc, const void* Vc,
+                        const int32_t* table, const int32_t* seq_lens, const int32_t* cu_q,
+                        const int32_t* prefix_table, void* O, float* lse, void* stream) {
+  const char* op = "lvb_attention_paged";
+  int st = lvb_attention_paged_check(d);
+  if (st) return st;
+  if (d->batch == 0 || d->tokens == 0 || d->max_q == 0 || d->heads_q == 0) return LVB_OK;
+  if (!Q || !O || !Kc || !Vc) return fail(LVB_ERR_INVALID_ARG, op, "Q, O or a cache is NULL");
+  if ((st = check_lists(op, d, table, seq_lens, cu_q, prefix_table))) return st;
+  if (d->prefix_len && !prefix_table)
+    return fail(LVB_ERR_INVALID_ARG, op, "prefix_table is NULL", "prefix_len is above 0");
+  if (((uintptr_t)Q | (uintptr_t)O | (uintptr_t)Kc | (uintptr_t)Vc) % 16)
+    return fail(LVB_ERR_UNSUPPORTED, op, "tensors must start on 16-byte boundaries");
+  if ((uintptr_t)lse % 4) return fail(LVB_ERR_INVALID_ARG, op, "lse not aligned to its element size");
+  DeviceState* dev = current_device_state(op);
+  if (!dev) return LVB_ERR_NO_DEVICE;
+  lvb_paged_plan pl;
+  if ((st = lvb_attention_paged_plan_for(d, dev->sm_count, &pl))) return st;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const PagedLayout lay = paged_layout(*d);
+  MergeParams mp = {};
+  paged_seqs(&mp.seqs, *d, table, seq_lens, cu_q, prefix_table, dev);
+  mp.Hq = (int)d->heads_q;
+  mp.Hkv = (int)d->heads_kv;
+  mp.group = mp.Hq / mp.Hkv;
+  mp.ppt = 128 / mp.group;
+  mp.O = O;
+  mp.o_st = lay.o[0];
+  mp.o_sh = lay.o[1];
+  mp.lse = lse;
+  uint8_t* ws = nullptr;
+  cudaError_t e = workspace_alloc(dev, reinterpret_cast<void**>(&ws), (size_t)pl.workspace_bytes, s);
+  if (e != cudaSuccess) return fail_cuda(e, op, "workspace allocation");
+  FlashWorkspace fw = {};
+  const bool bf16 = d->dtype == LVB_BF16;
+  const size_t fb = flash_bytes(d, pl);
+  if (pl.kernel == LVB_PAGED_DECODE) {
+    if (pl.prefix_splits) {
+      st = paged_flash_launch(d, lay, mp.seqs, Q, Kc, Vc, O, lse, kFlashPrefix, pl.prefix_splits, ws,
+                              &fw, s, dev);
+      mp.tile_o = fw.tile_o;
+      mp.tile_ml = fw.tile_ml;
+      mp.tile_splits = pl.prefix_splits;
+    }
+    DecodeWorkspace dw = {};
+    if (st == LVB_OK)
+      st = paged_decode_launch(d, lay, mp.seqs, Q, Kc, Vc, O, lse, pl.prefix_splits > 0, ws + fb,
+                               &dw, s, dev);
+    mp.dec_o = dw.part_o;
+    mp.dec_ml = dw.part_ml;
+    mp.dec_tab = dw.tab;
+    mp.dec_rows = dw.rows;
+    mp.dec_slots = dw.slots;
+    mp.dec_ctas = dw.ctas;
+    if (st == LVB_OK) st = merge_launch(mp, (int)d->head_dim, bf16, s);
+  } else {
+    const int parts = kFlashOwn | (d->prefix_len ? kFlashPrefix : 0);
+    st = paged_flash_launch(d, lay, mp.seqs, Q, Kc, Vc, O, lse, parts, pl.splits, ws, &fw, s, dev);
+    if (st == LVB_OK && pl.splits > 1) {
+      mp.tile_o = fw.tile_o;
+      mp.tile_ml = fw.tile_ml;
+      mp.tile_splits = pl.splits;
+      mp.pairs_per_seq = (int)((d->max_q + 2 * mp.ppt - 1) / (2 * mp.ppt));
+      st = merge_launch(mp, (int)d->head_dim, bf16, s);
+    }
+  }
+  e = cudaFreeAsync(ws, s);
+  if (st == LVB_OK && e != cudaSuccess) return fail_cuda(e, op, "workspace free");
+  return st;
+}
+
+}  // extern "C"

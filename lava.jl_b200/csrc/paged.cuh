@@ -1,0 +1,222 @@
+// paged.cuh — what the kernels on the paged KV cache share: the cache's description, a
+// sequence's lengths read and checked on the device, and the TMA loads of a 128-key block
+// that lies in several pages.
+//
+// Place p of sequence b is slot p % page_size of page table[b][p / page_size]; a shared prefix
+// has a table of its own and stands before place 0 of every sequence. Lengths, tables and the
+// queries' row offsets stay on the device (a captured graph is replayed while they change), so
+// the kernels check them: a length outside the table counts as 0, a sequence whose query rows
+// do not fit is left out, a page number outside the cache is read as zeros through the tensor
+// map's bounds (and never written); each is recorded in the device status word.
+#pragma once
+
+#include "lvb_internal.h"
+
+namespace lvb {
+
+// Sites of bad device data in the status word (code LVB_ERR_INVALID_ARG).
+constexpr int kBadLength = 81;   // seq_lens[b] negative or beyond the table's row
+constexpr int kBadPage = 82;     // a page number outside 0..num_pages-1
+constexpr int kBadRows = 83;     // cu_q not increasing, beyond `tokens`, or more than max_q rows
+
+struct PagedSeqs {
+  const int* table;            // [batch] rows of table_width page numbers
+  const int* lens;             // [batch]
+  const int* cu_q;             // [batch + 1], or NULL: max_q rows per sequence
+  const int* prefix_table;
+  long long table_stride;
+  int table_width;
+  int batch, max_q, tokens;
+  int page_size, num_pages;
+  int prefix_len;
+  DevStatus* status;
+};
+
+__device__ __forceinline__ void report_bad(DevStatus* status, int where, int detail) {
+  if (atomicCAS(&status->code, 0, 1 /* LVB_ERR_INVALID_ARG */) == 0) {
+    status->where = where;
+    status->block = blockIdx.x;
+    status->detail = detail;
+  }
+}
+
+// Element strides of a paged call with the packed ones filled in.
+struct PagedLayout {
+  long long q[2], o[2];     // token, head
+  long long kc[3], vc[3];   // page, slot, head
+};
+PagedLayout paged_layout(const lvb_paged_desc& d);
+int paged_kv_maps(CUtensorMap* tk, CUtensorMap* tv, const lvb_paged_desc* d, const PagedLayout& lay,
+                  const void* Kc, const void* Vc, const char* op);
+void paged_seqs(PagedSeqs* p, const lvb_paged_desc& d, const int32_t* table,
+                const int32_t* seq_lens, const int32_t* cu_q, const int32_t* prefix_table,
+                DeviceState* dev);
+// Slots per TMA box: min(128, the largest power of two dividing the page size).
+inline int paged_box(int64_t page_size) {
+  int b = 8;
+  while (b < 128 && page_size % (2 * b) == 0) b *= 2;
+  return b;
+}
+
+int rope_launch(const lvb_rope_desc* d, const long long qs[3], const long long ks[3],
+                const long long qos[3], const long long kos[3], const void* Q, const void* K,
+                void* Qo, void* Ko, const int32_t* pos, const double* freqs, cudaStream_t stream,
+                DeviceState* dev);
+int append_launch(const lvb_append_desc* d, const PagedLayout& lay, const long long ks[2],
+                  const long long vs[2], void* Kc, void* Vc, const void* K, const void* V,
+                  const void* Q, void* Qo, const int32_t* table, const int32_t* seq_lens,
+                  const int32_t* cu_q, const int32_t* pos, const double* freqs, cudaStream_t stream,
+                  DeviceState* dev);
+
+// Where the parts of a row's result lie, for the kernel that joins them (attn_paged_sm100.cu).
+// A part is an unnormalised O row of D fp32, and the row's (reference maximum in log2 units, sum).
+struct MergeParams {
+  PagedSeqs seqs;
+  int Hq, Hkv, group;
+  // The key-range splits of the flash kernel's tiles: a part's rows are the 256 of a tile pair.
+  const float* tile_o;         // [pair][Hkv][splits][256][D]
+  const float* tile_ml;        // [pair][Hkv][splits][256][2]
+  int tile_splits;             // 0: none
+  int ppt;                     // positions per 128-row tile
+  int pairs_per_seq;           // 0: pairs run over the tokens of the whole batch (the prefix)
+  // The pieces of the decoding kernel: [slot][rows][D], and where each item's pieces are.
+  const float* dec_o;
+  const float* dec_ml;
+  const int4* dec_tab;         // [batch·Hkv]; NULL: none
+  int dec_rows;
+  int dec_slots, dec_ctas;     // bounds of the table's entries
+  void* O;
+  long long o_st, o_sh;
+  float* lse;
+};
+int merge_launch(const MergeParams& p, int D, bool bf16, cudaStream_t stream);
+
+// The decoding kernel's table entry: (first slot, next CTA, last CTA, kind): the pieces are the
+// first slot, then slot 2c of every CTA c from the next to the last.
+enum { kItemDone = 0, kItemPieces = 1, kItemNoKeys = 2 };
+struct DecodeWorkspace {
+  float* part_o;
+  float* part_ml;
+  int4* tab;
+  int rows, slots, ctas;
+};
+size_t paged_decode_workspace(const lvb_paged_desc* d, int sm_count, bool keep_parts);
+// keep_parts: every item's result stays in the workspace for the join with a prefix's parts.
+int paged_decode_launch(const lvb_paged_desc* d, const PagedLayout& lay, const PagedSeqs& seqs,
+                        const void* Q, const void* Kc, const void* Vc, void* O, float* lse,
+                        bool keep_parts, void* ws, DecodeWorkspace* out, cudaStream_t stream,
+                        DeviceState* dev);
+
+// The flash kernel over the prefix's keys, the sequences' own, or both one after the other.
+struct FlashWorkspace {
+  float* tile_o;
+  float* tile_ml;
+};
+enum { kFlashOwn = 1, kFlashPrefix = 2 };
+int paged_flash_splits(const lvb_paged_desc* d, int sm_count, int parts);
+size_t paged_flash_workspace(const lvb_paged_desc* d, int splits, int parts);
+int paged_flash_launch(const lvb_paged_desc* d, const PagedLayout& lay, const PagedSeqs& seqs,
+                       const void* Q, const void* Kc, const void* Vc, void* O, float* lse, int parts,
+                       int splits, void* ws, FlashWorkspace* out, cudaStream_t stream,
+                       DeviceState* dev);
+
+struct SeqInfo {
+  int tok0;   // first query row
+  int qlen;   // query rows (0: the sequence takes no part)
+  int len;    // keys in the cache
+};
+
+// (LVB_ERR_INVALID_ARG is 1; the check costs a few integer operations per sequence.)
+__device__ __forceinline__ SeqInfo seq_info(const PagedSeqs& p, int b) {
+  SeqInfo s;
+  s.len = p.lens[b];
+  if (p.cu_q) {
+    s.tok0 = p.cu_q[b];
+    const long long q = (long long)p.cu_q[b + 1] - s.tok0;
+    s.qlen = (int)q;
+    if (q < 0 || q > p.max_q || s.tok0 < 0 || s.tok0 + q > p.tokens) {
+      report_bad(p.status, kBadRows, b);
+      s.qlen = 0;
+    }
+  } else {
+    s.tok0 = b * p.max_q;
+    s.qlen = p.max_q;
+  }
+  if (s.len < 0 || s.len > (long long)p.table_width * p.page_size) {
+    report_bad(p.status, kBadLength, b);
+    s.len = 0;
+  }
+  return s;
+}
+
+// ----------------------------------------------------------------------------------------
+// One 128-key block by TMA. The box is `box` = min(128, the largest power of two dividing the
+// page size) slots high and 64 elements (128 bytes) wide, so 128/box boxes times D/64 chunks
+// make a block: at most 32, one per lane of the producing warp. Lane i's box holds keys
+// sub·box .. of chunk c. Boxes without a valid key are not loaded.
+// ----------------------------------------------------------------------------------------
+template <int D>
+struct BlockLane {
+  static constexpr int kCh = D / 64;
+  int sub, c;
+  bool in;
+  __device__ __forceinline__ BlockLane(int lane, int box) {
+    sub = lane / kCh;
+    c = lane - sub * kCh;
+    in = sub * box < 128;
+  }
+};
+
+// The page (and slot) of the lane's box in block kb of a run of `len` keys whose pages are
+// row[0 ..]; page -1 when the box holds no valid key. A bad page number becomes num_pages,
+// which the tensor map reads as zeros.
+struct BoxAt {
+  int page, slot;
+};
+template <int D>
+__device__ __forceinline__ BoxAt box_at(const BlockLane<D>& bl, const int* row, int kb, int len,
+                                        int box, const PagedSeqs& p) {
+  BoxAt at{-1, 0};
+  const int key = kb * 128 + bl.sub * box;
+  if (bl.in && key < len) {
+    const int i = key / p.page_size;
+    at.slot = key - i * p.page_size;
+    at.page = row[i];
+    if (at.page < 0 || at.page >= p.num_pages) {
+      report_bad(p.status, kBadPage, i);
+      at.page = p.num_pages;
+    }
+  }
+  return at;
+}
+
+// Issue one block's loads into `dst` ([D/64 chunks][128 rows][128 B], 128-byte swizzle) on
+// `bar`; the whole warp calls it.
+template <int D>
+__device__ __forceinline__ void load_block(uint8_t* dst, const CUtensorMap* tm,
+                                           const BlockLane<D>& bl, const BoxAt& at, int box, int hk,
+                                           uint64_t* bar) {
+  const unsigned on = __ballot_sync(0xffffffffu, at.page >= 0);
+  if (lane_id() == 0) bar_arrive_expect_tx(bar, (uint32_t)__popc(on) * box * 128u);
+  __syncwarp();
+  if (at.page >= 0)
+    tma_load_4d(dst + bl.c * (128 * 128) + bl.sub * box * 128, tm, bl.c * 64, at.slot, hk, at.page,
+                bar);
+  __syncwarp();
+}
+
+// Zero rows [valid, 128) of a block ([D/64 chunks][128 rows][128 B]; whole rows, so the swizzle
+// plays no part) by one warp, and make the stores visible to the tensor core. What a page holds
+// behind a sequence's last place is stale (possibly infinite or NaN), and 0·NaN would reach the
+// sum through P·V although P is 0 there.
+template <int D>
+__device__ __forceinline__ void zero_tail(uint32_t block_saddr, int valid) {
+  const int lane = lane_id();
+  for (int c = 0; c < D / 64; ++c)
+    for (int i = valid * 8 + lane; i < 128 * 8; i += 32)
+      st_shared_v4(block_saddr + c * (128 * 128) + i * 16, 0, 0, 0, 0);
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
+}  // namespace lvb

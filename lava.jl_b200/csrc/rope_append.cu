@@ -1,0 +1,471 @@
+// rope_append.cu — rotation of queries and keys by their positions (lvb_rope) and the append of
+// new tokens to the paged KV cache with the rotation on the way (lvb_kv_append).
+//
+// Both are streams of 16-byte loads and stores with a few operations per element, bound by HBM
+// for many tokens and by the latency of one load-store chain for few. A CTA takes a few tokens;
+// its threads first work out cos and sin once per (token, pair) into shared memory (the angle
+// pos·freq in 64 bits, reduced to a fraction of a turn there: at position 100,000 a 32-bit angle
+// has an error of 4e-3 rad), then every thread keeps the cos and sin of its pairs in registers and
+// walks over the heads, two 16-byte vectors per head: with halves the two that face each other
+// (elements i.. and i+pairs..), with adjacent pairs two neighbouring ones, so either way the
+// vectors hold whole pairs and an in-place call is safe.
+#include <algorithm>
+#include <type_traits>
+
+#include "paged.cuh"
+
+namespace lvb {
+
+namespace {
+
+constexpr int kRotThreads = 256;
+constexpr int kRotTokens = 16;        // most tokens per CTA
+constexpr int kRotUnroll = 4;         // heads whose loads a thread has in flight
+
+struct RotArgs {
+  int pairs, layout, n_axes, inverse;
+  int sec_end[LVB_ROPE_MAX_AXES];     // first pair behind each axis's section
+  const double* freqs;
+  const int* pos;                     // NULL: the token's place (append)
+  long long pos_axis;
+};
+
+// A tensor's rows for one token: base + head·stride.
+struct HeadRows {
+  const uint8_t* src;
+  uint8_t* dst;
+  long long src_h, dst_h;             // bytes
+};
+
+__device__ __forceinline__ int axis_of(const RotArgs& r, int pair) {
+  int a = 0;
+#pragma unroll
+  for (int i = 0; i < LVB_ROPE_MAX_AXES - 1; ++i) a += (i + 1 < r.n_axes && pair >= r.sec_end[i]);
+  return a;
+}
+
+// cos and sin of pos·freq: the turn's fraction in 64 bits, then 32-bit functions of half-turns.
+__device__ __forceinline__ float2 turn(int pos, double freq, int inverse) {
+  const double t = (double)pos * freq * 0.15915494309189533577;   // 1/(2π)
+  const float f = (float)(t - rint(t));
+  float2 cs;
+  sincospif(2.f * f, &cs.y, &cs.x);
+  if (inverse) cs.y = -cs.y;
+  return cs;
+}
+
+template <typename T>
+struct Vec {
+  static constexpr int N = 16 / (int)sizeof(T);
+  __device__ static __forceinline__ void unpack(const uint4& u, float (&f)[N]) {
+    if constexpr (std::is_same<T, float>::value) {
+      f[0] = __uint_as_float(u.x);
+      f[1] = __uint_as_float(u.y);
+      f[2] = __uint_as_float(u.z);
+      f[3] = __uint_as_float(u.w);
+    } else {
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, __half>::value) {
+          const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+          f[2 * i] = v.x;
+          f[2 * i + 1] = v.y;
+        } else {   // a bf16 is the upper half of its fp32
+          f[2 * i] = __uint_as_float(w[i] << 16);
+          f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+      }
+    }
+  }
+  __device__ static __forceinline__ uint4 pack(const float (&f)[N]) {
+    if constexpr (std::is_same<T, float>::value) {
+      return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
+                        __float_as_uint(f[3]));
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, __half>::value) {
+          const __half2 v = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+          w[i] = *reinterpret_cast<const uint32_t*>(&v);
+        } else {
+          const __nv_bfloat162 v = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+          w[i] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+      }
+      return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+};
+
+// One thread's N pairs of one head: u and v become the rotated vectors.
+template <typename T, bool HALVES>
+__device__ __forceinline__ void rotate2(uint4& u, uint4& v, const float (&c)[Vec<T>::N],
+                                        const float (&s)[Vec<T>::N]) {
+  constexpr int N = Vec<T>::N;
+  float a[N], b[N];
+  Vec<T>::unpack(u, a);
+  Vec<T>::unpack(v, b);
+  if constexpr (HALVES) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float x = a[i], y = b[i];
+      a[i] = x * c[i] - y * s[i];
+      b[i] = y * c[i] + x * s[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const float x = a[2 * i], y = a[2 * i + 1], z = b[2 * i], w = b[2 * i + 1];
+      a[2 * i] = x * c[i] - y * s[i];
+      a[2 * i + 1] = y * c[i] + x * s[i];
+      b[2 * i] = z * c[N / 2 + i] - w * s[N / 2 + i];
+      b[2 * i + 1] = w * c[N / 2 + i] + z * s[N / 2 + i];
+    }
+  }
+  u = Vec<T>::pack(a);
+  v = Vec<T>::pack(b);
+}
+
+// Heads h0 + hl, + step, ... < h1 of one tensor, vectors at element offsets o0 and o1 of a head.
+template <typename T, bool HALVES>
+__device__ __forceinline__ void walk_heads(const HeadRows& r, int h, int h1, int step, int o0,
+                                           int o1, bool turns, const float (&c)[Vec<T>::N],
+                                           const float (&s)[Vec<T>::N]) {
+  for (; h < h1; h += kRotUnroll * step) {
+    uint4 u[kRotUnroll], v[kRotUnroll];
+#pragma unroll
+    for (int k = 0; k < kRotUnroll; ++k) {
+      const int hk = h + k * step;
+      if (hk < h1) {
+        const T* p = reinterpret_cast<const T*>(r.src + hk * r.src_h);
+        u[k] = *reinterpret_cast<const uint4*>(p + o0);
+        v[k] = *reinterpret_cast<const uint4*>(p + o1);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kRotUnroll; ++k) {
+      const int hk = h + k * step;
+      if (hk < h1) {
+        if (turns) rotate2<T, HALVES>(u[k], v[k], c, s);
+        T* p = reinterpret_cast<T*>(r.dst + hk * r.dst_h);
+        *reinterpret_cast<uint4*>(p + o0) = u[k];
+        *reinterpret_cast<uint4*>(p + o1) = v[k];
+      }
+    }
+  }
+}
+
+// A thread's place in its CTA: token i of the CTA's, vector pair j of a head, and the first of
+// the heads it walks (step `hpp`).
+struct Lane {
+  int i, j, hl, hpp;
+  bool on;
+  __device__ __forceinline__ Lane(int n_tok, int tasks) {
+    const int per = n_tok * tasks;
+    hpp = kRotThreads / per;
+    hl = threadIdx.x / per;
+    const int rem = threadIdx.x - hl * per;
+    i = rem / tasks;
+    j = rem - i * tasks;
+    on = hl < hpp;
+  }
+};
+
+// Element offsets of a thread's two vectors in a head, and whether they turn.
+template <typename T, bool HALVES>
+__device__ __forceinline__ bool lane_vectors(int j, int pairs, int& o0, int& o1) {
+  constexpr int N = Vec<T>::N;
+  const bool turns = j * N < pairs;
+  if (HALVES && turns) {
+    o0 = j * N;
+    o1 = pairs + j * N;
+  } else {
+    o0 = 2 * j * N;     // also the unrotated rest: elements from 2·pairs on, in order
+    o1 = o0 + N;
+  }
+  return turns;
+}
+
+template <typename T>
+__device__ __forceinline__ void lane_angles(const float2* cs, int i, int j, int pairs, bool turns,
+                                            float (&c)[Vec<T>::N], float (&s)[Vec<T>::N]) {
+  constexpr int N = Vec<T>::N;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const float2 v = turns ? cs[i * pairs + j * N + k] : make_float2(1.f, 0.f);
+    c[k] = v.x;
+    s[k] = v.y;
+  }
+}
+
+// ----------------------------------------------------------------------------------------
+// lvb_rope
+// ----------------------------------------------------------------------------------------
+struct RopeParams {
+  RotArgs rot;
+  int n_tok, tasks, S, heads_per_cta, Hq, Hkv;
+  long long pos_b, pos_s;
+  const uint8_t *Q, *K;
+  uint8_t *Qo, *Ko;
+  long long q[3], k[3], qo[3], ko[3];   // byte strides of batch, head, seq
+};
+
+template <typename T, bool HALVES>
+__global__ void __launch_bounds__(kRotThreads) rope_kernel(const RopeParams p) {
+  extern __shared__ float2 cs[];      // [n_tok][pairs]
+  const int s0 = blockIdx.x * p.n_tok;
+  const int b = blockIdx.z;
+  const int pairs = p.rot.pairs;
+  for (int x = threadIdx.x; x < p.n_tok * pairs; x += kRotThreads) {
+    const int i = x / pairs, pr = x - i * pairs;
+    if (s0 + i < p.S) {
+      const int pos = p.rot.pos[axis_of(p.rot, pr) * p.rot.pos_axis + b * p.pos_b +
+                                (s0 + i) * p.pos_s];
+      cs[x] = turn(pos, p.rot.freqs[pr], p.rot.inverse);
+    }
+  }
+  __syncthreads();
+  const Lane l(p.n_tok, p.tasks);
+  const long long s = s0 + l.i;
+  if (!l.on || s >= p.S) return;
+  int o0, o1;
+  const bool turns = lane_vectors<T, HALVES>(l.j, pairs, o0, o1);
+  float c[Vec<T>::N], sn[Vec<T>::N];
+  lane_angles<T>(cs, l.i, l.j, pairs, turns, c, sn);
+  // The CTA's heads of the list Q heads, K heads.
+  const int h0 = blockIdx.y * p.heads_per_cta;
+  const int h1 = min(h0 + p.heads_per_cta, p.Hq + p.Hkv);
+  const HeadRows rq{p.Q + b * p.q[0] + s * p.q[2], p.Qo + b * p.qo[0] + s * p.qo[2], p.q[1], p.qo[1]};
+  walk_heads<T, HALVES>(rq, h0 + l.hl, min(h1, p.Hq), l.hpp, o0, o1, turns, c, sn);
+  if (h1 > p.Hq) {
+    const HeadRows rk{p.K + b * p.k[0] + s * p.k[2], p.Ko + b * p.ko[0] + s * p.ko[2], p.k[1], p.ko[1]};
+    walk_heads<T, HALVES>(rk, max(h0 - p.Hq, 0) + l.hl, h1 - p.Hq, l.hpp, o0, o1, turns, c, sn);
+  }
+}
+
+// ----------------------------------------------------------------------------------------
+// lvb_kv_append
+// ----------------------------------------------------------------------------------------
+struct AppendParams {
+  RotArgs rot;
+  PagedSeqs seqs;
+  int n_tok, tasks, T, heads_per_cta, Hq, Hkv;   // Hq 0: no queries
+  const uint8_t *K, *V, *Q;
+  uint8_t *Kc, *Vc, *Qo;
+  long long k[2], v[2], q[2], qo[2];             // byte strides of token, head
+  long long kc[3], vc[3];                        // of page, slot, head
+};
+
+// Sequence of token t: the number of sequences that end at or before it (one warp).
+__device__ __forceinline__ int sequence_of(const PagedSeqs& p, int t) {
+  if (!p.cu_q) return t / p.max_q;
+  int b = 0;
+  for (int i = 0; i < p.batch; i += 32) {
+    const int k = i + (int)lane_id();
+    b += __popc(__ballot_sync(0xffffffffu, k < p.batch && p.cu_q[k + 1] <= t));
+  }
+  return b;
+}
+
+template <typename T, bool HALVES>
+__global__ void __launch_bounds__(kRotThreads) append_kernel(const AppendParams p) {
+  extern __shared__ float2 cs[];      // [n_tok][pairs]
+  __shared__ long long sh_k[kRotTokens], sh_v[kRotTokens];   // cache rows, bytes; -1: left out
+  __shared__ int sh_place[kRotTokens];
+  const int t0 = blockIdx.x * p.n_tok;
+  const int pairs = p.rot.pairs;
+  for (int i = warp_id(); i < p.n_tok; i += kRotThreads / 32) {
+    const int t = t0 + i;
+    int place = -1;
+    long long ko = -1, vo = -1;
+    if (t < p.T) {
+      const int b = sequence_of(p.seqs, t);
+      if (lane_id() == 0 && b < p.seqs.batch) {
+        const SeqInfo s = seq_info(p.seqs, b);
+        place = t >= s.tok0 && t - s.tok0 < s.qlen ? s.len - s.qlen + (t - s.tok0) : -1;
+        if (place >= 0) {
+          const int pi = place / p.seqs.page_size;
+          const int page = p.seqs.table[b * p.seqs.table_stride + pi];
+          if (page < 0 || page >= p.seqs.num_pages) {
+            report_bad(p.seqs.status, kBadPage, b);
+            place = -1;
+          } else {
+            const int slot = place - pi * p.seqs.page_size;
+            ko = page * p.kc[0] + slot * p.kc[1];
+            vo = page * p.vc[0] + slot * p.vc[1];
+          }
+        }
+      }
+    }
+    if (lane_id() == 0) {
+      sh_place[i] = place;
+      sh_k[i] = ko;
+      sh_v[i] = vo;
+    }
+  }
+  __syncthreads();
+  for (int x = threadIdx.x; x < p.n_tok * pairs; x += kRotThreads) {
+    const int i = x / pairs, pr = x - i * pairs;
+    if (sh_place[i] >= 0) {
+      const int pos = p.rot.pos ? p.rot.pos[axis_of(p.rot, pr) * p.rot.pos_axis + t0 + i]
+                                : p.seqs.prefix_len + sh_place[i];
+      cs[x] = turn(pos, p.rot.freqs[pr], p.rot.inverse);
+    }
+  }
+  __syncthreads();
+  const Lane l(p.n_tok, p.tasks);
+  if (!l.on || sh_place[l.i] < 0) return;
+  const long long t = t0 + l.i;
+  int o0, o1;
+  const bool turns = lane_vectors<T, HALVES>(l.j, pairs, o0, o1);
+  float c[Vec<T>::N], sn[Vec<T>::N];
+  lane_angles<T>(cs, l.i, l.j, pairs, turns, c, sn);
+  // The CTA's heads of the list Q heads, K heads, V heads.
+  const int h0 = blockIdx.y * p.heads_per_cta;
+  const int h1 = min(h0 + p.heads_per_cta, p.Hq + 2 * p.Hkv);
+  if (h0 < p.Hq) {
+    const HeadRows r{p.Q + t * p.q[0], p.Qo + t * p.qo[0], p.q[1], p.qo[1]};
+    walk_heads<T, HALVES>(r, h0 + l.hl, min(h1, p.Hq), l.hpp, o0, o1, turns, c, sn);
+  }
+  const int k0 = max(h0 - p.Hq, 0), k1 = min(h1 - p.Hq, p.Hkv);
+  if (k0 < k1) {
+    const HeadRows r{p.K + t * p.k[0], p.Kc + sh_k[l.i], p.k[1], p.kc[2]};
+    walk_heads<T, HALVES>(r, k0 + l.hl, k1, l.hpp, o0, o1, turns, c, sn);
+  }
+  const int v0 = max(h0 - p.Hq - p.Hkv, 0), v1 = h1 - p.Hq - p.Hkv;
+  if (v0 < v1) {
+    const HeadRows r{p.V + t * p.v[0], p.Vc + sh_v[l.i], p.v[1], p.vc[2]};
+    walk_heads<T, HALVES>(r, v0 + l.hl, v1, l.hpp, o0, o1, false, c, sn);
+  }
+}
+
+// Tokens per CTA and heads per CTA: up to `most` tokens, few enough for at least one head per
+// pass over the CTA's threads; the heads split until the grid has about four CTAs per SM (a
+// thread's loads in flight are kRotUnroll heads), never below one pass.
+void rot_grid(long long tokens_per_row, long long rows, int heads, int tasks, int most, int sms,
+              int* n_tok, int* heads_per_cta) {
+  int n = 1;
+  while (n < most && 2 * n * tasks <= kRotThreads && n < tokens_per_row) n *= 2;
+  // few tokens: one per CTA, so the heads of a token spread over its threads
+  while (n > 1 && rows * ((tokens_per_row + n - 1) / n) < 2LL * sms) n /= 2;
+  const int hpp = std::max(1, kRotThreads / (n * tasks));
+  const long long ctas = rows * ((tokens_per_row + n - 1) / n);
+  long long split = std::max<long long>(1, (4LL * sms + ctas - 1) / ctas);
+  int per = (int)((heads + split - 1) / split);
+  per = std::min(heads, (per + hpp - 1) / hpp * hpp);
+  *n_tok = n;
+  *heads_per_cta = std::max(1, per);
+}
+
+void fill_rot(RotArgs* r, const lvb_rotation& rot, const int32_t* pos, const double* freqs,
+              long long pos_axis) {
+  r->pairs = rot.pairs;
+  r->layout = rot.layout;
+  r->n_axes = rot.n_axes;
+  r->inverse = rot.inverse ? 1 : 0;
+  int end = 0;
+  for (int a = 0; a < LVB_ROPE_MAX_AXES; ++a) {
+    end += a < rot.n_axes ? rot.sections[a] : 0;
+    r->sec_end[a] = end;
+  }
+  r->freqs = freqs;
+  r->pos = pos;
+  r->pos_axis = pos_axis;
+}
+
+}  // namespace
+
+int rope_launch(const lvb_rope_desc* d, const long long qs[3], const long long ks[3],
+                const long long qos[3], const long long kos[3], const void* Q, const void* K,
+                void* Qo, void* Ko, const int32_t* pos, const double* freqs, cudaStream_t stream,
+                DeviceState* dev) {
+  const char* op = "lvb_rope";
+  const int es = dtype_size(d->dtype);
+  RopeParams p = {};
+  fill_rot(&p.rot, d->rot, pos, freqs, d->pos_stride[0]);
+  p.pos_b = d->pos_stride[1];
+  p.pos_s = d->pos_stride[2];
+  p.S = (int)d->seq;
+  p.Hq = (int)d->heads_q;
+  p.Hkv = (int)d->heads_kv;
+  p.tasks = (int)d->head_dim * es / 32;
+  p.Q = (const uint8_t*)Q;
+  p.K = (const uint8_t*)K;
+  p.Qo = (uint8_t*)Qo;
+  p.Ko = (uint8_t*)Ko;
+  for (int i = 0; i < 3; ++i) {
+    p.q[i] = qs[i] * es;
+    p.k[i] = ks[i] * es;
+    p.qo[i] = qos[i] * es;
+    p.ko[i] = kos[i] * es;
+  }
+  const int heads = p.Hq + p.Hkv;
+  rot_grid(d->seq, d->batch, heads, p.tasks, kRotTokens, dev->sm_count, &p.n_tok, &p.heads_per_cta);
+  const dim3 grid((unsigned)((d->seq + p.n_tok - 1) / p.n_tok),
+                  (unsigned)((heads + p.heads_per_cta - 1) / p.heads_per_cta), (unsigned)d->batch);
+  const size_t smem = (size_t)p.n_tok * p.rot.pairs * sizeof(float2);
+  const bool halves = d->rot.layout == LVB_ROPE_HALVES;
+  if (d->dtype == LVB_F32) {
+    if (halves) rope_kernel<float, true><<<grid, kRotThreads, smem, stream>>>(p);
+    else rope_kernel<float, false><<<grid, kRotThreads, smem, stream>>>(p);
+  } else if (d->dtype == LVB_F16) {
+    if (halves) rope_kernel<__half, true><<<grid, kRotThreads, smem, stream>>>(p);
+    else rope_kernel<__half, false><<<grid, kRotThreads, smem, stream>>>(p);
+  } else {
+    if (halves) rope_kernel<__nv_bfloat16, true><<<grid, kRotThreads, smem, stream>>>(p);
+    else rope_kernel<__nv_bfloat16, false><<<grid, kRotThreads, smem, stream>>>(p);
+  }
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? LVB_OK : fail_cuda(e, op, "kernel launch");
+}
+
+int append_launch(const lvb_append_desc* d, const PagedLayout& lay, const long long ks[2],
+                  const long long vs[2], void* Kc, void* Vc, const void* K, const void* V,
+                  const void* Q, void* Qo, const int32_t* table, const int32_t* seq_lens,
+                  const int32_t* cu_q, const int32_t* pos, const double* freqs, cudaStream_t stream,
+                  DeviceState* dev) {
+  const char* op = "lvb_kv_append";
+  const lvb_paged_desc& g = d->paged;
+  AppendParams p = {};
+  fill_rot(&p.rot, d->rot, pos, freqs, d->pos_stride);
+  paged_seqs(&p.seqs, g, table, seq_lens, cu_q, nullptr, dev);
+  p.T = (int)g.tokens;
+  p.Hq = Q ? (int)g.heads_q : 0;
+  p.Hkv = (int)g.heads_kv;
+  p.tasks = (int)g.head_dim * 2 / 32;
+  p.K = (const uint8_t*)K;
+  p.V = (const uint8_t*)V;
+  p.Q = (const uint8_t*)Q;
+  p.Kc = (uint8_t*)Kc;
+  p.Vc = (uint8_t*)Vc;
+  p.Qo = (uint8_t*)Qo;
+  for (int i = 0; i < 2; ++i) {
+    p.k[i] = ks[i] * 2;
+    p.v[i] = vs[i] * 2;
+    p.q[i] = lay.q[i] * 2;
+    p.qo[i] = lay.o[i] * 2;
+  }
+  for (int i = 0; i < 3; ++i) {
+    p.kc[i] = lay.kc[i] * 2;
+    p.vc[i] = lay.vc[i] * 2;
+  }
+  const int heads = p.Hq + 2 * p.Hkv;
+  rot_grid(g.tokens, 1, heads, p.tasks, 4, dev->sm_count, &p.n_tok, &p.heads_per_cta);
+  const dim3 grid((unsigned)((g.tokens + p.n_tok - 1) / p.n_tok),
+                  (unsigned)((heads + p.heads_per_cta - 1) / p.heads_per_cta));
+  const size_t smem = (size_t)p.n_tok * p.rot.pairs * sizeof(float2);
+  const bool halves = d->rot.layout == LVB_ROPE_HALVES;
+  if (g.dtype == LVB_F16) {
+    if (halves) append_kernel<__half, true><<<grid, kRotThreads, smem, stream>>>(p);
+    else append_kernel<__half, false><<<grid, kRotThreads, smem, stream>>>(p);
+  } else {
+    if (halves) append_kernel<__nv_bfloat16, true><<<grid, kRotThreads, smem, stream>>>(p);
+    else append_kernel<__nv_bfloat16, false><<<grid, kRotThreads, smem, stream>>>(p);
+  }
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? LVB_OK : fail_cuda(e, op, "kernel launch");
+}
+
+}  // namespace lvb

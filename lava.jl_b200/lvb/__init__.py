@@ -11,6 +11,9 @@ library exactly the way the Julia host does (``ccall`` ≙ ``ctypes``):
   accumulation type of ``C``'s pair, layouts read from the tensors' strides (row-major
   ≙ ``Val(true)``, ``src/vocabulary/coopmat.jl:124-161``);
 * ``attention(O, Q, K, V; causal, scale)`` — the flash-attention forward (``attention!``);
+* ``rope(Qo, Q, pos, freqs; ...)`` — rotation of queries and keys by position, and its gradient;
+* ``kv_append(...)`` and ``attention_paged(...)`` — new tokens into a paged KV cache, and the
+  attention of ragged batches over it, with a prefix that all sequences share;
 * ``device_status()`` — the exception-flag check Lava's host does after a sync
   (``src/compiler/entry_wrapper.jl:199-216``).
 
@@ -50,6 +53,8 @@ EXPORTS = [
     "lvb_gemm_noalloc_status", "lvb_gemm_noalloc_selftest_wait_timeout",
     "lvb_gemm_ex_check", "lvb_gemm_ex", "lvb_pe_program_check",
     "lvb_attention_check", "lvb_attention_plan_for", "lvb_attention_fwd",
+    "lvb_rope_check", "lvb_rope", "lvb_kv_append_check", "lvb_kv_append",
+    "lvb_attention_paged_check", "lvb_attention_paged_plan_for", "lvb_attention_paged",
     "lvb_abi_version", "lvb_last_error", "lvb_status_string", "lvb_device_count",
     "lvb_set_device", "lvb_malloc", "lvb_free", "lvb_memcpy_htod", "lvb_memcpy_dtoh",
     "lvb_stream_create", "lvb_stream_destroy", "lvb_stream_synchronize",
@@ -133,6 +138,41 @@ class lvb_attn_desc(C.Structure):
                 ("v_stride", C.c_int64 * 3), ("o_stride", C.c_int64 * 3)]
 
 
+class lvb_rotation(C.Structure):
+    _fields_ = [("pairs", C.c_int32), ("layout", C.c_int32), ("n_axes", C.c_int32),
+                ("inverse", C.c_int32), ("sections", C.c_int32 * 4)]
+
+
+class lvb_rope_desc(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("reserved", C.c_int32),
+                ("batch", C.c_int64), ("heads_q", C.c_int64), ("heads_kv", C.c_int64),
+                ("seq", C.c_int64), ("head_dim", C.c_int64),
+                ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3),
+                ("qo_stride", C.c_int64 * 3), ("ko_stride", C.c_int64 * 3),
+                ("pos_stride", C.c_int64 * 3), ("rot", lvb_rotation)]
+
+
+class lvb_paged_desc(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("causal", C.c_int32),
+                ("batch", C.c_int64), ("heads_q", C.c_int64), ("heads_kv", C.c_int64),
+                ("head_dim", C.c_int64), ("tokens", C.c_int64), ("max_q", C.c_int64),
+                ("page_size", C.c_int64), ("num_pages", C.c_int64), ("table_width", C.c_int64),
+                ("table_stride", C.c_int64), ("prefix_len", C.c_int64),
+                ("kc_stride", C.c_int64 * 3), ("vc_stride", C.c_int64 * 3),
+                ("q_stride", C.c_int64 * 2), ("o_stride", C.c_int64 * 2),
+                ("scale", C.c_float), ("reserved", C.c_int32)]
+
+
+class lvb_append_desc(C.Structure):
+    _fields_ = [("paged", lvb_paged_desc), ("k_stride", C.c_int64 * 2),
+                ("v_stride", C.c_int64 * 2), ("pos_stride", C.c_int64), ("rot", lvb_rotation)]
+
+
+class lvb_paged_plan(C.Structure):
+    _fields_ = [("kernel", C.c_int32), ("splits", C.c_int32), ("prefix_splits", C.c_int32),
+                ("launches", C.c_int32), ("workspace_bytes", C.c_int64)]
+
+
 class lvb_comm_id(C.Structure):
     _fields_ = [("bytes", C.c_char * 128)]
 
@@ -160,6 +200,14 @@ def _load() -> C.CDLL:
         "lvb_attention_check": ([C.POINTER(lvb_attn_desc)], C.c_int),
         "lvb_attention_fwd": ([C.POINTER(lvb_attn_desc), P, P, P, P, P, P], C.c_int),
         "lvb_attention_plan_for": ([C.POINTER(lvb_attn_desc), C.c_int32, C.POINTER(lvb_attn_plan)], C.c_int),
+        "lvb_rope_check": ([C.POINTER(lvb_rope_desc)], C.c_int),
+        "lvb_rope": ([C.POINTER(lvb_rope_desc)] + [P] * 7, C.c_int),
+        "lvb_kv_append_check": ([C.POINTER(lvb_append_desc)], C.c_int),
+        "lvb_kv_append": ([C.POINTER(lvb_append_desc)] + [P] * 12, C.c_int),
+        "lvb_attention_paged_check": ([C.POINTER(lvb_paged_desc)], C.c_int),
+        "lvb_attention_paged_plan_for": ([C.POINTER(lvb_paged_desc), C.c_int32,
+                                          C.POINTER(lvb_paged_plan)], C.c_int),
+        "lvb_attention_paged": ([C.POINTER(lvb_paged_desc)] + [P] * 10, C.c_int),
         "lvb_abi_version": ([], C.c_int),
         "lvb_last_error": ([], C.c_char_p),
         "lvb_status_string": ([C.c_int], C.c_char_p),
@@ -588,6 +636,296 @@ def attention_plan(B, Hq, Hkv, Sq, Skv, D=128, dtype=BF16, causal=True,
     d.scale = float(D) ** -0.5
     p = lvb_attn_plan()
     check(lib.lvb_attention_plan_for(C.byref(d), sm_count, C.byref(p)))
+    return p
+
+
+# ---- position rotation, paged KV cache ---------------------------------------------------
+ROPE_LAYOUTS = {"halves": 0, "pairs": 1}
+PAGED_FLASH, PAGED_DECODE = 0, 1
+
+
+def _refuse(op, message, status=LVB_ERR_INVALID_ARG):
+    raise LavaError(status, f"{op}: {message}")
+
+
+def _rows(op, name, t, extents):
+    """Element strides of a tensor whose last dimension (head_dim) is contiguous; a dimension of
+    extent 1 gets one that any tensor could have (torch leaves it as it was)."""
+    if tuple(t.shape[:-1]) != tuple(extents):
+        _refuse(op, f"{name} has shape {tuple(t.shape)}, needs {tuple(extents)} rows")
+    D = t.shape[-1]
+    if D > 1 and t.stride(-1) != 1:
+        _refuse(op, f"{name}: head_dim must be contiguous", LVB_ERR_UNSUPPORTED)
+    return [t.stride(i) if n > 1 else D for i, n in enumerate(extents)]
+
+
+def _list_of(op, name, t, dtype, n=None):
+    """A contiguous 1-D list (int32 or float64), with at least n entries."""
+    if t.dtype != dtype or t.dim() != 1 or (t.shape[0] > 1 and t.stride(0) != 1):
+        _refuse(op, f"{name} must be a contiguous vector of {dtype}")
+    if n is not None and t.shape[0] < n:
+        _refuse(op, f"{name} has {t.shape[0]} entries, needs {n}")
+    return t
+
+
+def _on_current_device(op, tensors):
+    """Every tensor on the current CUDA device, where the kernels run."""
+    torch = _torch()
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            _refuse(op, f"{name} is not a CUDA tensor")
+        if t.device.index != torch.cuda.current_device():
+            _refuse(op, f"{name} is on {t.device}, the current device is "
+                        f"cuda:{torch.cuda.current_device()}")
+
+
+def _ptr(t):
+    return C.c_void_p(t.data_ptr() if t is not None else None)
+
+
+class PreparedCall:
+    """A call of the library described once and made many times: ``c = prepare_...(...)``, then
+    ``c()`` (torch's current stream) or ``c(stream)``: one foreign call. The tensors must stay
+    alive and keep their storage while the object is used (it holds them); what they hold may
+    change between calls, and a call captured into a CUDA graph reads it at the replay."""
+
+    def __init__(self, fn, desc, pointers, keep):
+        self.d = desc
+        self.keep = keep
+        self._fn = fn
+        self._args = (C.byref(desc), *pointers)
+        self._device = next(t for t in keep if t is not None).device.index
+
+    def __call__(self, stream=None):
+        s = (_torch()._C._cuda_getCurrentRawStream(self._device) if stream is None
+             else _stream_ptr(stream))
+        st = self._fn(*self._args, s)
+        if st:
+            check(st)
+
+
+def _rotation(op, freqs, sections, layout, inverse):
+    torch = _torch()
+    _list_of(op, "freqs", freqs, torch.float64)
+    if layout not in ROPE_LAYOUTS:
+        _refuse(op, f"layout {layout!r}: 'halves' or 'pairs'")
+    r = lvb_rotation()
+    r.pairs = freqs.shape[0]
+    r.layout = ROPE_LAYOUTS[layout]
+    r.inverse = int(bool(inverse))
+    sections = [r.pairs] if sections is None else [int(x) for x in sections]
+    if not 1 <= len(sections) <= 4:
+        _refuse(op, f"{len(sections)} sections: 1 to 4 axes")
+    r.n_axes = len(sections)
+    for i, x in enumerate(sections):
+        r.sections[i] = x
+    return r
+
+
+def prepare_rope(Qo, Q, pos, freqs, Ko=None, K=None, sections=None, layout="halves",
+                 inverse=False) -> PreparedCall:
+    """``rope`` described once (see ``PreparedCall``)."""
+    op = "lvb_rope"
+    if Q.dim() != 4 or Qo.shape != Q.shape:
+        _refuse(op, f"Q and Qo are [B][H][S][D] of one shape, got {tuple(Q.shape)} and {tuple(Qo.shape)}")
+    if (K is None) != (Ko is None):
+        _refuse(op, "K and Ko come together")
+    B, Hq, S, D = Q.shape
+    d = lvb_rope_desc()
+    d.dtype = dtype_of(Q)
+    d.batch, d.heads_q, d.seq, d.head_dim = B, Hq, S, D
+    d.rot = _rotation(op, freqs, sections, layout, inverse)
+    pairs = [("q_stride", "Q", Q), ("qo_stride", "Qo", Qo)]
+    if K is not None:
+        if K.dim() != 4 or (K.shape[0], K.shape[2], K.shape[3]) != (B, S, D) or Ko.shape != K.shape:
+            _refuse(op, f"K and Ko are [B][H][S][D] as Q is, got {tuple(K.shape)} and {tuple(Ko.shape)}")
+        d.heads_kv = K.shape[1]
+        pairs += [("k_stride", "K", K), ("ko_stride", "Ko", Ko)]
+    for field_, name, t in pairs:
+        if t.dtype != Q.dtype:
+            _refuse(op, "Q, K and their results must share a dtype", LVB_ERR_UNSUPPORTED)
+        getattr(d, field_)[:] = _rows(op, name, t, t.shape[:3])
+    if pos.dtype != _torch().int32:
+        _refuse(op, "pos must be int32")
+    p = pos if pos.dim() == 3 else pos.unsqueeze(0)
+    if p.dim() != 3 or p.shape[0] != d.rot.n_axes or p.shape[1] not in (1, B) or p.shape[2] != S:
+        _refuse(op, f"pos is [{B} or 1][{S}], or [{d.rot.n_axes}][{B} or 1][{S}] for several axes, "
+                    f"got {tuple(pos.shape)}")
+    d.pos_stride[:] = [p.stride(0), p.stride(1) if p.shape[1] > 1 else 0, p.stride(2)]
+    check(lib.lvb_rope_check(C.byref(d)))
+    _on_current_device(op, {"Qo": Qo, "Q": Q, "pos": pos, "freqs": freqs, "Ko": Ko, "K": K})
+    return PreparedCall(lib.lvb_rope, d, (_ptr(Q), _ptr(K), _ptr(Qo), _ptr(Ko), _ptr(pos), _ptr(freqs)),
+                        (Qo, Q, pos, freqs, Ko, K))
+
+
+def rope(Qo, Q, pos, freqs, Ko=None, K=None, sections=None, layout="halves", inverse=False,
+         stream=None):
+    """Rotate queries (and keys) by their positions: Q/Qo [B][Hq][S][D], K/Ko [B][Hkv][S][D] (fp16,
+    bf16 or fp32; a result may be its input). Pair i of a head turns by pos·freqs[i]: ``freqs``
+    float64 on the GPU, one per pair, its length the number of pairs (the rest of the head is
+    copied); ``pos`` int32 [B or 1][S], or [axes][B or 1][S] with ``sections`` the pairs of each
+    axis. ``layout``: pair i is elements i and i + pairs ("halves") or 2i and 2i + 1 ("pairs").
+    ``inverse`` turns back, which is also the gradient: dQ = rope(dQo, inverse)."""
+    prepare_rope(Qo, Q, pos, freqs, Ko, K, sections, layout, inverse)(stream)
+    return Qo if Ko is None else (Qo, Ko)
+
+
+def _paged_desc(op, Kc, Vc, block_table, seq_lens, cu_q, max_q, tokens, heads_q, prefix_len):
+    torch = _torch()
+    if Kc.dim() != 4 or Kc.shape != Vc.shape:
+        _refuse(op, f"the caches are [pages][page_size][Hkv][D] of one shape, got {tuple(Kc.shape)} "
+                    f"and {tuple(Vc.shape)}")
+    if Kc.dtype != Vc.dtype:
+        _refuse(op, "the caches must share a dtype", LVB_ERR_UNSUPPORTED)
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or (
+            block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        _refuse(op, "block_table is int32 [B][pages per sequence], its rows contiguous")
+    B = block_table.shape[0]
+    _list_of(op, "seq_lens", seq_lens, torch.int32)
+    if seq_lens.shape[0] != B:
+        _refuse(op, f"seq_lens has {seq_lens.shape[0]} entries, block_table {B} rows")
+    if cu_q is not None:
+        _list_of(op, "cu_q", cu_q, torch.int32)
+        if cu_q.shape[0] != B + 1:
+            _refuse(op, f"cu_q has {cu_q.shape[0]} entries, needs {B + 1}")
+        if max_q is None:
+            _refuse(op, "cu_q without max_q: the most query rows of a sequence, known on the host")
+    else:
+        if max_q is None:
+            max_q = tokens // B if B else 0
+        if B * max_q != tokens:
+            _refuse(op, f"{tokens} rows for {B} sequences of {max_q}: pass cu_q")
+    d = lvb_paged_desc()
+    d.dtype = dtype_of(Kc)
+    d.batch, d.heads_q, d.heads_kv, d.head_dim = B, heads_q, Kc.shape[2], Kc.shape[3]
+    d.tokens, d.max_q = tokens, int(max_q)
+    d.page_size, d.num_pages = Kc.shape[1], Kc.shape[0]
+    d.table_width = block_table.shape[1]
+    d.table_stride = block_table.stride(0) if B > 1 else block_table.shape[1]
+    d.prefix_len = int(prefix_len)
+    d.scale = float(Kc.shape[3]) ** -0.5
+    d.kc_stride[:] = _rows(op, "Kc", Kc, Kc.shape[:3])
+    d.vc_stride[:] = _rows(op, "Vc", Vc, Vc.shape[:3])
+    return d
+
+
+def prepare_kv_append(Kc, Vc, K, V, block_table, seq_lens, cu_q=None, max_q=None, Qo=None, Q=None,
+                      pos=None, freqs=None, sections=None, layout="halves",
+                      prefix_len=0) -> PreparedCall:
+    """``kv_append`` described once (see ``PreparedCall``)."""
+    op = "lvb_kv_append"
+    torch = _torch()
+    if (Q is None) != (Qo is None):
+        _refuse(op, "Q and Qo come together")
+    if K.dim() != 3:
+        _refuse(op, f"K and V are [tokens][Hkv][D], got {tuple(K.shape)}")
+    T = K.shape[0]
+    heads_q = Q.shape[1] if Q is not None and Q.dim() == 3 else 0
+    d = lvb_append_desc()
+    d.paged = _paged_desc(op, Kc, Vc, block_table, seq_lens, cu_q, max_q, T, heads_q, prefix_len)
+    Hkv, D = Kc.shape[2], Kc.shape[3]
+    for field_, name, t in (("k_stride", "K", K), ("v_stride", "V", V)):
+        if tuple(t.shape) != (T, Hkv, D) or t.dtype != Kc.dtype:
+            _refuse(op, f"{name} must be [{T}][{Hkv}][{D}] of the cache's dtype")
+        getattr(d, field_)[:] = _rows(op, name, t, (T, Hkv))
+    if Q is not None:
+        for field_, name, t in (("q_stride", "Q", Q), ("o_stride", "Qo", Qo)):
+            if t.dim() != 3 or tuple(t.shape) != (T, heads_q, D) or t.dtype != Kc.dtype:
+                _refuse(op, f"{name} must be [{T}][Hq][{D}] of the cache's dtype")
+            getattr(d.paged, field_)[:] = _rows(op, name, t, (T, heads_q))
+    if freqs is not None:
+        d.rot = _rotation(op, freqs, sections, layout, False)
+        if pos is not None:
+            p = pos if pos.dim() == 2 else pos.unsqueeze(0)
+            if (pos.dtype != torch.int32 or tuple(p.shape) != (d.rot.n_axes, T)
+                    or (T > 1 and p.stride(1) != 1)):
+                _refuse(op, f"pos is int32 [{T}], or [{d.rot.n_axes}][{T}] for several axes, "
+                            "its rows contiguous")
+            d.pos_stride = p.stride(0)
+        elif d.rot.n_axes != 1:
+            _refuse(op, "several axes need pos")
+    elif pos is not None or Q is not None:
+        _refuse(op, "pos or Q without freqs")
+    check(lib.lvb_kv_append_check(C.byref(d)))
+    keep = (Kc, Vc, K, V, Q, Qo, block_table, seq_lens, cu_q, pos, freqs)
+    _on_current_device(op, dict(zip(("Kc", "Vc", "K", "V", "Q", "Qo", "block_table", "seq_lens",
+                                     "cu_q", "pos", "freqs"), keep)))
+    return PreparedCall(lib.lvb_kv_append, d, tuple(_ptr(t) for t in keep), keep)
+
+
+def kv_append(Kc, Vc, K, V, block_table, seq_lens, cu_q=None, max_q=None, Qo=None, Q=None, pos=None,
+              freqs=None, sections=None, layout="halves", prefix_len=0, stream=None):
+    """Write the new tokens' keys and values into a paged cache. Kc/Vc [pages][page_size][Hkv][D]
+    (any strides), K/V [tokens][Hkv][D] packed by sequence: sequence b has rows cu_q[b] ..
+    cu_q[b+1]-1 (at most ``max_q``; without ``cu_q`` all have the same number) and they become its
+    last places, up to seq_lens[b] - 1 (``seq_lens`` counts them), place p in slot p % page_size of
+    page block_table[b][p // page_size]. With ``freqs`` the keys are rotated on the way (as
+    ``rope``; ``pos`` int32 [tokens] or [axes][tokens], by default prefix_len + place), and
+    ``Q`` [tokens][Hq][D] beside them into ``Qo`` (which may be Q). A row whose place is negative (an
+    idle entry of a padded batch) is left out. Lists are int32 on the GPU and read there: what they
+    get wrong is reported by ``device_status`` (see include/lvb.h)."""
+    prepare_kv_append(Kc, Vc, K, V, block_table, seq_lens, cu_q, max_q, Qo, Q, pos, freqs, sections,
+                      layout, prefix_len)(stream)
+    return Kc, Vc
+
+
+def prepare_attention_paged(O, Q, Kc, Vc, block_table, seq_lens, cu_q=None, max_q=None, causal=True,
+                            scale=None, lse=None, prefix_table=None, prefix_len=0) -> PreparedCall:
+    """``attention_paged`` described once (see ``PreparedCall``)."""
+    op = "lvb_attention_paged"
+    torch = _torch()
+    if Q.dim() != 3 or O.shape != Q.shape or Q.shape[2] != Kc.shape[-1]:
+        _refuse(op, f"Q and O are [tokens][Hq][D], got {tuple(Q.shape)} and {tuple(O.shape)}")
+    T, Hq, _ = Q.shape
+    d = _paged_desc(op, Kc, Vc, block_table, seq_lens, cu_q, max_q, T, Hq, prefix_len)
+    if not Q.dtype == O.dtype == Kc.dtype:
+        _refuse(op, "Q, O and the caches must share a dtype", LVB_ERR_UNSUPPORTED)
+    d.causal = int(bool(causal))
+    if scale is not None:
+        d.scale = float(scale)
+    d.q_stride[:] = _rows(op, "Q", Q, (T, Hq))
+    d.o_stride[:] = _rows(op, "O", O, (T, Hq))
+    if d.prefix_len > 0:
+        if prefix_table is None:
+            _refuse(op, "prefix_len without prefix_table")
+        _list_of(op, "prefix_table", prefix_table, torch.int32,
+                 -(-d.prefix_len // max(1, d.page_size)))
+    if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (T, Hq)
+                            or not lse.is_contiguous()):
+        _refuse(op, f"lse must be contiguous float32 [{T}][{Hq}]")
+    check(lib.lvb_attention_paged_check(C.byref(d)))
+    keep = (Q, Kc, Vc, block_table, seq_lens, cu_q, prefix_table, O, lse)
+    _on_current_device(op, dict(zip(("Q", "Kc", "Vc", "block_table", "seq_lens", "cu_q",
+                                     "prefix_table", "O", "lse"), keep)))
+    return PreparedCall(lib.lvb_attention_paged, d, tuple(_ptr(t) for t in keep), keep)
+
+
+def attention_paged(O, Q, Kc, Vc, block_table, seq_lens, cu_q=None, max_q=None, causal=True,
+                    scale=None, lse=None, prefix_table=None, prefix_len=0, stream=None):
+    """Attention of packed queries over a paged cache: Q/O [tokens][Hq][D], the caches, the table and
+    the lists as in ``kv_append`` (seq_lens counts the queries' own tokens). A query at place p
+    sees places 0..p (``causal``; else all of its sequence's), and before them the ``prefix_len``
+    keys whose pages ``prefix_table`` (int32) lists, which all sequences share and the kernel reads
+    once for all when there are at most 32 query rows per KV head and sequence. Optional ``lse``
+    float32 [tokens][Hq]. Rows that see no key give O = 0 and lse = -inf; rows behind cu_q[B] are
+    left as they were."""
+    prepare_attention_paged(O, Q, Kc, Vc, block_table, seq_lens, cu_q, max_q, causal, scale, lse,
+                            prefix_table, prefix_len)(stream)
+    return O
+
+
+def attention_paged_plan(B, Hq, Hkv, tokens, max_q, page_size, table_width, D=128, dtype=BF16,
+                         causal=True, prefix_len=0, sm_count=148) -> lvb_paged_plan:
+    """How lvb_attention_paged runs a call of these extents (host only, no GPU)."""
+    d = lvb_paged_desc()
+    d.dtype, d.causal = dtype, int(bool(causal))
+    d.batch, d.heads_q, d.heads_kv, d.head_dim = B, Hq, Hkv, D
+    d.tokens, d.max_q, d.page_size, d.num_pages = tokens, max_q, page_size, 1
+    d.table_width, d.prefix_len, d.scale = table_width, prefix_len, float(D) ** -0.5
+    p = lvb_paged_plan()
+    check(lib.lvb_attention_paged_plan_for(C.byref(d), sm_count, C.byref(p)))
     return p
 
 
