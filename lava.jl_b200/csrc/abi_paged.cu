@@ -122,6 +122,9 @@ int check_paged(const char* op, const lvb_paged_desc* d) {
       d->batch > INT32_MAX || d->heads_q > 65535 || d->batch * d->heads_kv > INT32_MAX ||
       (d->batch > 0 && d->max_q > INT32_MAX / d->batch))
     return fail(LVB_ERR_UNSUPPORTED, op, "extent above 2^31-1", "split the batch");
+  // (key blocks of all items together: the decoding kernel counts them in 32 bits)
+  if (d->batch * d->heads_kv > INT32_MAX / 2 / (d->table_width * d->page_size / 128 + 2))
+    return fail(LVB_ERR_UNSUPPORTED, op, "more than 2^30 key blocks in the tables", "split the batch");
   const int64_t cache[3] = {d->num_pages, d->page_size, d->heads_kv};
   const int64_t rows[2] = {d->tokens, d->heads_q};
   int st;
@@ -361,7 +364,7 @@ int lvb_attention_paged(const lvb_paged_desc* d, const void* Q, const void* Kc, 
     mp.dec_rows = dw.rows;
     mp.dec_slots = dw.slots;
     mp.dec_ctas = dw.ctas;
-    if (st == LVB_OK) st = merge_launch(mp, (int)d->head_dim, bf16, s);
+    if (st == LVB_OK) st = merge_launch(mp, (int)d->head_dim, bf16, s, dev);
   } else {
     const int parts = kFlashOwn | (d->prefix_len ? kFlashPrefix : 0);
     st = paged_flash_launch(d, lay, mp.seqs, Q, Kc, Vc, O, lse, parts, pl.splits, ws, &fw, s, dev);
@@ -370,7 +373,7 @@ int lvb_attention_paged(const lvb_paged_desc* d, const void* Q, const void* Kc, 
       mp.tile_ml = fw.tile_ml;
       mp.tile_splits = pl.splits;
       mp.pairs_per_seq = (int)((d->max_q + 2 * mp.ppt - 1) / (2 * mp.ppt));
-      st = merge_launch(mp, (int)d->head_dim, bf16, s);
+      st = merge_launch(mp, (int)d->head_dim, bf16, s, dev);
     }
   }
   e = cudaFreeAsync(ws, s);

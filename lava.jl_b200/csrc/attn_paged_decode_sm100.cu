@@ -9,17 +9,20 @@
 // product (the tensor core takes both operands in one 16-bit type); l sums the unrounded p.
 //
 //   * the 128-key blocks of all (sequence, KV head) items, one after the other, are dealt to the
-//     CTAs in equal contiguous runs, so lengths from one key to the whole cache load the SMs
-//     evenly. The lengths are on the device: every CTA sums the block counts itself. An item that
-//     a run boundary cuts leaves pieces (O, m, l in 32 bits) in the workspace, at most two per
-//     CTA, and the join kernel adds them in a fixed order; an item inside a run stores its result;
-//   * 192 threads: warp 4 brings Q and the K and V blocks (a box of slots per page and lane)
-//     through a ring that runs ahead across items and publishes the items; warp 5 issues the
-//     products (QK_j, then PV_{j-1}); warps 0-3 do the softmax (thread = key) and the epilogue
-//     (thread = head-dim element);
+//     CTAs in equal contiguous runs (an item also counts kItemCost blocks for its start and end), so
+//     lengths from one key to the whole cache load the SMs evenly. The lengths are on the device:
+//     every CTA sums the block counts itself. An item that a run boundary cuts leaves pieces (O, m,
+//     l in 32 bits) in the workspace, at most two per CTA, and the join kernel adds them in a
+//     fixed order; an item inside a run stores its result;
+//   * 352 threads: two softmax warpgroups take the blocks in turn, each with its own S and P
+//     buffer, maxima, sums and O accumulator (thread = key for Sᵀ, = head-dim element for Oᵀ), so
+//     one's chain of waits runs beside the other's; the one with an item's last block joins the
+//     other's O (read from TMEM), m and l to its own. A TMA warp brings Q and the K
+//     and V blocks (a box of slots per page and lane) through a ring that runs ahead across items
+//     and publishes the items; one warp issues the Q·Kᵀ products, one the P·V products;
 //   * m of a row moves only when a score exceeds it by 2^8 (p stays <= 256): a block whose scores
-//     all stay below needs no row maximum, only one vote over the 128 threads. In fp16 the
-//     exponent is shifted by 2^6, away from the subnormals (p <= 2^14).
+//     all stay below needs no row maximum, only one vote over the warpgroup. In fp16 the exponent
+//     is shifted by 2^6, away from the subnormals (p <= 2^14).
 #include <algorithm>
 #include <cmath>
 
@@ -29,10 +32,13 @@ namespace lvb {
 
 namespace {
 
-constexpr int kThreads = 192;
-constexpr int kTmaWarp = 4;
-constexpr int kMmaWarp = 5;
-constexpr int kQueue = 4;                  // items published ahead
+constexpr int kThreads = 352;
+// Warps 0-3 and 4-7: the softmax warpgroups.
+constexpr int kTmaWarp = 8;
+constexpr int kQkWarp = 9;
+constexpr int kPvWarp = 10;
+constexpr int kQueue = 8;                  // items published ahead
+constexpr int kItemCost = 1;               // blocks that an item's start and end count for
 constexpr int kChunk = 128 * 128;          // one 64-element chunk of a 128-key block
 constexpr float kLazy = 8.f;               // log2 units a score may exceed the reference maximum
 
@@ -53,11 +59,13 @@ template <int D, int NR>
 struct Cfg {
   static constexpr int kCh = D / 64;
   static constexpr int kBlock = kCh * kChunk;
-  static constexpr int kRing = D == 128 ? 6 : 12;
+  static constexpr int kRing = D == 64 ? 12 : NR == 16 ? 6 : 5;
   static constexpr int kQ = kCh * NR * 128;            // Q of an item
   static constexpr int kP = 2 * NR * 128;              // P of a block: two 64-key chunks
-  static constexpr int kTmemCols = NR == 16 ? 64 : 128;
-  static constexpr int kSmem = kRing * kBlock + 2 * kQ + 2 * kP + 4 * NR * 4 + 1024 + 1024;
+  static constexpr int kTmemCols = NR == 16 ? 128 : 256;   // S and two O per warpgroup
+  static constexpr int kSmem =
+      kRing * kBlock + 2 * kQ + 2 * kP + 2 * 4 * NR * 4 + 2 * NR * 8 + 1536 +
+      kThreads * 12 + 1024;
 };
 
 // What the roles need of an item (a run of key blocks of one sequence and KV head).
@@ -99,18 +107,25 @@ __device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity, uint6
   }
 }
 
-// Whether `pred` holds for any of the 128 softmax threads (barrier 1).
-__device__ __forceinline__ bool vote_any(bool pred) {
+// Whether `pred` holds for any of the warpgroup's 128 threads (named barrier `id`).
+__device__ __forceinline__ bool vote_any(int id, bool pred) {
   uint32_t any;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.or.pred q, 1, 128, p;\n\t"
+      "setp.ne.u32 p, %2, 0;\n\t"
+      "barrier.cta.red.or.pred q, %1, 128, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(any)
-      : "r"((uint32_t)pred)
+      : "r"(id), "r"((uint32_t)pred)
       : "memory");
   return any != 0;
+}
+
+// A single thread's wait that tests before it suspends.
+__device__ __forceinline__ bool wait_soon(uint64_t* bar, uint32_t parity, const WaitGuard& g,
+                                          int where, int detail) {
+  if (bar_test_wait(smem_u32(bar), parity)) return true;
+  return wait_bar(bar, parity, g, where, detail);
 }
 
 // Key blocks of a sequence (0 when it has no query rows).
@@ -136,25 +151,30 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* sRing = smem;                                  // [R][D/64 chunks][128 keys][128 B]
   uint8_t* sQ = sRing + R * C::kBlock;                    // [2][D/64 chunks][NR rows][128 B]
   uint8_t* sP = sQ + 2 * C::kQ;                           // [2][2 chunks][NR rows][128 B]
-  float* sRed = reinterpret_cast<float*>(sP + 2 * C::kP); // [4 warps][NR]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sRed + 4 * NR);
+  float* sXml = reinterpret_cast<float*>(sP + 2 * C::kP); // [2 warpgroups][NR][2] deposited m, l
+  float* sRed = sXml + 2 * NR * 2;                        // [2 warpgroups][4 warps][NR]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sRed + 2 * 4 * NR);
   uint64_t* kv_full = bars;              // [R]
   uint64_t* kv_empty = kv_full + R;      // [R]
   uint64_t* q_full = kv_empty + R;       // [2]
   uint64_t* q_empty = q_full + 2;        // [2]
-  uint64_t* s_full = q_empty + 2;        // [2]
-  uint64_t* s_empty = s_full + 2;        // [2] (128 arrivals)
-  uint64_t* p_full = s_empty + 2;        // [2] (128 arrivals)
+  uint64_t* s_full = q_empty + 2;        // [2] per warpgroup, as all below
+  uint64_t* s_empty = s_full + 2;        // [2] (4 warps)
+  uint64_t* p_full = s_empty + 2;        // [2] (4 warps)
   uint64_t* p_empty = p_full + 2;        // [2]
-  uint64_t* o_full = p_empty + 2;        // an item's last PV done
-  uint64_t* o_empty = o_full + 1;        // its epilogue has read Oᵀ (128 arrivals)
-  uint64_t* i_full = o_empty + 1;        // [kQueue] item published
-  uint64_t* i_empty = i_full + kQueue;   // [kQueue] read by the MMA warp and four softmax warps
+  uint64_t* o_full = p_empty + 2;        // [2][2] an item's last PV done
+  uint64_t* o_empty = o_full + 4;        // [2][2] its Oᵀ read (4 warps)
+  uint64_t* x_full = o_empty + 4;        // [2] the warpgroup's m and l deposited (4 warps)
+  uint64_t* x_empty = x_full + 2;        // [2] they are read (4 warps of the other)
+  uint64_t* i_full = x_empty + 2;        // [kQueue] item published
+  uint64_t* i_empty = i_full + kQueue;   // [kQueue] read by the two MMA warps and 8 softmax warps
   uint64_t* drain = i_empty + kQueue;
   Item* items = reinterpret_cast<Item*>(drain + 1);       // [kQueue]
-  long long* sScan = reinterpret_cast<long long*>(items + kQueue);   // [8]: warp sums, then
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sScan + 8);      // the start's offset and b
+  int* sScan = reinterpret_cast<int*>(items + kQueue);    // [12]: the warps' sums
+  int* sStart = sScan + 12;                               // the run's sequence and its offset
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sStart + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  SeqInfo* sSeq = reinterpret_cast<SeqInfo*>(tmem_slot + 2);   // [kThreads]
 
   const uint32_t warp = warp_id();
   const uint32_t lane = lane_id();
@@ -169,60 +189,79 @@ __global__ void __launch_bounds__(kThreads, 1)
       bar_init(&q_full[i], 1);
       bar_init(&q_empty[i], 1);
       bar_init(&s_full[i], 1);
-      bar_init(&s_empty[i], 128);
-      bar_init(&p_full[i], 128);
+      bar_init(&s_empty[i], 4);
+      bar_init(&p_full[i], 4);
       bar_init(&p_empty[i], 1);
+      bar_init(&x_full[i], 4);
+      bar_init(&x_empty[i], 4);
     }
-    bar_init(o_full, 1);
-    bar_init(o_empty, 128);
+    for (int i = 0; i < 4; ++i) {
+      bar_init(&o_full[i], 1);
+      bar_init(&o_empty[i], 4);
+    }
     for (int i = 0; i < kQueue; ++i) {
       bar_init(&i_full[i], 1);
-      bar_init(&i_empty[i], 5);
+      bar_init(&i_empty[i], 10);
     }
-    bar_init(drain, 1);
+    bar_init(drain, 2);
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == kMmaWarp) {
+  if (warp == kQkWarp) {
     tmem_alloc(tmem_slot, C::kTmemCols);
     tmem_relinquish();
   }
+  if (warp == kTmaWarp && lane == 0) {
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+
+  // The setup above may run while the stream's previous kernel ends; the join kernel, which reads
+  // this one's results after its own wait, may be scheduled from here on.
+  griddep_wait();
+  griddep_launch_dependents();
 
   // ---------------- this CTA's run of blocks ----------------
-  // Thread i sums the blocks of sequences [i·per, (i+1)·per); a scan over the threads gives the
-  // total and the thread whose sequences hold the run's first block.
+  // Thread i sums the costs of sequences [i·per, (i+1)·per); a scan over the threads gives the
+  // total and the thread whose sequences hold the run's first unit. An item's units are its
+  // kItemCost, then its blocks.
   const int batch = p.seqs.batch;
   const int per = (batch + kThreads - 1) / kThreads;
   const int sb0 = min((int)threadIdx.x * per, batch), sb1 = min(sb0 + per, batch);
-  long long mine = 0;
-  for (int b = sb0; b < sb1; ++b) mine += blocks_of(seq_info(p.seqs, b));
-  mine *= p.Hkv;
-  long long incl = mine;
+  auto units_of = [&](int nb) -> int { return nb ? (nb + kItemCost) * p.Hkv : 0; };
+  const bool kept = batch <= kThreads;     // one sequence per thread: the producer reads them here
+  int mine = 0;
+  for (int b = sb0; b < sb1; ++b) {
+    const SeqInfo s = seq_info(p.seqs, b);
+    if (kept) sSeq[b] = s;
+    mine += units_of(blocks_of(s));
+  }
+  int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+    const int v = __shfl_up_sync(0xffffffffu, incl, o);
     if ((int)lane >= o) incl += v;
   }
   if (lane == 31) sScan[warp] = incl;
   __syncthreads();
-  long long before = 0, total = 0;
+  int before = 0, total = 0;
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) {
     if (w < (int)warp) before += sScan[w];
     total += sScan[w];
   }
-  const long long share = max(1LL, (total + G - 1) / G);
-  const long long u0 = blockIdx.x * share;
-  const long long u1 = min(u0 + share, total);
-  const long long first = before + incl - mine;
-  __syncthreads();
+  const int share = max(1, (total + G - 1) / G);
+  const int u0 = min((int)blockIdx.x, total / share + 1) * share;   // (no product above 2·total + share)
+  const int u1 = min(u0 + share, total);
+  const int first = before + incl - mine;
   if (u0 < total && u0 >= first && u0 < first + mine) {
-    long long off = first;
+    int off = first;
     for (int b = sb0; b < sb1; ++b) {
-      const long long n = (long long)blocks_of(seq_info(p.seqs, b)) * p.Hkv;
+      const int n = kept ? mine : units_of(blocks_of(seq_info(p.seqs, b)));
       if (u0 < off + n) {
-        sScan[0] = off;
-        sScan[1] = b;
+        sStart[0] = off;
+        sStart[1] = b;
         break;
       }
       off += n;
@@ -232,99 +271,131 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const uint32_t tS = tmem;                 // Sᵀ buffers: columns [0, NR) and [NR, 2NR)
-  const uint32_t tO = tmem + 2 * NR;        // Oᵀ: columns [2NR, 3NR)
+  // columns: S of warpgroup w at w·NR, its O buffers at (2 + 2w + ob)·NR
   const WaitGuard g{p.seqs.status, abort_flag, p.timeout_ns};
 
   if (warp == kTmaWarp) {
     // ---------------- producer: items, Q, K and V blocks ----------------
-    if (lane == 0) {
-      tma_prefetch_desc(&tmQ);
-      tma_prefetch_desc(&tmK);
-      tma_prefetch_desc(&tmV);
-    }
     const BlockLane<D> bl((int)lane, p.box);
     int n = 0;        // ring slots filled
     int it = 0;       // items published
     bool ok = true;
-    long long u = u0;
     int base = 0;     // the lanes hold sequences base .. base+31
     SeqInfo sq{0, 0, 0};
     int nb_lane = 0;
-    long long off = 0;
+    int off = 0;      // first unit of sequence b
     int b = 0;
-    if (u < u1) {
-      off = sScan[0];
-      b = (int)sScan[1];
-      base = b & ~31;
-      if (base + (int)lane < batch) sq = seq_info(p.seqs, base + lane);
+    auto fetch = [&]() {
+      sq = SeqInfo{0, 0, 0};
+      if (base + (int)lane < batch) sq = kept ? sSeq[base + lane] : seq_info(p.seqs, base + lane);
       nb_lane = blocks_of(sq);
-    }
-    while (u < u1 && ok) {
-      // the sequence of block u: the next one with blocks once the current one is passed
-      int nb = __shfl_sync(0xffffffffu, nb_lane, b - base);
-      if (u >= off + (long long)nb * p.Hkv) {
-        off += (long long)nb * p.Hkv;
-        int from = b + 1 - base;
-        while (true) {
-          const unsigned some = from < 32 ? __ballot_sync(0xffffffffu, nb_lane > 0) >> from : 0u;
-          if (some) {
-            b = base + from + __ffs(some) - 1;
-            break;
+    };
+    // The item at or after unit u, or false when the run has no further block.
+    struct Next {
+      Item im;
+      const int* row;
+      int id, nb, c1;
+      int end;            // first unit behind it
+    };
+    auto next_item = [&](int u, Next& x) -> bool {
+      while (u < u1) {
+        int nb = __shfl_sync(0xffffffffu, nb_lane, b - base);
+        if (u >= off + units_of(nb)) {
+          // the next sequence with blocks (u < total: there is one)
+          off += units_of(nb);
+          int from = b + 1 - base;
+          while (true) {
+            const unsigned some = from < 32 ? __ballot_sync(0xffffffffu, nb_lane > 0) >> from : 0u;
+            if (some) {
+              b = base + from + __ffs(some) - 1;
+              break;
+            }
+            base += 32;
+            from = 0;
+            fetch();
           }
-          base += 32;      // u < total: a later sequence has blocks
-          from = 0;
-          sq = SeqInfo{0, 0, 0};
-          if (base + (int)lane < batch) sq = seq_info(p.seqs, base + lane);
-          nb_lane = blocks_of(sq);
+          nb = __shfl_sync(0xffffffffu, nb_lane, b - base);
         }
-        nb = __shfl_sync(0xffffffffu, nb_lane, b - base);
+        const int hk = (u - off) / (nb + kItemCost);
+        const int o_item = off + hk * (nb + kItemCost) + kItemCost;   // its first block
+        const int kb0 = max(0, u - o_item);
+        const int kb1 = min(nb, u1 - o_item);
+        x.end = o_item + nb;
+        if (kb1 <= kb0) {     // the run ends within the item's own cost
+          u = x.end;
+          continue;
+        }
+        x.im.hk = hk;
+        x.im.kb0 = kb0;
+        x.im.nblk = kb1 - kb0;
+        x.im.len = __shfl_sync(0xffffffffu, sq.len, b - base);
+        x.im.qlen = __shfl_sync(0xffffffffu, sq.qlen, b - base);
+        x.im.tok0 = __shfl_sync(0xffffffffu, sq.tok0, b - base);
+        x.im.last = 0;
+        x.nb = nb;
+        x.id = b * p.Hkv + hk;
+        x.row = p.seqs.table + b * p.seqs.table_stride;
+        const int c0 = o_item / share;
+        x.c1 = (o_item + nb - 1) / share;
+        x.im.slot = -1;
+        // an item that only this CTA works on is whole; of one that begins in an earlier CTA this
+        // is the run's first piece, of the other kind its last
+        if (x.c1 > c0) x.im.slot = 2 * blockIdx.x + ((int)blockIdx.x == c0 ? 1 : 0);
+        else if (p.keep_parts) x.im.slot = 2 * G + x.id;
+        return true;
       }
-      const int len = __shfl_sync(0xffffffffu, sq.len, b - base);
-      const int qlen = __shfl_sync(0xffffffffu, sq.qlen, b - base);
-      const int tok0 = __shfl_sync(0xffffffffu, sq.tok0, b - base);
-      const int hk = (int)((u - off) / nb);
-      const long long o_item = off + (long long)hk * nb;   // the item's first block
-      const int kb0 = (int)(u - o_item);
-      const int nblk = (int)min((long long)(nb - kb0), u1 - u);
-      const bool whole = nblk == nb;
-      const int id = b * p.Hkv + hk;
-      int slot = -1;
-      if (!whole) slot = 2 * blockIdx.x + (u == u0 ? 0 : 1);
-      else if (p.keep_parts) slot = 2 * G + id;
-      if (kb0 == 0 && lane == 0) {
-        const int c1 = (int)((o_item + nb - 1) / share);
-        p.tab[id] = make_int4(slot, blockIdx.x + 1, c1,
-                              whole && !p.keep_parts ? kItemDone : kItemPieces);
-      }
+      return false;
+    };
+    Next cur, nx;
+    bool have = false;
+    BoxAt at{0, 0, false};
+    if (u0 < u1) {
+      off = sStart[0];
+      b = sStart[1];
+      base = b & ~31;
+      fetch();
+      have = next_item(u0, cur);
+      if (have) at = box_at(bl, cur.row, cur.im.kb0, cur.im.len, p.box, p.seqs);
+    }
+    while (have && ok) {
+      const Item im = cur.im;
+      if (im.kb0 == 0 && lane == 0)
+        p.tab[cur.id] = make_int4(im.slot, blockIdx.x + 1, cur.c1, im.slot < 0 ? kItemDone : kItemPieces);
       const int qi = it % kQueue;
-      if (!wait_bar_warp(&i_empty[qi], (uint32_t)((it / kQueue) & 1) ^ 1, g, 70, it)) { ok = false; break; }
+      if (!wait_soon_warp(&i_empty[qi], (uint32_t)((it / kQueue) & 1) ^ 1, g, 70, it)) { ok = false; break; }
       if (lane == 0) {
-        items[qi] = Item{hk, kb0, nblk, len, qlen, tok0, slot, 0};
+        items[qi] = im;
         bar_arrive(&i_full[qi]);
       }
       const int qb = it & 1;
-      if (!wait_bar_warp(&q_empty[qb], (uint32_t)((it >> 1) & 1) ^ 1, g, 51, it)) { ok = false; break; }
+      if (!wait_soon_warp(&q_empty[qb], (uint32_t)((it >> 1) & 1) ^ 1, g, 51, it)) { ok = false; break; }
       if (lane == 0) {
         bar_arrive_expect_tx(&q_full[qb], C::kCh * p.nrows * 128);
         for (int c = 0; c < C::kCh; ++c)
-          tma_load_3d(sQ + qb * C::kQ + c * NR * 128, &tmQ, c * 64, hk * p.group, tok0, &q_full[qb]);
+          tma_load_3d(sQ + qb * C::kQ + c * NR * 128, &tmQ, c * 64, im.hk * p.group, im.tok0, &q_full[qb]);
       }
+      __syncwarp();
       ++it;
-      const int* row = p.seqs.table + b * p.seqs.table_stride;
-      BoxAt at = box_at(bl, row, kb0, len, p.box, p.seqs);
-      for (int kb = kb0; kb < kb0 + nblk && ok; ++kb) {
-        // the next block's page numbers are on their way while this one's slots are waited for
-        BoxAt next{-1, 0};
-        if (kb + 1 < kb0 + nblk) next = box_at(bl, row, kb + 1, len, p.box, p.seqs);
+      bool more = false;
+      for (int kb = im.kb0; kb < im.kb0 + im.nblk && ok; ++kb) {
+        // the next block's page numbers (of this item or the next) are on their way while this
+        // one's slots are waited for
+        BoxAt next{0, 0, false};
+        if (kb + 1 < im.kb0 + im.nblk) {
+          next = box_at(bl, cur.row, kb + 1, im.len, p.box, p.seqs);
+        } else {
+          more = next_item(cur.end, nx);
+          if (more) next = box_at(bl, nx.row, nx.im.kb0, nx.im.len, p.box, p.seqs);
+        }
         for (int v = 0; v < 2; ++v, ++n) {
           const int s = n % R;
-          if (!wait_bar_warp(&kv_empty[s], (uint32_t)((n / R) & 1) ^ 1, g, 52, n)) { ok = false; break; }
-          load_block<D>(sRing + s * C::kBlock, v ? &tmV : &tmK, bl, at, p.box, hk, &kv_full[s]);
+          if (!wait_soon_warp(&kv_empty[s], (uint32_t)((n / R) & 1) ^ 1, g, 52, n)) { ok = false; break; }
+          load_block<D>(sRing + s * C::kBlock, v ? &tmV : &tmK, bl, at, p.box, im.hk, &kv_full[s], p.seqs);
         }
         at = next;
       }
-      u += nblk;
+      cur = nx;
+      have = more;
     }
     if (ok) {
       const int qi = it % kQueue;
@@ -340,13 +411,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         drain_wait(&q_full[i & 1], (uint32_t)((i >> 1) & 1), p.timeout_ns);
     }
     __syncwarp();
-  } else if (warp == kMmaWarp) {
-    // ---------------- MMA issuer: the warp waits, one elected lane issues ----------------
-    const uint32_t r_base = smem_u32(sRing);
-    const uint32_t q_base = smem_u32(sQ);
-    const uint32_t p_base = smem_u32(sP);
-    int n_ring = 0;   // ring slots before this item
+  } else if (warp == kQkWarp || warp == kPvWarp) {
+    // ---------------- MMA issuers: the warp waits, one elected lane issues ----------------
+    const uint64_t r_desc = sdesc_sw128(smem_u32(sRing), 16, 1024);        // K_j, K-major
+    const uint64_t q_desc = sdesc_sw128(smem_u32(sQ), 16, 1024);
+    const uint64_t p_desc = sdesc_sw128(smem_u32(sP), 16, 1024);
+    // V_j, MN-major. 64-wide heads: the second 64 of the product's 128 rows read the same chunk
+    // again (leading offset 0) and are never looked at.
+    const uint64_t v_desc = sdesc_sw128(smem_u32(sRing), D == 128 ? kChunk : 0, 1024);
     int gb = 0;       // blocks before this item
+    int wi[2] = {0, 0};   // items that each warpgroup had a block of
     bool ok = true;
     for (int it = 0; ok; ++it) {
       const int qi = it % kQueue;
@@ -356,147 +430,166 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) bar_arrive(&i_empty[qi]);
       if (im.last) break;
       const int nb = im.nblk;
-      const int qb = it & 1;
-      if (!wait_bar_warp(&q_full[qb], (uint32_t)((it >> 1) & 1), g, 53, it)) break;
-      for (int j = 0; j <= nb && ok; ++j) {
-        if (j < nb) {
-          const int gj = gb + j;
-          const int nk = n_ring + 2 * j;
-          const int sk = nk % R;
-          if (!wait_bar_warp(&kv_full[sk], (uint32_t)((nk / R) & 1), g, 54, nk)) { ok = false; break; }
-          if (!wait_bar_warp(&s_empty[gj & 1], (uint32_t)((gj >> 1) & 1) ^ 1, g, 55, gj)) { ok = false; break; }
+      if (warp == kQkWarp) {
+        const int qb = it & 1;
+        if (!wait_soon_warp(&q_full[qb], (uint32_t)((it >> 1) & 1), g, 53, it)) break;
+        for (int j = 0; j < nb; ++j) {
+          const int gj = gb + j, w = gj & 1, nk = 2 * gj, sk = nk % R;
+          if (!wait_soon_warp(&kv_full[sk], (uint32_t)((nk / R) & 1), g, 54, nk) ||
+              !wait_soon_warp(&s_empty[w], (uint32_t)((gj >> 1) & 1) ^ 1, g, 55, gj)) { ok = false; break; }
           tc_fence_after();
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t o = (kk >> 2) * kChunk + (kk & 3) * 32;
-            const uint64_t ad = sdesc_sw128(r_base + sk * C::kBlock + o, 16, 1024);
-            const uint64_t bd = sdesc_sw128(q_base + qb * C::kQ + (kk >> 2) * NR * 128 +
-                                                (kk & 3) * 32, 16, 1024);
-            if (elect_one()) mma_f16_ss(tS + NR * (gj & 1), ad, bd, kIdescQK, kk > 0 ? 1u : 0u);
-          }
           if (elect_one()) {
-            mma_commit(&s_full[gj & 1]);
+            const uint64_t ad = r_desc + (uint64_t)((sk * C::kBlock) >> 4);
+            const uint64_t bd = q_desc + (uint64_t)((qb * C::kQ) >> 4);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk)
+              mma_f16_ss(tmem + NR * w, ad + (((kk >> 2) * kChunk + (kk & 3) * 32) >> 4),
+                         bd + (((kk >> 2) * NR * 128 + (kk & 3) * 32) >> 4), kIdescQK, kk > 0 ? 1u : 0u);
+            mma_commit(&s_full[w]);
             mma_commit(&kv_empty[sk]);                   // K_j read
             if (j == nb - 1) mma_commit(&q_empty[qb]);   // the item's Q read for the last time
           }
           __syncwarp();
         }
-        if (j > 0) {
-          const int gp = gb + j - 1;
-          const int nv = n_ring + 2 * (j - 1) + 1;
-          const int sv = nv % R;
-          const int pb = gp & 1;
-          if (!wait_bar_warp(&kv_full[sv], (uint32_t)((nv / R) & 1), g, 56, nv)) { ok = false; break; }
-          const int valid = im.len - (im.kb0 + j - 1) * 128;
-          if (valid < 128) zero_tail<D>(r_base + sv * C::kBlock, valid);
-          if (!wait_bar_warp(&p_full[pb], (uint32_t)((gp >> 1) & 1), g, 57, gp)) { ok = false; break; }
-          if (j == 1 && it > 0) {
-            // Oᵀ of the previous item read by its epilogue before the first PV overwrites it.
-            if (!wait_bar_warp(o_empty, (uint32_t)((it - 1) & 1), g, 58, it)) { ok = false; break; }
-          }
+      } else {
+        for (int j = 0; j < nb; ++j) {
+          const int gj = gb + j, w = gj & 1, nv = 2 * gj + 1, sv = nv % R;
+          const int ob = wi[w] & 1;
+          if (!wait_soon_warp(&kv_full[sv], (uint32_t)((nv / R) & 1), g, 56, nv)) { ok = false; break; }
+          const int valid = im.len - (im.kb0 + j) * 128;
+          if (valid < 128) zero_tail<D>(smem_u32(sRing) + sv * C::kBlock, valid);
+          // the warpgroup's O buffer is free once the epilogue of its last item but one read it
+          if (j < 2 && !wait_soon_warp(&o_empty[2 * w + ob], (uint32_t)((wi[w] >> 1) & 1) ^ 1, g, 58, gj)) { ok = false; break; }
+          if (!wait_soon_warp(&p_full[w], (uint32_t)((gj >> 1) & 1), g, 57, gj)) { ok = false; break; }
           tc_fence_after();
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk) {   // 16 keys per MMA
-            // 64-wide heads: the second 64 of the 128 rows read the same chunk again (leading
-            // offset 0) and are never looked at.
-            const uint64_t ad = sdesc_sw128(r_base + sv * C::kBlock + kk * 16 * 128,
-                                            D == 128 ? kChunk : 0, 1024);
-            const uint64_t bd = sdesc_sw128(p_base + pb * C::kP + (kk >> 2) * NR * 128 + (kk & 3) * 32, 16, 1024);
-            if (elect_one()) mma_f16_ss(tO, ad, bd, kIdescPV, (j == 1 && kk == 0) ? 0u : 1u);
-          }
           if (elect_one()) {
-            mma_commit(&p_empty[pb]);
-            mma_commit(&kv_empty[sv]);                   // V_{j-1} read
-            if (j == nb) mma_commit(o_full);
+            const uint64_t ad = v_desc + (uint64_t)((sv * C::kBlock) >> 4);
+            const uint64_t bd = p_desc + (uint64_t)((w * C::kP) >> 4);
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk)   // 16 keys per MMA
+              mma_f16_ss(tmem + NR * (2 + 2 * w + ob), ad + ((kk * 16 * 128) >> 4),
+                         bd + (((kk >> 2) * NR * 128 + (kk & 3) * 32) >> 4), kIdescPV,
+                         (j < 2 && kk == 0) ? 0u : 1u);
+            mma_commit(&p_empty[w]);
+            mma_commit(&kv_empty[sv]);                   // V_j read
+            if (j + 2 >= nb) mma_commit(&o_full[2 * w + ob]);   // its last block of the item
           }
           __syncwarp();
         }
       }
-      n_ring += 2 * nb;
+      ++wi[gb & 1];
+      if (nb > 1) ++wi[(gb & 1) ^ 1];
       gb += nb;
     }
     if (elect_one()) mma_commit(drain);
     __syncwarp();
     drain_wait(drain, 0, p.timeout_ns);
   } else {
-    // ---------------- softmax and epilogue: warps 0-3 ----------------
-    const int t = (int)(warp * 32 + lane);              // key within the block / Oᵀ lane (d)
-    const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
+    // ---------------- softmax and epilogue: warpgroup w takes blocks gb with gb & 1 == w -----
+    const int w = warp >> 2;
+    const int t = threadIdx.x & 127;                    // key within the block / Oᵀ lane (d)
+    const int wl = warp & 3;
+    const uint32_t lane_off = (uint32_t)(wl * 32) << 16;
+    const uint32_t tS = tmem + lane_off + NR * w;
+    const int bar_id = 1 + w;
+    float* red = sRed + w * 4 * NR;
+    uint8_t* pt = sP + w * C::kP + (t >> 6) * NR * 128 + (t & 7) * 2;   // Pᵀ: this key's column
     const float NEG_INF = -INFINITY;
     const float sl = p.scale_log2;
 
     // Sequences without a key: zero rows (or no part for the join).
-    for (int b = blockIdx.x; b < batch; b += G) {
-      const SeqInfo s = seq_info(p.seqs, b);
-      if (blocks_of(s) > 0) continue;
-      const bool rows = s.qlen > 0;
-      for (int hk = t; hk < p.Hkv; hk += 128)
-        p.tab[b * p.Hkv + hk] = make_int4(0, 0, -1, rows && p.keep_parts ? kItemNoKeys : kItemDone);
-      if (rows && !p.keep_parts) {
-        for (int i = 0; i < s.qlen; ++i)
-          for (int h = 0; h < p.Hq; ++h) {
-            uint16_t* o = reinterpret_cast<uint16_t*>(p.O) + (long long)(s.tok0 + i) * p.o_st + h * p.o_sh;
-            if (t < D) o[t] = 0;
-            if (p.lse && t == 0) p.lse[(long long)(s.tok0 + i) * p.Hq + h] = NEG_INF;
-          }
+    if (w == 1) {
+      for (int b = blockIdx.x; b < batch; b += G) {
+        const SeqInfo s = seq_info(p.seqs, b);
+        if (blocks_of(s) > 0) continue;
+        const bool rows = s.qlen > 0;
+        for (int hk = t; hk < p.Hkv; hk += 128)
+          p.tab[b * p.Hkv + hk] = make_int4(0, 0, -1, rows && p.keep_parts ? kItemNoKeys : kItemDone);
+        if (rows && !p.keep_parts) {
+          for (int i = 0; i < s.qlen; ++i)
+            for (int h = 0; h < p.Hq; ++h) {
+              uint16_t* o = reinterpret_cast<uint16_t*>(p.O) + (long long)(s.tok0 + i) * p.o_st + h * p.o_sh;
+              if (t < D) o[t] = 0;
+              if (p.lse && t == 0) p.lse[(long long)(s.tok0 + i) * p.Hq + h] = NEG_INF;
+            }
+        }
       }
     }
 
-    int gb = 0;
+    // r / group by a product: exact for r < 32 and group <= 32
+    const uint32_t inv_group = 65536u / (uint32_t)p.group + 1u;
+    auto row_pos = [&](int r) -> int { return (int)((uint32_t)r * inv_group >> 16); };
+    int gb = 0;       // blocks before this item
+    int wi = 0;       // this warpgroup's items before this one
+    int wo = 0;       // the other's
+    int xn[2] = {0, 0};   // deposits of each warpgroup before this item
     for (int it = 0;; ++it) {
       const int qi = it % kQueue;
       // A wait that gave up leaves the CTA's abort flag up; every thread sees it at its next
-      // wait, and all 128 leave together after a vote.
+      // wait, and the 128 leave together after a vote.
       bool ok = wait_bar(&i_full[qi], (uint32_t)((it / kQueue) & 1), g, 72, it);
-      if (vote_any(!ok)) break;
+      if (vote_any(bar_id, !ok)) break;
       const Item im = items[qi];
       __syncwarp();
       if (lane == 0) bar_arrive(&i_empty[qi]);
       if (im.last) break;
-      // Row r = position·group + head of the group; its last visible key.
-      int last_key[RR];
-#pragma unroll
-      for (int r = 0; r < RR; ++r) {
-        const int pos = r / p.group;
-        last_key[r] = r < p.nrows && pos < im.qlen ? (p.causal ? im.len - im.qlen + pos : im.len - 1) : -1;
+      const int nb = im.nblk;
+      const int j0 = (gb & 1) == w ? 0 : 1;             // this warpgroup's first block
+      const int depositor = nb > 1 ? (gb + nb) & 1 : -1;   // the one without the last block
+      const int x_before = depositor >= 0 ? xn[depositor]++ : 0;
+      if (j0 >= nb) {                                    // the other's only block
+        gb += nb;
+        ++wo;
+        continue;
       }
+      const int n_rows = min(p.nrows, im.qlen * p.group);   // rows r < n_rows are real
+      // Row r = position·group + head of the group sees keys up to lim0 + position.
+      const int lim0 = p.causal ? im.len - im.qlen : im.len - 1;
+      const uint32_t tO = tmem + lane_off + NR * (2 + 2 * w + (wi & 1));
       float m_ref[RR], l_part[RR];
 #pragma unroll
       for (int r = 0; r < RR; ++r) {
         m_ref[r] = NEG_INF;
         l_part[r] = 0.f;
       }
-      for (int j = 0; j < im.nblk; ++j, ++gb) {
+      for (int j = j0; j < nb; j += 2) {
+        const int gj = gb + j;
         const int key = (im.kb0 + j) * 128 + t;
-        if (!wait_bar(&s_full[gb & 1], (uint32_t)((gb >> 1) & 1), g, 61, gb)) ok = false;
+        const uint32_t ph = (uint32_t)((gj >> 1) & 1);
+        if (!wait_soon(&s_full[w], ph, g, 61, gj)) ok = false;
+        __syncwarp();
         tc_fence_after();
         uint32_t sv[RR];
-        ld_cols<RR>(tS + lane_off + NR * (gb & 1), sv);
+        ld_cols<RR>(tS, sv);
         tmem_wait_ld();
         tc_fence_before();
-        bar_arrive(&s_empty[gb & 1]);
+        __syncwarp();
+        if (lane == 0) bar_arrive(&s_empty[w]);
         float x[RR];
         bool up = false;
+        const bool open = (im.kb0 + j) * 128 + 127 <= lim0;   // every row sees the whole block
 #pragma unroll
         for (int r = 0; r < RR; ++r) {
-          x[r] = key <= last_key[r] ? __uint_as_float(sv[r]) * sl : NEG_INF;
+          bool see = r < n_rows;
+          if (!open) see = see && key <= lim0 + (p.causal ? row_pos(r) : 0);
+          x[r] = see ? __uint_as_float(sv[r]) * sl : NEG_INF;
           up |= x[r] > m_ref[r] + kLazy;
         }
-        if (vote_any(up)) {
+        if (vote_any(bar_id, up)) {
           // A row's reference moves: the block's row maxima, within the warps and across them.
 #pragma unroll
           for (int r = 0; r < RR; ++r) {
             float v = x[r];
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-            if (lane == 0) sRed[warp * NR + r] = v;
+            if (lane == 0) red[wl * NR + r] = v;
           }
-          named_barrier_sync(1, 128);
+          named_barrier_sync(bar_id, 128);
           bool resc = false;
           float alpha[RR];
 #pragma unroll
           for (int r = 0; r < RR; ++r) {
-            const float bm = fmaxf(fmaxf(sRed[r], sRed[NR + r]), fmaxf(sRed[2 * NR + r], sRed[3 * NR + r]));
+            const float bm = fmaxf(fmaxf(red[r], red[NR + r]), fmaxf(red[2 * NR + r], red[3 * NR + r]));
             alpha[r] = 1.f;
             if (bm > m_ref[r] + kLazy) {
               if (m_ref[r] != NEG_INF) {
@@ -507,88 +600,134 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             l_part[r] *= alpha[r];
           }
-          if (resc && j > 0) {
-            // Oᵀ holds PV up to block j-1: let it finish, then rescale its columns.
-            if (!wait_bar(&p_empty[(gb - 1) & 1], (uint32_t)(((gb - 1) >> 1) & 1), g, 62, gb)) ok = false;
+          if (resc && j > j0) {
+            // Oᵀ holds this warpgroup's PV up to its last block: let it finish, then rescale.
+            if (!wait_soon(&p_empty[w], ph ^ 1, g, 62, gj)) ok = false;
+            __syncwarp();
             tc_fence_after();
             uint32_t o[RR];
-            ld_cols<RR>(tO + lane_off, o);
+            ld_cols<RR>(tO, o);
             tmem_wait_ld();
 #pragma unroll
             for (int r = 0; r < RR; ++r) o[r] = __float_as_uint(__uint_as_float(o[r]) * alpha[r]);
-            st_cols<RR>(tO + lane_off, o);
+            st_cols<RR>(tO, o);
             tmem_wait_st();
           }
-          named_barrier_sync(1, 128);     // sRed is read: the next block may write it
+          named_barrier_sync(bar_id, 128);     // red is read: the next block may write it
         }
-        // Pᵀ of this block into buffer gb & 1 once the PV of block gb - 2 has read it.
-        if (!wait_bar(&p_empty[gb & 1], (uint32_t)((gb >> 1) & 1) ^ 1, g, 63, gb)) ok = false;
-        uint8_t* pb = sP + (gb & 1) * C::kP + (t >> 6) * NR * 128;
-        const int kin = t & 63;            // key within the 64-key chunk
+        // Pᵀ of this block, once the PV of this warpgroup's block before has read the buffer.
+        if (!wait_soon(&p_empty[w], ph ^ 1, g, 63, gj)) ok = false;
 #pragma unroll
         for (int r = 0; r < RR; ++r) {
           const float mu = m_ref[r] == NEG_INF ? 0.f : m_ref[r] - kShift;
           const float pr = fast_exp2(x[r] - mu);
           l_part[r] += pr;
-          // K-major, 128-byte swizzle: 16-byte unit (kin / 8) of row r moves to (kin / 8) ^ (r % 8).
-          const int unit = (kin >> 3) ^ (r & 7);
-          *reinterpret_cast<uint16_t*>(pb + r * 128 + unit * 16 + (kin & 7) * 2) = bits16<BF16>(pr);
+          // K-major, 128-byte swizzle: 16-byte unit (key / 8) of row r moves to (key / 8) ^ (r % 8).
+          const int unit = ((t & 63) >> 3) ^ (r & 7);
+          *reinterpret_cast<uint16_t*>(pt + r * 128 + unit * 16) = bits16<BF16>(pr);
         }
         fence_proxy_async_smem();
         tc_fence_before();
-        bar_arrive(&p_full[gb & 1]);
+        __syncwarp();
+        if (lane == 0) bar_arrive(&p_full[w]);
       }
 
-      // ---------------- epilogue of the item ----------------
-      if (!wait_bar(o_full, (uint32_t)(it & 1), g, 64, it)) ok = false;
-      tc_fence_after();
-      uint32_t o[RR];
-      ld_cols<RR>(tO + lane_off, o);
-      tmem_wait_ld();
-      tc_fence_before();
-      bar_arrive(o_empty);
-      // Row sums: each thread holds its keys' share.
+      // ---------------- the item's end ----------------
+      // Row sums: each thread holds its keys' share. The warps' sums meet at the vote below.
 #pragma unroll
       for (int r = 0; r < RR; ++r) {
         float v = l_part[r];
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-        if (lane == 0) sRed[warp * NR + r] = v;
+        if (lane == 0) red[wl * NR + r] = v;
       }
-      const bool bad = vote_any(!ok);      // also the barrier between the sums' writes and reads
+      if (depositor == w) {
+        if (!wait_bar(&x_empty[w], (uint32_t)(x_before & 1) ^ 1, g, 65, it)) ok = false;
+        if (vote_any(bar_id, !ok)) break;
 #pragma unroll
-      for (int r = 0; r < RR; ++r) {
-        const int pos = r / p.group;
-        if (r >= p.nrows || pos >= im.qlen || bad) continue;
-        const float l = (sRed[r] + sRed[NR + r]) + (sRed[2 * NR + r] + sRed[3 * NR + r]);
-        const float ov = __uint_as_float(o[r]);
-        const float m = m_ref[r] == NEG_INF ? NEG_INF : m_ref[r] - kShift;
-        if (im.slot < 0) {
-          const long long tok = im.tok0 + pos;
-          const int h = im.hk * p.group + r - pos * p.group;
-          const float inv = l == 0.f ? 0.f : 1.f / l;
-          uint16_t* dst = reinterpret_cast<uint16_t*>(p.O) + tok * p.o_st + h * p.o_sh;
-          if (t < D) dst[t] = bits16<BF16>(ov * inv);
-          if (p.lse && t == 0)
-            p.lse[tok * p.Hq + h] = l == 0.f ? NEG_INF : (m + log2f(l)) * 0.69314718055994530942f;
-        } else {
-          const long long at = (long long)im.slot * NR + r;
-          if (t < D) p.part_o[at * D + t] = ov;
-          if (t == 0) {
-            p.part_ml[at * 2] = m;
-            p.part_ml[at * 2 + 1] = l;
+        for (int r = 0; r < RR; ++r)
+          if (t == r) {
+            sXml[(w * NR + r) * 2] = m_ref[r];
+            sXml[(w * NR + r) * 2 + 1] = (red[r] + red[NR + r]) + (red[2 * NR + r] + red[3 * NR + r]);
+          }
+        __syncwarp();
+        if (lane == 0) bar_arrive(&x_full[w]);
+      } else {
+        const int ww = w ^ 1;
+        const bool both = depositor == ww;
+        if (!wait_bar(&o_full[2 * w + (wi & 1)], (uint32_t)((wi >> 1) & 1), g, 64, it)) ok = false;
+        if (both && (!wait_bar(&o_full[2 * ww + (wo & 1)], (uint32_t)((wo >> 1) & 1), g, 67, it) ||
+                     !wait_bar(&x_full[ww], (uint32_t)(x_before & 1), g, 66, it))) ok = false;
+        if (vote_any(bar_id, !ok)) break;
+        tc_fence_after();
+        uint32_t o[RR];
+        ld_cols<RR>(tO, o);
+        tmem_wait_ld();
+        float l[RR], m[RR];
+#pragma unroll
+        for (int r = 0; r < RR; ++r) {
+          l[r] = (red[r] + red[NR + r]) + (red[2 * NR + r] + red[3 * NR + r]);
+          m[r] = m_ref[r];
+        }
+        if (both) {
+          // the two warpgroups' sums over the larger of their references
+          uint32_t o2[RR];
+          ld_cols<RR>(tmem + lane_off + NR * (2 + 2 * ww + (wo & 1)), o2);
+          tmem_wait_ld();
+#pragma unroll
+          for (int r = 0; r < RR; ++r) {
+            const float m2 = sXml[(ww * NR + r) * 2], l2 = sXml[(ww * NR + r) * 2 + 1];
+            const float mm = fmaxf(m[r], m2);
+            const float mu = mm == NEG_INF ? 0.f : mm;
+            const float a1 = fast_exp2(m[r] - mu), a2 = fast_exp2(m2 - mu);
+            l[r] = l[r] * a1 + l2 * a2;
+            o[r] = __float_as_uint(__uint_as_float(o[r]) * a1 + __uint_as_float(o2[r]) * a2);
+            m[r] = mm;
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          bar_arrive(&o_empty[2 * w + (wi & 1)]);
+          if (both) {
+            bar_arrive(&o_empty[2 * ww + (wo & 1)]);
+            bar_arrive(&x_empty[ww]);
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < RR; ++r) {
+          if (r >= n_rows) continue;
+          const float ov = __uint_as_float(o[r]);
+          const float mr = m[r] == NEG_INF ? NEG_INF : m[r] - kShift;
+          if (im.slot < 0) {
+            const int pos = row_pos(r);
+            const long long tok = im.tok0 + pos;
+            const int h = im.hk * p.group + r - pos * p.group;
+            const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
+            uint16_t* dst = reinterpret_cast<uint16_t*>(p.O) + tok * p.o_st + h * p.o_sh;
+            if (t < D) dst[t] = bits16<BF16>(ov * inv);
+            if (p.lse && t == 0)
+              p.lse[tok * p.Hq + h] = l[r] == 0.f ? NEG_INF : (mr + log2f(l[r])) * 0.69314718055994530942f;
+          } else {
+            const long long at = (long long)im.slot * NR + r;
+            if (t < D) p.part_o[at * D + t] = ov;
+            if (t == 0) {
+              p.part_ml[at * 2] = mr;
+              p.part_ml[at * 2 + 1] = l[r];
+            }
           }
         }
       }
-      if (bad) break;
-      named_barrier_sync(1, 128);     // the sums are read: the next item may write the slots
+      named_barrier_sync(bar_id, 128);     // the sums are read: the next item may write them
+      gb += nb;
+      ++wi;
+      if (nb > 1) ++wo;
     }
   }
 
   tc_fence_before();
   __syncthreads();
-  griddep_launch_dependents();
-  if (warp == kMmaWarp) {
+  if (warp == kQkWarp) {
     tc_fence_after();
     tmem_dealloc(tmem, C::kTmemCols);
   }
@@ -596,24 +735,20 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 template <int D, int NR, int RR, bool BF16>
 int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const DecParams& p,
-           int ctas, cudaStream_t stream) {
-  auto kern = paged_decode_kernel<D, NR, RR, BF16>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       Cfg<D, NR>::kSmem);
-  if (e != cudaSuccess) return fail_cuda(e, "lvb_attention_paged", "cudaFuncSetAttribute (decode)");
-  kern<<<ctas, kThreads, Cfg<D, NR>::kSmem, stream>>>(tq, tk, tv, p);
-  e = cudaGetLastError();
-  return e == cudaSuccess ? LVB_OK : fail_cuda(e, "lvb_attention_paged", "decode launch");
+           int ctas, cudaStream_t stream, DeviceState* dev) {
+  static SmemAttr attr;
+  return launch_serial("lvb_attention_paged", paged_decode_kernel<D, NR, RR, BF16>, attr, dev, ctas,
+                       kThreads, Cfg<D, NR>::kSmem, stream, tq, tk, tv, p);
 }
 
 template <int D, bool BF16>
 int launch_rows(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
-                const DecParams& p, int ctas, cudaStream_t stream) {
-  if (p.nrows == 1) return launch<D, 16, 1, BF16>(tq, tk, tv, p, ctas, stream);
-  if (p.nrows <= 4) return launch<D, 16, 4, BF16>(tq, tk, tv, p, ctas, stream);
-  if (p.nrows <= 8) return launch<D, 16, 8, BF16>(tq, tk, tv, p, ctas, stream);
-  if (p.nrows <= 16) return launch<D, 16, 16, BF16>(tq, tk, tv, p, ctas, stream);
-  return launch<D, 32, 32, BF16>(tq, tk, tv, p, ctas, stream);
+                const DecParams& p, int ctas, cudaStream_t stream, DeviceState* dev) {
+  if (p.nrows == 1) return launch<D, 16, 1, BF16>(tq, tk, tv, p, ctas, stream, dev);
+  if (p.nrows <= 4) return launch<D, 16, 4, BF16>(tq, tk, tv, p, ctas, stream, dev);
+  if (p.nrows <= 8) return launch<D, 16, 8, BF16>(tq, tk, tv, p, ctas, stream, dev);
+  if (p.nrows <= 16) return launch<D, 16, 16, BF16>(tq, tk, tv, p, ctas, stream, dev);
+  return launch<D, 32, 32, BF16>(tq, tk, tv, p, ctas, stream, dev);
 }
 
 int product_rows(const lvb_paged_desc* d) {
@@ -676,10 +811,10 @@ int paged_decode_launch(const lvb_paged_desc* d, const PagedLayout& lay, const P
   int st = paged_kv_maps(&tk, &tv, d, lay, Kc, Vc, op);
   if (st) return st;
   if (d->head_dim == 128)
-    return d->dtype == LVB_BF16 ? launch_rows<128, true>(tq, tk, tv, p, ctas, stream)
-                                : launch_rows<128, false>(tq, tk, tv, p, ctas, stream);
-  return d->dtype == LVB_BF16 ? launch_rows<64, true>(tq, tk, tv, p, ctas, stream)
-                              : launch_rows<64, false>(tq, tk, tv, p, ctas, stream);
+    return d->dtype == LVB_BF16 ? launch_rows<128, true>(tq, tk, tv, p, ctas, stream, dev)
+                                : launch_rows<128, false>(tq, tk, tv, p, ctas, stream, dev);
+  return d->dtype == LVB_BF16 ? launch_rows<64, true>(tq, tk, tv, p, ctas, stream, dev)
+                              : launch_rows<64, false>(tq, tk, tv, p, ctas, stream, dev);
 }
 
 }  // namespace lvb

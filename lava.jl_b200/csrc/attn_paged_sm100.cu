@@ -78,14 +78,6 @@ __device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity, uint6
 __device__ __forceinline__ int ring_k(int j) { return j == 0 ? 0 : 2 * j - 1; }
 __device__ __forceinline__ int ring_v(int j, int nb) { return j + 1 < nb ? 2 * j + 2 : 2 * j + 1; }
 
-// An issuer's wait: a non-blocking test first, the bounded suspending wait otherwise.
-__device__ __forceinline__ bool issuer_wait(uint64_t* bar, uint32_t parity, const WaitGuard& g,
-                                            int where, int detail) {
-  bool ok = bar_test_wait(smem_u32(bar), parity);
-  if (!__all_sync(0xffffffffu, ok)) ok = wait_bar_warp(bar, parity, g, where, detail);
-  return ok;
-}
-
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if constexpr (BF16) {
@@ -180,6 +172,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const WaitGuard g{p.seqs.status, abort_flag, p.timeout_ns};
+  // The setup above may run while the stream's previous kernel ends; what reads this kernel's
+  // results after its own wait may be scheduled from here on.
+  griddep_wait();
+  griddep_launch_dependents();
   const int npb = (p.prefix + 127) / 128;
 
   if (warp == kTmaWarp) {
@@ -309,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int s = rn % R;
         if (!wait_bar_warp(&ring_empty[s], (uint32_t)((rn / R) & 1) ^ 1, g, 12, rn)) { ok = false; break; }
         load_block<D>(sRing + s * C::kTileBytes, is_k ? &tmK : &tmV, bl, is_k ? ak : av, p.box,
-                      im.hk, &ring_full[s]);
+                      im.hk, &ring_full[s], p.seqs);
       }
     }
     if (!ok && lane == 0) {
@@ -349,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto ring_wait = [&](int i, int where) -> bool {
         if (i <= ring_seen) return true;
         const int x = rc + i;
-        if (!issuer_wait(&ring_full[x % R], (uint32_t)((x / R) & 1), g, where, i)) return false;
+        if (!wait_soon_warp(&ring_full[x % R], (uint32_t)((x / R) & 1), g, where, i)) return false;
         ring_seen = i;
         return true;
       };
@@ -363,7 +359,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         int qk_done = 0;
         auto fill = [&](int t, int j) -> bool {
           if (!ring_wait(ring_k(j), 13)) return false;
-          if (fills > 0 && !issuer_wait(s_free, (uint32_t)((fills - 1) & 1), g, 17, j))
+          if (fills > 0 && !wait_soon_warp(s_free, (uint32_t)((fills - 1) & 1), g, 17, j))
             return false;
           tc_fence_after();
           const bool last = ++qk_done == n_qk;
@@ -408,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             zero_tail<D>(r_base + ((rc + ring_v(j, nb)) % R) * C::kTileBytes, valid);
           for (int t = 0; t < 2; ++t) {
             if (j >= nt[t]) continue;
-            if (!issuer_wait(&p_full[t], (uint32_t)((gt[t] + j) & 1), g, 15, j)) {
+            if (!wait_soon_warp(&p_full[t], (uint32_t)((gt[t] + j) & 1), g, 15, j)) {
               ok = false;
               break;
             }
@@ -637,7 +633,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   tc_fence_before();
   __syncthreads();
-  griddep_launch_dependents();
   if (warp == kQkWarp) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
@@ -647,22 +642,26 @@ __global__ void __launch_bounds__(kThreads, 1)
 // ----------------------------------------------------------------------------------------
 // The join: O = Σ 2^(m_s - m) O_s / Σ 2^(m_s - m) l_s, m = max m_s, over a row's parts in a fixed
 // order (the prefix's or the tile's key ranges, then the decoding kernel's pieces). One warp per
-// row; lanes hold the parts' (m, l) and then D/32 elements of the row each. A programmatic
-// dependent of the kernel before it.
+// row, D/32 elements per lane. Bound by the latency of its loads (the lists, the item's table
+// entry, the parts), so the parts' rows are loaded beside their (m, l), before their weights are
+// known.
 // ----------------------------------------------------------------------------------------
 template <int D, bool BF16>
-__global__ void __launch_bounds__(256) merge_kernel(const MergeParams p, long long rows) {
+__global__ void __launch_bounds__(256) merge_kernel(const MergeParams p, int rows) {
   constexpr int V = D / 32;            // elements per lane
   const int lane = lane_id();
+  griddep_launch_dependents();
+  // one row per warp: (sequence, position, head)
+  const int row = blockIdx.x * 8 + warp_id();
+  const int bq = row / p.Hq;
+  const int h = row - bq * p.Hq;
+  const int b = bq / p.seqs.max_q;
+  const int pos = bq - b * p.seqs.max_q;
+  // The lists are older than the kernel before this one; what that kernel wrote is not. Every
+  // warp waits for it, so that this grid's end is also that kernel's.
+  SeqInfo s{0, 0, 0};
+  if (row < rows) s = seq_info(p.seqs, b);
   griddep_wait();
-  const long long idx = blockIdx.x * 8LL + warp_id();
-  if (idx >= rows) return;
-  // idx = (sequence·max_q + position)·Hq + head
-  const int h = (int)(idx % p.Hq);
-  const long long bq = idx / p.Hq;
-  const int b = (int)(bq / p.seqs.max_q);
-  const int pos = (int)(bq - (long long)b * p.seqs.max_q);
-  const SeqInfo s = seq_info(p.seqs, b);
   if (pos >= s.qlen) return;
   const long long tok = s.tok0 + pos;
   const int hk = h / p.group, gh = h - hk * p.group;
@@ -695,51 +694,48 @@ __global__ void __launch_bounds__(256) merge_kernel(const MergeParams p, long lo
     return ~(slot * p.dec_rows + dec_row);
   };
   const int n = nt + nd;
-  float m = -INFINITY;
-  for (int i = lane; i < n; i += 32) {
-    const long long r = row_of(i);
-    m = fmaxf(m, r >= 0 ? p.tile_ml[2 * r] : p.dec_ml[2 * ~r]);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float mu = m == -INFINITY ? 0.f : m;
-  float den = 0.f;
+  // Part by part in chunks of eight, whose rows are all under way at once, beside their (m, l): a
+  // running maximum m, and sums relative to it. A part without a key has l = 0 and an O that
+  // nothing wrote: its weight is 0 and its row is dropped.
+  float m = -INFINITY, den = 0.f;
   float acc[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) acc[e] = 0.f;
-  for (int i0 = 0; i0 < n; i0 += 32) {
-    float w = 0.f;
-    if (i0 + lane < n) {
-      const long long r = row_of(i0 + lane);
-      const float* ml = r >= 0 ? p.tile_ml + 2 * r : p.dec_ml + 2 * ~r;
-      const float l = ml[1];
-      // A part without a key has l = 0 and an O that nothing wrote: weight 0, not read.
-      w = l == 0.f ? 0.f : exp2f(ml[0] - mu);
-      den += w * l;
-    }
-    const int k1 = min(32, n - i0);
-#pragma unroll 4
-    for (int k = 0; k < k1; ++k) {
-      const float wk = __shfl_sync(0xffffffffu, w, k);
-      if (wk != 0.f) {
-        const long long r = row_of(i0 + k);
-        const float* src = (r >= 0 ? p.tile_o + r * D : p.dec_o + ~r * D) + lane * V;
-        if constexpr (V == 4) {
-          const float4 v = *reinterpret_cast<const float4*>(src);
-          acc[0] += wk * v.x;
-          acc[1] += wk * v.y;
-          acc[2] += wk * v.z;
-          acc[3] += wk * v.w;
-        } else {
-          const float2 v = *reinterpret_cast<const float2*>(src);
-          acc[0] += wk * v.x;
-          acc[1] += wk * v.y;
-        }
+  for (int i0 = 0; i0 < n; i0 += 8) {
+    float v[8][V];
+    float2 ml[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const long long r = row_of(min(i0 + q, n - 1));
+      const float* src = (r >= 0 ? p.tile_o + r * D : p.dec_o + ~r * D) + lane * V;
+      ml[q] = *reinterpret_cast<const float2*>(r >= 0 ? p.tile_ml + 2 * r : p.dec_ml + 2 * ~r);
+      if constexpr (V == 4) {
+        const float4 f = *reinterpret_cast<const float4*>(src);
+        v[q][0] = f.x, v[q][1] = f.y, v[q][2] = f.z, v[q][3] = f.w;
+      } else {
+        const float2 f = *reinterpret_cast<const float2*>(src);
+        v[q][0] = f.x, v[q][1] = f.y;
       }
     }
-  }
+    float mn = m;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
+    for (int q = 0; q < 8; ++q) mn = fmaxf(mn, ml[q].y == 0.f ? -INFINITY : ml[q].x);
+    const float mu = mn == -INFINITY ? 0.f : mn;
+    const float keep = exp2f(m - mu);
+    den *= keep;
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] *= keep;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const bool in = i0 + q < n && ml[q].y != 0.f;
+      const float wq = in ? exp2f(ml[q].x - mu) : 0.f;
+      den += in ? wq * ml[q].y : 0.f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] += in ? wq * v[q][e] : 0.f;
+    }
+    m = mn;
+  }
+  const float mu = m == -INFINITY ? 0.f : m;
   const float inv = den == 0.f ? 0.f : 1.f / den;
   uint16_t* dst = reinterpret_cast<uint16_t*>(p.O) + tok * p.o_st + h * p.o_sh + lane * V;
 #pragma unroll
@@ -751,14 +747,10 @@ __global__ void __launch_bounds__(256) merge_kernel(const MergeParams p, long lo
 
 template <int D, bool BF16>
 int launch_flash(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
-                 const FlashParams& p, int ctas, cudaStream_t stream) {
-  auto kern = paged_flash_kernel<D, BF16>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       Cfg<D>::kSmem);
-  if (e != cudaSuccess) return fail_cuda(e, "lvb_attention_paged", "cudaFuncSetAttribute");
-  kern<<<ctas, kThreads, Cfg<D>::kSmem, stream>>>(tq, tk, tv, p);
-  e = cudaGetLastError();
-  return e == cudaSuccess ? LVB_OK : fail_cuda(e, "lvb_attention_paged", "kernel launch");
+                 const FlashParams& p, int ctas, cudaStream_t stream, DeviceState* dev) {
+  static SmemAttr attr;
+  return launch_serial("lvb_attention_paged", paged_flash_kernel<D, BF16>, attr, dev, ctas, kThreads,
+                       Cfg<D>::kSmem, stream, tq, tk, tv, p);
 }
 
 constexpr size_t kCounterBytes = 256;   // the item counter, before the 32-byte stores' parts
@@ -845,31 +837,22 @@ int paged_flash_launch(const lvb_paged_desc* d, const PagedLayout& lay, const Pa
     if (e != cudaSuccess) return fail_cuda(e, op, "work counter reset");
   }
   if (d->head_dim == 128)
-    return d->dtype == LVB_BF16 ? launch_flash<128, true>(tq, tk, tv, p, ctas, stream)
-                                : launch_flash<128, false>(tq, tk, tv, p, ctas, stream);
-  return d->dtype == LVB_BF16 ? launch_flash<64, true>(tq, tk, tv, p, ctas, stream)
-                              : launch_flash<64, false>(tq, tk, tv, p, ctas, stream);
+    return d->dtype == LVB_BF16 ? launch_flash<128, true>(tq, tk, tv, p, ctas, stream, dev)
+                                : launch_flash<128, false>(tq, tk, tv, p, ctas, stream, dev);
+  return d->dtype == LVB_BF16 ? launch_flash<64, true>(tq, tk, tv, p, ctas, stream, dev)
+                              : launch_flash<64, false>(tq, tk, tv, p, ctas, stream, dev);
 }
 
-int merge_launch(const MergeParams& p, int D, bool bf16, cudaStream_t stream) {
-  const long long rows = (long long)p.seqs.batch * p.seqs.max_q * p.Hq;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((rows + 7) / 8));
-  cfg.blockDim = dim3(256);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cudaError_t e;
+int merge_launch(const MergeParams& p, int D, bool bf16, cudaStream_t stream, DeviceState* dev) {
+  const char* op = "lvb_attention_paged";
+  const int rows = p.seqs.batch * p.seqs.max_q * p.Hq;
+  const dim3 grid((unsigned)((rows + 7) / 8));
+  SmemAttr none;
   if (D == 128)
-    e = bf16 ? cudaLaunchKernelEx(&cfg, merge_kernel<128, true>, p, rows)
-             : cudaLaunchKernelEx(&cfg, merge_kernel<128, false>, p, rows);
-  else
-    e = bf16 ? cudaLaunchKernelEx(&cfg, merge_kernel<64, true>, p, rows)
-             : cudaLaunchKernelEx(&cfg, merge_kernel<64, false>, p, rows);
-  return e == cudaSuccess ? LVB_OK : fail_cuda(e, "lvb_attention_paged", "join launch");
+    return bf16 ? launch_serial(op, merge_kernel<128, true>, none, dev, grid, 256, 0, stream, p, rows)
+                : launch_serial(op, merge_kernel<128, false>, none, dev, grid, 256, 0, stream, p, rows);
+  return bf16 ? launch_serial(op, merge_kernel<64, true>, none, dev, grid, 256, 0, stream, p, rows)
+              : launch_serial(op, merge_kernel<64, false>, none, dev, grid, 256, 0, stream, p, rows);
 }
 
 }  // namespace lvb

@@ -10,9 +10,47 @@
 // map's bounds (and never written); each is recorded in the device status word.
 #pragma once
 
+#include <atomic>
+
 #include "lvb_internal.h"
 
 namespace lvb {
+
+// A kernel's shared-memory attribute: per function and per device, set once (two threads setting
+// it at once set the same value).
+struct SmemAttr {
+  static constexpr int kMaxDevices = 64;
+  std::atomic<bool> set[kMaxDevices] = {};
+};
+
+// Launch with programmatic stream serialization: the kernel may be scheduled while the stream's
+// previous kernel ends, and calls griddep_wait() before it touches global memory.
+template <typename... P, typename... A>
+int launch_serial(const char* op, void (*kern)(P...), SmemAttr& attr, DeviceState* dev, dim3 grid,
+                  int threads, size_t smem, cudaStream_t stream, const A&... args) {
+  if (smem > 48 * 1024) {
+    const int dv = dev->device;
+    const bool known = dv >= 0 && dv < SmemAttr::kMaxDevices;
+    if (!known || !attr.set[dv].load(std::memory_order_acquire)) {
+      const cudaError_t e =
+          cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+      if (e != cudaSuccess) return fail_cuda(e, op, "cudaFuncSetAttribute");
+      if (known) attr.set[dv].store(true, std::memory_order_release);
+    }
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+  return e == cudaSuccess ? LVB_OK : fail_cuda(e, op, "kernel launch");
+}
 
 // Sites of bad device data in the status word (code LVB_ERR_INVALID_ARG).
 constexpr int kBadLength = 81;   // seq_lens[b] negative or beyond the table's row
@@ -89,7 +127,7 @@ struct MergeParams {
   long long o_st, o_sh;
   float* lse;
 };
-int merge_launch(const MergeParams& p, int D, bool bf16, cudaStream_t stream);
+int merge_launch(const MergeParams& p, int D, bool bf16, cudaStream_t stream, DeviceState* dev);
 
 // The decoding kernel's table entry: (first slot, next CTA, last CTA, kind): the pieces are the
 // first slot, then slot 2c of every CTA c from the next to the last.
@@ -168,41 +206,54 @@ struct BlockLane {
 };
 
 // The page (and slot) of the lane's box in block kb of a run of `len` keys whose pages are
-// row[0 ..]; page -1 when the box holds no valid key. A bad page number becomes num_pages,
-// which the tensor map reads as zeros.
+// row[0 ..]. The page number is only looked at by load_block, so its load may be under way while
+// other work is done.
 struct BoxAt {
   int page, slot;
+  bool on;            // the box holds a valid key
 };
 template <int D>
 __device__ __forceinline__ BoxAt box_at(const BlockLane<D>& bl, const int* row, int kb, int len,
                                         int box, const PagedSeqs& p) {
-  BoxAt at{-1, 0};
+  BoxAt at{0, 0, false};
   const int key = kb * 128 + bl.sub * box;
   if (bl.in && key < len) {
     const int i = key / p.page_size;
     at.slot = key - i * p.page_size;
     at.page = row[i];
-    if (at.page < 0 || at.page >= p.num_pages) {
-      report_bad(p.status, kBadPage, i);
-      at.page = p.num_pages;
-    }
+    at.on = true;
   }
   return at;
 }
 
 // Issue one block's loads into `dst` ([D/64 chunks][128 rows][128 B], 128-byte swizzle) on
-// `bar`; the whole warp calls it.
+// `bar`; the whole warp calls it. A bad page number becomes num_pages, which the tensor map
+// reads as zeros.
 template <int D>
 __device__ __forceinline__ void load_block(uint8_t* dst, const CUtensorMap* tm,
-                                           const BlockLane<D>& bl, const BoxAt& at, int box, int hk,
-                                           uint64_t* bar) {
-  const unsigned on = __ballot_sync(0xffffffffu, at.page >= 0);
+                                           const BlockLane<D>& bl, BoxAt at, int box, int hk,
+                                           uint64_t* bar, const PagedSeqs& p) {
+  const unsigned on = __ballot_sync(0xffffffffu, at.on);
   if (lane_id() == 0) bar_arrive_expect_tx(bar, (uint32_t)__popc(on) * box * 128u);
   __syncwarp();
-  if (at.page >= 0)
+  if (at.on) {
+    if (at.page < 0 || at.page >= p.num_pages) {
+      report_bad(p.status, kBadPage, at.page);
+      at.page = p.num_pages;
+    }
     tma_load_4d(dst + bl.c * (128 * 128) + bl.sub * box * 128, tm, bl.c * 64, at.slot, hk, at.page,
                 bar);
+  }
   __syncwarp();
+}
+
+// A wait by a whole warp that tests once before it suspends: the phase is often complete already,
+// and the suspending form costs a few hundred cycles even then.
+__device__ __forceinline__ bool wait_soon_warp(uint64_t* bar, uint32_t parity, const WaitGuard& g,
+                                               int where, int detail) {
+  const bool ok = bar_test_wait(smem_u32(bar), parity);
+  if (__all_sync(0xffffffffu, ok)) return true;
+  return wait_bar_warp(bar, parity, g, where, detail);
 }
 
 // Zero rows [valid, 128) of a block ([D/64 chunks][128 rows][128 B]; whole rows, so the swizzle

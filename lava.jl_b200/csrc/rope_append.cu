@@ -215,6 +215,8 @@ struct RopeParams {
 template <typename T, bool HALVES>
 __global__ void __launch_bounds__(kRotThreads) rope_kernel(const RopeParams p) {
   extern __shared__ float2 cs[];      // [n_tok][pairs]
+  griddep_wait();
+  griddep_launch_dependents();
   const int s0 = blockIdx.x * p.n_tok;
   const int b = blockIdx.z;
   const int pairs = p.rot.pairs;
@@ -274,6 +276,8 @@ __global__ void __launch_bounds__(kRotThreads) append_kernel(const AppendParams 
   extern __shared__ float2 cs[];      // [n_tok][pairs]
   __shared__ long long sh_k[kRotTokens], sh_v[kRotTokens];   // cache rows, bytes; -1: left out
   __shared__ int sh_place[kRotTokens];
+  griddep_wait();
+  griddep_launch_dependents();
   const int t0 = blockIdx.x * p.n_tok;
   const int pairs = p.rot.pairs;
   for (int i = warp_id(); i < p.n_tok; i += kRotThreads / 32) {
@@ -407,18 +411,13 @@ int rope_launch(const lvb_rope_desc* d, const long long qs[3], const long long k
                   (unsigned)((heads + p.heads_per_cta - 1) / p.heads_per_cta), (unsigned)d->batch);
   const size_t smem = (size_t)p.n_tok * p.rot.pairs * sizeof(float2);
   const bool halves = d->rot.layout == LVB_ROPE_HALVES;
-  if (d->dtype == LVB_F32) {
-    if (halves) rope_kernel<float, true><<<grid, kRotThreads, smem, stream>>>(p);
-    else rope_kernel<float, false><<<grid, kRotThreads, smem, stream>>>(p);
-  } else if (d->dtype == LVB_F16) {
-    if (halves) rope_kernel<__half, true><<<grid, kRotThreads, smem, stream>>>(p);
-    else rope_kernel<__half, false><<<grid, kRotThreads, smem, stream>>>(p);
-  } else {
-    if (halves) rope_kernel<__nv_bfloat16, true><<<grid, kRotThreads, smem, stream>>>(p);
-    else rope_kernel<__nv_bfloat16, false><<<grid, kRotThreads, smem, stream>>>(p);
-  }
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? LVB_OK : fail_cuda(e, op, "kernel launch");
+  SmemAttr none;
+  auto go = [&](auto kern) {
+    return launch_serial(op, kern, none, dev, grid, kRotThreads, smem, stream, p);
+  };
+  if (d->dtype == LVB_F32) return go(halves ? rope_kernel<float, true> : rope_kernel<float, false>);
+  if (d->dtype == LVB_F16) return go(halves ? rope_kernel<__half, true> : rope_kernel<__half, false>);
+  return go(halves ? rope_kernel<__nv_bfloat16, true> : rope_kernel<__nv_bfloat16, false>);
 }
 
 int append_launch(const lvb_append_desc* d, const PagedLayout& lay, const long long ks[2],
@@ -457,15 +456,12 @@ int append_launch(const lvb_append_desc* d, const PagedLayout& lay, const long l
                   (unsigned)((heads + p.heads_per_cta - 1) / p.heads_per_cta));
   const size_t smem = (size_t)p.n_tok * p.rot.pairs * sizeof(float2);
   const bool halves = d->rot.layout == LVB_ROPE_HALVES;
-  if (g.dtype == LVB_F16) {
-    if (halves) append_kernel<__half, true><<<grid, kRotThreads, smem, stream>>>(p);
-    else append_kernel<__half, false><<<grid, kRotThreads, smem, stream>>>(p);
-  } else {
-    if (halves) append_kernel<__nv_bfloat16, true><<<grid, kRotThreads, smem, stream>>>(p);
-    else append_kernel<__nv_bfloat16, false><<<grid, kRotThreads, smem, stream>>>(p);
-  }
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? LVB_OK : fail_cuda(e, op, "kernel launch");
+  SmemAttr none;
+  auto go = [&](auto kern) {
+    return launch_serial(op, kern, none, dev, grid, kRotThreads, smem, stream, p);
+  };
+  if (g.dtype == LVB_F16) return go(halves ? append_kernel<__half, true> : append_kernel<__half, false>);
+  return go(halves ? append_kernel<__nv_bfloat16, true> : append_kernel<__nv_bfloat16, false>);
 }
 
 }  // namespace lvb
