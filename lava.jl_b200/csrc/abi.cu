@@ -231,7 +231,7 @@ int make_tmap_3d(CUtensorMap* tm, const void* base, int esize, uint64_t inner, u
 }
 
 int make_tmap_nd(CUtensorMap* tm, const void* base, int esize, int rank, const uint64_t* dims,
-                 const uint64_t* strides, const uint32_t* box, const char* op) {
+                 const uint64_t* strides, const uint32_t* box, const char* op, int fetch_bytes) {
   EncodeTiledFn enc = encode_tiled_fn();
   if (!enc) return fail(LVB_ERR_CUDA, op, "cuTensorMapEncodeTiled unavailable", "driver too old");
   if (rank < 1 || rank > 5) return fail(LVB_ERR_INVALID_ARG, op, "tensor map rank");
@@ -245,7 +245,9 @@ int make_tmap_nd(CUtensorMap* tm, const void* base, int esize, int rank, const u
   }
   CUresult r = enc(tm, tma_type(esize), rank, const_cast<void*>(base), d, s, b, e,
                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                   fetch_bytes == 128 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B
+                                      : CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     char buf[160];
     std::snprintf(buf, sizeof buf, "cuTensorMapEncodeTiled(rank %d) failed (%d)", rank, (int)r);

@@ -55,9 +55,11 @@ int paged_kv_maps(CUtensorMap* tk, CUtensorMap* tv, const lvb_paged_desc* d, con
   const uint32_t box[4] = {64, (uint32_t)paged_box(d->page_size), 1, 1};
   const uint64_t sk[3] = {(uint64_t)lay.kc[1], (uint64_t)lay.kc[2], (uint64_t)lay.kc[0]};
   const uint64_t sv[3] = {(uint64_t)lay.vc[1], (uint64_t)lay.vc[2], (uint64_t)lay.vc[0]};
-  int st = make_tmap_nd(tk, Kc, 2, 4, dims, sk, box, op);
+  // A head's row may lie between other heads': fetch no more than it.
+  const int fetch = (int)d->head_dim * 2;
+  int st = make_tmap_nd(tk, Kc, 2, 4, dims, sk, box, op, fetch);
   if (st) return st;
-  return make_tmap_nd(tv, Vc, 2, 4, dims, sv, box, op);
+  return make_tmap_nd(tv, Vc, 2, 4, dims, sv, box, op, fetch);
 }
 
 namespace {

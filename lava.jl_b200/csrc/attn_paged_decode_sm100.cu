@@ -14,16 +14,18 @@
 //     every CTA sums the block counts itself. An item that a run boundary cuts leaves pieces (O, m,
 //     l in 32 bits) in the workspace, at most two per CTA, and the join kernel adds them in a
 //     fixed order; an item inside a run stores its result;
-//   * 352 threads: two softmax warpgroups take the blocks in turn, each with its own S and P
+//   * 384 threads: two softmax warpgroups take the blocks in turn, each with its own S and P
 //     buffer, maxima, sums and O accumulator (thread = key for Sᵀ, = head-dim element for Oᵀ), so
 //     one's chain of waits runs beside the other's; the one with an item's last block joins the
-//     other's O (read from TMEM), m and l to its own. A TMA warp brings Q and the K
-//     and V blocks (a box of slots per page and lane) through a ring that runs ahead across items
-//     and publishes the items; one warp issues the Q·Kᵀ products, one the P·V products;
+//     other's O (read from TMEM), m and l to its own. One warp works out
+//     the items, publishes them and brings Q and the K blocks, one brings the V blocks (a box of
+//     slots per page and lane), through rings that run ahead across items; one warp issues the
+//     Q·Kᵀ products, one the P·V products;
 //   * m of a row moves only when a score exceeds it by 2^8 (p stays <= 256): a block whose scores
 //     all stay below needs no row maximum, only one vote over the warpgroup. In fp16 the exponent
 //     is shifted by 2^6, away from the subnormals (p <= 2^14).
 #include <algorithm>
+#include <climits>
 #include <cmath>
 
 #include "paged.cuh"
@@ -32,11 +34,12 @@ namespace lvb {
 
 namespace {
 
-constexpr int kThreads = 352;
+constexpr int kThreads = 384;
 // Warps 0-3 and 4-7: the softmax warpgroups.
-constexpr int kTmaWarp = 8;
-constexpr int kQkWarp = 9;
-constexpr int kPvWarp = 10;
+constexpr int kTmaWarp = 8;                // the items, Q and the K blocks
+constexpr int kVWarp = 9;                  // the V blocks
+constexpr int kQkWarp = 10;
+constexpr int kPvWarp = 11;
 constexpr int kQueue = 8;                  // items published ahead
 constexpr int kItemCost = 1;               // blocks that an item's start and end count for
 constexpr int kChunk = 128 * 128;          // one 64-element chunk of a 128-key block
@@ -59,21 +62,25 @@ template <int D, int NR>
 struct Cfg {
   static constexpr int kCh = D / 64;
   static constexpr int kBlock = kCh * kChunk;
-  static constexpr int kRing = D == 64 ? 12 : NR == 16 ? 6 : 5;
+  static constexpr int kK = D == 64 ? 6 : 3;             // K ring slots
+  static constexpr int kV = D == 64 ? 6 : NR == 16 ? 3 : 2;   // V ring slots
+  static constexpr int kRing = kK + kV;
   static constexpr int kQ = kCh * NR * 128;            // Q of an item
   static constexpr int kP = 2 * NR * 128;              // P of a block: two 64-key chunks
   static constexpr int kTmemCols = NR == 16 ? 128 : 256;   // S and two O per warpgroup
   static constexpr int kSmem =
-      kRing * kBlock + 2 * kQ + 2 * kP + 2 * 4 * NR * 4 + 2 * NR * 8 + 1536 +
+      kRing * kBlock + 2 * kQ + 2 * kP + 2 * 4 * NR * 4 + 2 * NR * 8 + 2048 +
       kThreads * 12 + 1024;
 };
 
 // What the roles need of an item (a run of key blocks of one sequence and KV head).
 struct Item {
-  int hk, kb0, nblk;        // KV head, first block, blocks
+  int b, hk, kb0, nblk;     // sequence, KV head, first block, blocks
   int len, qlen, tok0;
   int slot;                 // where its piece goes; -1: the whole item, O is stored
   int last;                 // 1: no item, the CTA is done
+  int pad;
+  int entries[32];          // the table's entries from the first block's on
 };
 
 template <bool BF16>
@@ -140,7 +147,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     paged_decode_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                         const __grid_constant__ CUtensorMap tmV, const DecParams p) {
   using C = Cfg<D, NR>;
-  constexpr int R = C::kRing;
+  constexpr int KR = C::kK, VR = C::kV;
   constexpr uint32_t kFmt = BF16 ? 1 : 0;
   constexpr uint32_t kIdescQK = make_idesc(1, kFmt, kFmt, 0, 0, 128, NR);
   constexpr uint32_t kIdescPV = make_idesc(1, kFmt, kFmt, 1, 0, 128, NR);
@@ -148,15 +155,17 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align_1024(smem_raw);
-  uint8_t* sRing = smem;                                  // [R][D/64 chunks][128 keys][128 B]
-  uint8_t* sQ = sRing + R * C::kBlock;                    // [2][D/64 chunks][NR rows][128 B]
+  uint8_t* sRing = smem;                                  // [KR + VR][D/64 chunks][128 keys][128 B]
+  uint8_t* sQ = sRing + C::kRing * C::kBlock;                    // [2][D/64 chunks][NR rows][128 B]
   uint8_t* sP = sQ + 2 * C::kQ;                           // [2][2 chunks][NR rows][128 B]
   float* sXml = reinterpret_cast<float*>(sP + 2 * C::kP); // [2 warpgroups][NR][2] deposited m, l
   float* sRed = sXml + 2 * NR * 2;                        // [2 warpgroups][4 warps][NR]
   uint64_t* bars = reinterpret_cast<uint64_t*>(sRed + 2 * 4 * NR);
-  uint64_t* kv_full = bars;              // [R]
-  uint64_t* kv_empty = kv_full + R;      // [R]
-  uint64_t* q_full = kv_empty + R;       // [2]
+  uint64_t* k_full = bars;               // [KR]
+  uint64_t* k_empty = k_full + KR;       // [KR]
+  uint64_t* v_full = k_empty + KR;       // [VR]
+  uint64_t* v_empty = v_full + VR;       // [VR]
+  uint64_t* q_full = v_empty + VR;       // [2]
   uint64_t* q_empty = q_full + 2;        // [2]
   uint64_t* s_full = q_empty + 2;        // [2] per warpgroup, as all below
   uint64_t* s_empty = s_full + 2;        // [2] (4 warps)
@@ -167,10 +176,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* x_full = o_empty + 4;        // [2] the warpgroup's m and l deposited (4 warps)
   uint64_t* x_empty = x_full + 2;        // [2] they are read (4 warps of the other)
   uint64_t* i_full = x_empty + 2;        // [kQueue] item published
-  uint64_t* i_empty = i_full + kQueue;   // [kQueue] read by the two MMA warps and 8 softmax warps
+  uint64_t* i_empty = i_full + kQueue;   // [kQueue] read by all 12 warps
   uint64_t* drain = i_empty + kQueue;
   Item* items = reinterpret_cast<Item*>(drain + 1);       // [kQueue]
-  int* sScan = reinterpret_cast<int*>(items + kQueue);    // [12]: the warps' sums
+  int* sScan = reinterpret_cast<int*>(items + kQueue);    // [12] the warps' sums
   int* sStart = sScan + 12;                               // the run's sequence and its offset
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sStart + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -181,10 +190,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int G = gridDim.x;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < R; ++s) {
-      bar_init(&kv_full[s], 1);
-      bar_init(&kv_empty[s], 1);
-    }
+    for (int s = 0; s < 2 * C::kRing; ++s) bar_init(&k_full[s], 1);   // all four rings' barriers
     for (int i = 0; i < 2; ++i) {
       bar_init(&q_full[i], 1);
       bar_init(&q_empty[i], 1);
@@ -200,8 +206,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       bar_init(&o_empty[i], 4);
     }
     for (int i = 0; i < kQueue; ++i) {
-      bar_init(&i_full[i], 1);
-      bar_init(&i_empty[i], 10);
+      bar_init(&i_full[i], 33);     // 32 lanes' table entries and the item itself
+      bar_init(&i_empty[i], 12);
     }
     bar_init(drain, 2);
     *abort_flag = 0;
@@ -277,8 +283,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kTmaWarp) {
     // ---------------- producer: items, Q, K and V blocks ----------------
     const BlockLane<D> bl((int)lane, p.box);
-    int n = 0;        // ring slots filled
-    int it = 0;       // items published
+    int n = 0;        // blocks loaded
     bool ok = true;
     int base = 0;     // the lanes hold sequences base .. base+31
     SeqInfo sq{0, 0, 0};
@@ -290,15 +295,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (base + (int)lane < batch) sq = kept ? sSeq[base + lane] : seq_info(p.seqs, base + lane);
       nb_lane = blocks_of(sq);
     };
-    // The item at or after unit u, or false when the run has no further block.
-    struct Next {
-      Item im;
-      const int* row;
-      int id, nb, c1;
-      int end;            // first unit behind it
-    };
-    auto next_item = [&](int u, Next& x) -> bool {
-      while (u < u1) {
+    // Publish the next item with blocks, or the end. The table entries of its first blocks are copied
+    // beside it without waiting: with several items published ahead, short sequences do not wait for
+    // their page numbers one after the other.
+    int u = u0;
+    int pub = 0;
+    bool ended = false;
+    auto publish = [&]() -> bool {
+      const int qi = pub % kQueue;
+      if (!wait_soon_warp(&i_empty[qi], (uint32_t)((pub / kQueue) & 1) ^ 1, g, 70, pub)) return false;
+      Item& im = items[qi];
+      bool found = false;
+      while (u < u1 && !found) {
         int nb = __shfl_sync(0xffffffffu, nb_lane, b - base);
         if (u >= off + units_of(nb)) {
           // the next sequence with blocks (u < total: there is one)
@@ -320,96 +328,124 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int o_item = off + hk * (nb + kItemCost) + kItemCost;   // its first block
         const int kb0 = max(0, u - o_item);
         const int kb1 = min(nb, u1 - o_item);
-        x.end = o_item + nb;
-        if (kb1 <= kb0) {     // the run ends within the item's own cost
-          u = x.end;
-          continue;
-        }
-        x.im.hk = hk;
-        x.im.kb0 = kb0;
-        x.im.nblk = kb1 - kb0;
-        x.im.len = __shfl_sync(0xffffffffu, sq.len, b - base);
-        x.im.qlen = __shfl_sync(0xffffffffu, sq.qlen, b - base);
-        x.im.tok0 = __shfl_sync(0xffffffffu, sq.tok0, b - base);
-        x.im.last = 0;
-        x.nb = nb;
-        x.id = b * p.Hkv + hk;
-        x.row = p.seqs.table + b * p.seqs.table_stride;
-        const int c0 = o_item / share;
-        x.c1 = (o_item + nb - 1) / share;
-        x.im.slot = -1;
+        u = o_item + nb;
+        if (kb1 <= kb0) continue;     // the run ends within the item's own cost
+        found = true;
+        const int len = __shfl_sync(0xffffffffu, sq.len, b - base);
+        const int qlen = __shfl_sync(0xffffffffu, sq.qlen, b - base);
+        const int tok0 = __shfl_sync(0xffffffffu, sq.tok0, b - base);
+        const int id = b * p.Hkv + hk;
+        const int c0 = o_item / share, c1 = (o_item + nb - 1) / share;
         // an item that only this CTA works on is whole; of one that begins in an earlier CTA this
         // is the run's first piece, of the other kind its last
-        if (x.c1 > c0) x.im.slot = 2 * blockIdx.x + ((int)blockIdx.x == c0 ? 1 : 0);
-        else if (p.keep_parts) x.im.slot = 2 * G + x.id;
-        return true;
+        int slot = -1;
+        if (c1 > c0) slot = 2 * blockIdx.x + ((int)blockIdx.x == c0 ? 1 : 0);
+        else if (p.keep_parts) slot = 2 * G + id;
+        const int entry = kb0 * 128 / p.seqs.page_size + (int)lane;
+        if (entry <= (len - 1) / p.seqs.page_size)
+          copy_async4(&im.entries[lane], p.seqs.table + b * p.seqs.table_stride + entry);
+        if (lane == 0) {
+          im.b = b;
+          im.hk = hk;
+          im.kb0 = kb0;
+          im.nblk = kb1 - kb0;
+          im.len = len;
+          im.qlen = qlen;
+          im.tok0 = tok0;
+          im.slot = slot;
+          im.last = 0;
+          if (kb0 == 0)
+            p.tab[id] = make_int4(slot, blockIdx.x + 1, c1, slot < 0 ? kItemDone : kItemPieces);
+        }
       }
-      return false;
+      if (!found) {
+        ended = true;
+        if (lane == 0) im.last = 1;
+      }
+      copy_async_arrive(&i_full[qi]);
+      if (lane == 0) bar_arrive(&i_full[qi]);
+      __syncwarp();
+      ++pub;
+      return true;
     };
-    Next cur, nx;
-    bool have = false;
-    BoxAt at{0, 0, false};
     if (u0 < u1) {
       off = sStart[0];
       b = sStart[1];
       base = b & ~31;
       fetch();
-      have = next_item(u0, cur);
-      if (have) at = box_at(bl, cur.row, cur.im.kb0, cur.im.len, p.box, p.seqs);
     }
-    while (have && ok) {
-      const Item im = cur.im;
-      if (im.kb0 == 0 && lane == 0)
-        p.tab[cur.id] = make_int4(im.slot, blockIdx.x + 1, cur.c1, im.slot < 0 ? kItemDone : kItemPieces);
+    int it = 0;
+    for (; ok; ++it) {
+      if (pub == it && !publish()) { ok = false; break; }
       const int qi = it % kQueue;
-      if (!wait_soon_warp(&i_empty[qi], (uint32_t)((it / kQueue) & 1) ^ 1, g, 70, it)) { ok = false; break; }
-      if (lane == 0) {
-        items[qi] = im;
-        bar_arrive(&i_full[qi]);
-      }
+      if (!wait_soon_warp(&i_full[qi], (uint32_t)((it / kQueue) & 1), g, 75, it)) { ok = false; break; }
+      const Item& im = items[qi];
+      if (im.last) break;
+      const int hk = im.hk, nblk = im.nblk, tok0 = im.tok0;
+      BoxWalk<D> walk;
+      walk.start(bl, p.seqs.table + im.b * p.seqs.table_stride, im.kb0, im.len, p.box,
+                 p.seqs.page_size, im.entries);
+      __syncwarp();
+      if (lane == 0) bar_arrive(&i_empty[qi]);
       const int qb = it & 1;
       if (!wait_soon_warp(&q_empty[qb], (uint32_t)((it >> 1) & 1) ^ 1, g, 51, it)) { ok = false; break; }
       if (lane == 0) {
         bar_arrive_expect_tx(&q_full[qb], C::kCh * p.nrows * 128);
         for (int c = 0; c < C::kCh; ++c)
-          tma_load_3d(sQ + qb * C::kQ + c * NR * 128, &tmQ, c * 64, im.hk * p.group, im.tok0, &q_full[qb]);
+          tma_load_3d(sQ + qb * C::kQ + c * NR * 128, &tmQ, c * 64, hk * p.group, tok0, &q_full[qb]);
       }
       __syncwarp();
-      ++it;
-      bool more = false;
-      for (int kb = im.kb0; kb < im.kb0 + im.nblk && ok; ++kb) {
-        // the next block's page numbers (of this item or the next) are on their way while this
-        // one's slots are waited for
-        BoxAt next{0, 0, false};
-        if (kb + 1 < im.kb0 + im.nblk) {
-          next = box_at(bl, cur.row, kb + 1, im.len, p.box, p.seqs);
-        } else {
-          more = next_item(cur.end, nx);
-          if (more) next = box_at(bl, nx.row, nx.im.kb0, nx.im.len, p.box, p.seqs);
+      for (int j = 0; j < nblk; ++j, ++n) {
+        const BoxAt at = walk.take();
+        const int s = n % KR;
+        if (!wait_soon_warp(&k_empty[s], (uint32_t)((n / KR) & 1) ^ 1, g, 52, n)) { ok = false; break; }
+        load_block<D>(sRing + s * C::kBlock, &tmK, bl, at, p.box, hk, &k_full[s], p.seqs);
+        // publish ahead, two items for one, while their queue slots are free
+        for (int k = 0; k < 2 && !ended && pub < it + kQueue; ++k) {
+          const bool free = bar_test_wait(smem_u32(&i_empty[pub % kQueue]), (uint32_t)((pub / kQueue) & 1) ^ 1);
+          if (!__all_sync(0xffffffffu, free)) break;
+          if (!publish()) { ok = false; break; }
         }
-        for (int v = 0; v < 2; ++v, ++n) {
-          const int s = n % R;
-          if (!wait_soon_warp(&kv_empty[s], (uint32_t)((n / R) & 1) ^ 1, g, 52, n)) { ok = false; break; }
-          load_block<D>(sRing + s * C::kBlock, v ? &tmV : &tmK, bl, at, p.box, im.hk, &kv_full[s], p.seqs);
-        }
-        at = next;
+        if (!ok) break;
       }
-      cur = nx;
-      have = more;
     }
-    if (ok) {
-      const int qi = it % kQueue;
-      if (wait_bar_warp(&i_empty[qi], (uint32_t)((it / kQueue) & 1) ^ 1, g, 70, it) && lane == 0) {
-        items[qi].last = 1;
-        bar_arrive(&i_full[qi]);
-      }
-    } else if (lane == 0) {
+    if (!ok && lane == 0) {
       // Let the copies in flight land before the CTA's shared memory goes away.
-      for (int i = max(0, n - R); i < n; ++i)
-        drain_wait(&kv_full[i % R], (uint32_t)((i / R) & 1), p.timeout_ns);
+      for (int i = max(0, n - KR); i < n; ++i)
+        drain_wait(&k_full[i % KR], (uint32_t)((i / KR) & 1), p.timeout_ns);
       for (int i = max(0, it - 2); i < it; ++i)
         drain_wait(&q_full[i & 1], (uint32_t)((i >> 1) & 1), p.timeout_ns);
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncwarp();
+  } else if (warp == kVWarp) {
+    // ---------------- producer: V blocks of the published items ----------------
+    const BlockLane<D> bl((int)lane, p.box);
+    uint8_t* ring = sRing + KR * C::kBlock;
+    int n = 0;
+    bool ok = true;
+    for (int it = 0; ok; ++it) {
+      const int qi = it % kQueue;
+      if (!wait_soon_warp(&i_full[qi], (uint32_t)((it / kQueue) & 1), g, 74, it)) { ok = false; break; }
+      const Item& im = items[qi];
+      const int last = im.last, hk = im.hk, nblk = im.nblk;
+      BoxWalk<D> walk;
+      if (!last)
+        walk.start(bl, p.seqs.table + im.b * p.seqs.table_stride, im.kb0, im.len, p.box,
+                   p.seqs.page_size, im.entries);
+      __syncwarp();
+      if (lane == 0) bar_arrive(&i_empty[qi]);
+      if (last) break;
+      for (int j = 0; j < nblk; ++j, ++n) {
+        const BoxAt at = walk.take();
+        const int s = n % VR;
+        if (!wait_soon_warp(&v_empty[s], (uint32_t)((n / VR) & 1) ^ 1, g, 59, n)) { ok = false; break; }
+        load_block<D>(ring + s * C::kBlock, &tmV, bl, at, p.box, hk, &v_full[s], p.seqs);
+      }
+    }
+    if (!ok && lane == 0)
+      for (int i = max(0, n - VR); i < n; ++i)
+        drain_wait(&v_full[i % VR], (uint32_t)((i / VR) & 1), p.timeout_ns);
     __syncwarp();
   } else if (warp == kQkWarp || warp == kPvWarp) {
     // ---------------- MMA issuers: the warp waits, one elected lane issues ----------------
@@ -418,24 +454,24 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t p_desc = sdesc_sw128(smem_u32(sP), 16, 1024);
     // V_j, MN-major. 64-wide heads: the second 64 of the product's 128 rows read the same chunk
     // again (leading offset 0) and are never looked at.
-    const uint64_t v_desc = sdesc_sw128(smem_u32(sRing), D == 128 ? kChunk : 0, 1024);
+    uint8_t* v_ring = sRing + KR * C::kBlock;
+    const uint64_t v_desc = sdesc_sw128(smem_u32(v_ring), D == 128 ? kChunk : 0, 1024);
     int gb = 0;       // blocks before this item
-    int wi[2] = {0, 0};   // items that each warpgroup had a block of
+    int wi0 = 0, wi1 = 0; // items that each warpgroup had a block of
     bool ok = true;
     for (int it = 0; ok; ++it) {
       const int qi = it % kQueue;
       if (!wait_bar_warp(&i_full[qi], (uint32_t)((it / kQueue) & 1), g, 71, it)) break;
-      const Item im = items[qi];
+      const int nb = items[qi].nblk, kb0 = items[qi].kb0, len = items[qi].len, last = items[qi].last;
       __syncwarp();
       if (lane == 0) bar_arrive(&i_empty[qi]);
-      if (im.last) break;
-      const int nb = im.nblk;
+      if (last) break;
       if (warp == kQkWarp) {
         const int qb = it & 1;
         if (!wait_soon_warp(&q_full[qb], (uint32_t)((it >> 1) & 1), g, 53, it)) break;
         for (int j = 0; j < nb; ++j) {
-          const int gj = gb + j, w = gj & 1, nk = 2 * gj, sk = nk % R;
-          if (!wait_soon_warp(&kv_full[sk], (uint32_t)((nk / R) & 1), g, 54, nk) ||
+          const int gj = gb + j, w = gj & 1, sk = gj % KR;
+          if (!wait_soon_warp(&k_full[sk], (uint32_t)((gj / KR) & 1), g, 54, gj) ||
               !wait_soon_warp(&s_empty[w], (uint32_t)((gj >> 1) & 1) ^ 1, g, 55, gj)) { ok = false; break; }
           tc_fence_after();
           if (elect_one()) {
@@ -446,20 +482,21 @@ __global__ void __launch_bounds__(kThreads, 1)
               mma_f16_ss(tmem + NR * w, ad + (((kk >> 2) * kChunk + (kk & 3) * 32) >> 4),
                          bd + (((kk >> 2) * NR * 128 + (kk & 3) * 32) >> 4), kIdescQK, kk > 0 ? 1u : 0u);
             mma_commit(&s_full[w]);
-            mma_commit(&kv_empty[sk]);                   // K_j read
+            mma_commit(&k_empty[sk]);                    // K_j read
             if (j == nb - 1) mma_commit(&q_empty[qb]);   // the item's Q read for the last time
           }
           __syncwarp();
         }
       } else {
         for (int j = 0; j < nb; ++j) {
-          const int gj = gb + j, w = gj & 1, nv = 2 * gj + 1, sv = nv % R;
-          const int ob = wi[w] & 1;
-          if (!wait_soon_warp(&kv_full[sv], (uint32_t)((nv / R) & 1), g, 56, nv)) { ok = false; break; }
-          const int valid = im.len - (im.kb0 + j) * 128;
-          if (valid < 128) zero_tail<D>(smem_u32(sRing) + sv * C::kBlock, valid);
+          const int gj = gb + j, w = gj & 1, sv = gj % VR;
+          const int wi = w ? wi1 : wi0;
+          const int ob = wi & 1;
+          if (!wait_soon_warp(&v_full[sv], (uint32_t)((gj / VR) & 1), g, 56, gj)) { ok = false; break; }
+          const int valid = len - (kb0 + j) * 128;
+          if (valid < 128) zero_tail<D>(smem_u32(v_ring) + sv * C::kBlock, valid);
           // the warpgroup's O buffer is free once the epilogue of its last item but one read it
-          if (j < 2 && !wait_soon_warp(&o_empty[2 * w + ob], (uint32_t)((wi[w] >> 1) & 1) ^ 1, g, 58, gj)) { ok = false; break; }
+          if (j < 2 && !wait_soon_warp(&o_empty[2 * w + ob], (uint32_t)((wi >> 1) & 1) ^ 1, g, 58, gj)) { ok = false; break; }
           if (!wait_soon_warp(&p_full[w], (uint32_t)((gj >> 1) & 1), g, 57, gj)) { ok = false; break; }
           tc_fence_after();
           if (elect_one()) {
@@ -471,14 +508,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                          bd + (((kk >> 2) * NR * 128 + (kk & 3) * 32) >> 4), kIdescPV,
                          (j < 2 && kk == 0) ? 0u : 1u);
             mma_commit(&p_empty[w]);
-            mma_commit(&kv_empty[sv]);                   // V_j read
+            mma_commit(&v_empty[sv]);                    // V_j read
             if (j + 2 >= nb) mma_commit(&o_full[2 * w + ob]);   // its last block of the item
           }
           __syncwarp();
         }
       }
-      ++wi[gb & 1];
-      if (nb > 1) ++wi[(gb & 1) ^ 1];
+      wi0 += nb > 1 || !(gb & 1);
+      wi1 += nb > 1 || (gb & 1);
       gb += nb;
     }
     if (elect_one()) mma_commit(drain);
@@ -522,29 +559,32 @@ __global__ void __launch_bounds__(kThreads, 1)
     int gb = 0;       // blocks before this item
     int wi = 0;       // this warpgroup's items before this one
     int wo = 0;       // the other's
-    int xn[2] = {0, 0};   // deposits of each warpgroup before this item
+    int xn0 = 0, xn1 = 0;   // deposits of each warpgroup before this item
     for (int it = 0;; ++it) {
       const int qi = it % kQueue;
       // A wait that gave up leaves the CTA's abort flag up; every thread sees it at its next
       // wait, and the 128 leave together after a vote.
       bool ok = wait_bar(&i_full[qi], (uint32_t)((it / kQueue) & 1), g, 72, it);
       if (vote_any(bar_id, !ok)) break;
-      const Item im = items[qi];
+      const int nb = items[qi].nblk, kb0 = items[qi].kb0, len = items[qi].len;
+      const int qlen = items[qi].qlen, tok0 = items[qi].tok0, hk = items[qi].hk;
+      const int slot = items[qi].slot, last = items[qi].last;
       __syncwarp();
       if (lane == 0) bar_arrive(&i_empty[qi]);
-      if (im.last) break;
-      const int nb = im.nblk;
+      if (last) break;
       const int j0 = (gb & 1) == w ? 0 : 1;             // this warpgroup's first block
       const int depositor = nb > 1 ? (gb + nb) & 1 : -1;   // the one without the last block
-      const int x_before = depositor >= 0 ? xn[depositor]++ : 0;
+      const int x_before = depositor == 1 ? xn1 : xn0;
+      xn0 += depositor == 0;
+      xn1 += depositor == 1;
       if (j0 >= nb) {                                    // the other's only block
         gb += nb;
         ++wo;
         continue;
       }
-      const int n_rows = min(p.nrows, im.qlen * p.group);   // rows r < n_rows are real
+      const int n_rows = min(p.nrows, qlen * p.group);   // rows r < n_rows are real
       // Row r = position·group + head of the group sees keys up to lim0 + position.
-      const int lim0 = p.causal ? im.len - im.qlen : im.len - 1;
+      const int lim0 = p.causal ? len - qlen : len - 1;
       const uint32_t tO = tmem + lane_off + NR * (2 + 2 * w + (wi & 1));
       float m_ref[RR], l_part[RR];
 #pragma unroll
@@ -554,7 +594,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       for (int j = j0; j < nb; j += 2) {
         const int gj = gb + j;
-        const int key = (im.kb0 + j) * 128 + t;
+        const int key = (kb0 + j) * 128 + t;
         const uint32_t ph = (uint32_t)((gj >> 1) & 1);
         if (!wait_soon(&s_full[w], ph, g, 61, gj)) ok = false;
         __syncwarp();
@@ -565,16 +605,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) bar_arrive(&s_empty[w]);
+        // Masked scores. Inside a run of keys that every row sees (and with all RR rows real) there
+        // is nothing to mask; the two forms are apart so that no row's code has a branch.
         float x[RR];
         bool up = false;
-        const bool open = (im.kb0 + j) * 128 + 127 <= lim0;   // every row sees the whole block
+        const bool open = (kb0 + j) * 128 + 127 <= lim0;
+        if (open && n_rows >= RR) {
 #pragma unroll
-        for (int r = 0; r < RR; ++r) {
-          bool see = r < n_rows;
-          if (!open) see = see && key <= lim0 + (p.causal ? row_pos(r) : 0);
-          x[r] = see ? __uint_as_float(sv[r]) * sl : NEG_INF;
-          up |= x[r] > m_ref[r] + kLazy;
+          for (int r = 0; r < RR; ++r) x[r] = __uint_as_float(sv[r]) * sl;
+        } else {
+          // row r sees the key when its position is at least key - lim0
+          const int need = p.causal ? key - lim0 : (key <= lim0 ? 0 : INT_MAX);
+#pragma unroll
+          for (int r = 0; r < RR; ++r)
+            x[r] = r < n_rows && row_pos(r) >= need ? __uint_as_float(sv[r]) * sl : NEG_INF;
         }
+#pragma unroll
+        for (int r = 0; r < RR; ++r) up |= x[r] > m_ref[r] + kLazy;
         if (vote_any(bar_id, up)) {
           // A row's reference moves: the block's row maxima, within the warps and across them.
 #pragma unroll
@@ -619,8 +666,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!wait_soon(&p_empty[w], ph ^ 1, g, 63, gj)) ok = false;
 #pragma unroll
         for (int r = 0; r < RR; ++r) {
-          const float mu = m_ref[r] == NEG_INF ? 0.f : m_ref[r] - kShift;
-          const float pr = fast_exp2(x[r] - mu);
+          // (a row without a key so far: a finite reference, so that -inf gives 0 and NaN stays)
+          const float pr = fast_exp2(x[r] - (fmaxf(m_ref[r], -3.0e38f) - kShift));
           l_part[r] += pr;
           // K-major, 128-byte swizzle: 16-byte unit (key / 8) of row r moves to (key / 8) ^ (r % 8).
           const int unit = ((t & 63) >> 3) ^ (r & 7);
@@ -667,7 +714,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int r = 0; r < RR; ++r) {
           l[r] = (red[r] + red[NR + r]) + (red[2 * NR + r] + red[3 * NR + r]);
-          m[r] = m_ref[r];
+          m[r] = fmaxf(m_ref[r], -3.0e38f);      // finite: 2^(m - m') is 0 or 1, not NaN
         }
         if (both) {
           // the two warpgroups' sums over the larger of their references
@@ -676,11 +723,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_wait_ld();
 #pragma unroll
           for (int r = 0; r < RR; ++r) {
-            const float m2 = sXml[(ww * NR + r) * 2], l2 = sXml[(ww * NR + r) * 2 + 1];
+            const float2 x2 = *reinterpret_cast<const float2*>(&sXml[(ww * NR + r) * 2]);
+            const float m2 = fmaxf(x2.x, -3.0e38f);
             const float mm = fmaxf(m[r], m2);
-            const float mu = mm == NEG_INF ? 0.f : mm;
-            const float a1 = fast_exp2(m[r] - mu), a2 = fast_exp2(m2 - mu);
-            l[r] = l[r] * a1 + l2 * a2;
+            const float a1 = fast_exp2(m[r] - mm), a2 = fast_exp2(m2 - mm);
+            l[r] = l[r] * a1 + x2.y * a2;
             o[r] = __float_as_uint(__uint_as_float(o[r]) * a1 + __uint_as_float(o2[r]) * a2);
             m[r] = mm;
           }
@@ -694,27 +741,30 @@ __global__ void __launch_bounds__(kThreads, 1)
             bar_arrive(&x_empty[ww]);
           }
         }
+        if (slot < 0) {
+          // O = sum / l; thread r of the warpgroup stores row r's lse
+          float my_l = 0.f, my_m = 0.f;
+          uint16_t* base = reinterpret_cast<uint16_t*>(p.O) + tok0 * p.o_st + hk * p.group * p.o_sh + t;
 #pragma unroll
-        for (int r = 0; r < RR; ++r) {
-          if (r >= n_rows) continue;
-          const float ov = __uint_as_float(o[r]);
-          const float mr = m[r] == NEG_INF ? NEG_INF : m[r] - kShift;
-          if (im.slot < 0) {
-            const int pos = row_pos(r);
-            const long long tok = im.tok0 + pos;
-            const int h = im.hk * p.group + r - pos * p.group;
-            const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
-            uint16_t* dst = reinterpret_cast<uint16_t*>(p.O) + tok * p.o_st + h * p.o_sh;
-            if (t < D) dst[t] = bits16<BF16>(ov * inv);
-            if (p.lse && t == 0)
-              p.lse[tok * p.Hq + h] = l[r] == 0.f ? NEG_INF : (mr + log2f(l[r])) * 0.69314718055994530942f;
-          } else {
-            const long long at = (long long)im.slot * NR + r;
-            if (t < D) p.part_o[at * D + t] = ov;
-            if (t == 0) {
-              p.part_ml[at * 2] = mr;
-              p.part_ml[at * 2 + 1] = l[r];
-            }
+          for (int r = 0; r < RR; ++r) {
+            const int pos = row_pos(r), h = r - pos * p.group;
+            const float inv = l[r] == 0.f ? 0.f : __frcp_rn(l[r]);
+            if (r < n_rows && t < D)
+              base[pos * p.o_st + h * p.o_sh] = bits16<BF16>(__uint_as_float(o[r]) * inv);
+            if (t == r) my_l = l[r], my_m = m[r] - kShift;
+          }
+          if (p.lse && t < n_rows) {
+            const int pos = row_pos(t);
+            p.lse[(long long)(tok0 + pos) * p.Hq + hk * p.group + t - pos * p.group] =
+                my_l == 0.f ? NEG_INF : (my_m + log2f(my_l)) * 0.69314718055994530942f;
+          }
+        } else {
+          const long long at = (long long)slot * NR;
+#pragma unroll
+          for (int r = 0; r < RR; ++r) {
+            if (r < n_rows && t < D) p.part_o[(at + r) * D + t] = __uint_as_float(o[r]);
+            if (r < n_rows && t == r)
+              *reinterpret_cast<float2*>(&p.part_ml[(at + r) * 2]) = make_float2(m[r] - kShift, l[r]);
           }
         }
       }

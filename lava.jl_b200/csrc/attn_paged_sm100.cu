@@ -283,13 +283,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       ++qi;
       const int* row = p.seqs.table + b * p.seqs.table_stride;
-      auto box_of = [&](int kb) -> BoxAt {
-        return kb < npb ? box_at(bl, p.seqs.prefix_table, kb, p.prefix, p.box, p.seqs)
-                        : box_at(bl, row, kb - npb, im.len, p.box, p.seqs);
+      // the prefix's blocks, then the sequence's own
+      BoxWalk<D> walk;
+      int kb_next = im.kb0;
+      auto start_run = [&]() {
+        if (kb_next < npb) walk.start(bl, p.seqs.prefix_table, kb_next, p.prefix, p.box, p.seqs.page_size);
+        else walk.start(bl, row, kb_next - npb, im.len, p.box, p.seqs.page_size);
+      };
+      start_run();
+      auto next_box = [&]() -> BoxAt {
+        if (kb_next == npb && kb_next > im.kb0) start_run();
+        ++kb_next;
+        return walk.take();
       };
       // K_j is loaded one block ahead of V_{j-1}: the boxes of the last two blocks are kept, and
       // the next block's page numbers are on their way.
-      BoxAt ak = box_of(im.kb0), av = ak, an = ak;
+      BoxAt ak = next_box(), av = ak, an = ak;
       for (int i = 0; i < 2 * im.n_blocks && ok; ++i, ++rn) {
         // Item i of the ring order: K_0; odd i: K_{(i+1)/2}, or V_{nb-1} for the last;
         // even i > 0: V_{i/2 - 1}.
@@ -298,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int j = (i + 1) / 2;
           av = ak;
           ak = i == 0 ? ak : an;
-          if (j + 1 < im.n_blocks) an = box_of(im.kb0 + j + 1);
+          if (j + 1 < im.n_blocks) an = next_box();
         } else if (i & 1) {
           av = ak;          // the last V: the block of the last K
         }

@@ -55,9 +55,11 @@ int make_tmap_2d_sw(CUtensorMap* tm, const void* base, int esize, uint64_t inner
                     const char* op);
 
 // Rank-n tiled map (n <= 5), 128-byte swizzle. dims/box innermost first; strides[i] is the
-// element stride of dimension i+1.
+// element stride of dimension i+1. `fetch_bytes`: how much L2 fetches from DRAM around a missed
+// sector (128 or 256).
 int make_tmap_nd(CUtensorMap* tm, const void* base, int esize, int rank, const uint64_t* dims,
-                 const uint64_t* strides, const uint32_t* box, const char* op);
+                 const uint64_t* strides, const uint32_t* box, const char* op,
+                 int fetch_bytes = 256);
 
 // 3-D map [outer][rows][inner] with element strides (ld_rows, ld_outer).
 int make_tmap_3d(CUtensorMap* tm, const void* base, int esize, uint64_t inner, uint64_t rows,

@@ -205,26 +205,63 @@ struct BlockLane {
   }
 };
 
-// The page (and slot) of the lane's box in block kb of a run of `len` keys whose pages are
-// row[0 ..]. The page number is only looked at by load_block, so its load may be under way while
-// other work is done.
+// The page and slot of a lane's box.
 struct BoxAt {
   int page, slot;
   bool on;            // the box holds a valid key
 };
+
+// The boxes of one block after the other of a run of `n` keys whose pages are r[0 ..], worked out by
+// a whole warp. The table entries come 32 at a time, one
+// per lane, with the next 32 on their way, and a box's entry is fetched from its lane: under a
+// saturated memory system a table load takes as long as several blocks (measured: every fourth
+// block of a 64-slot-page cache waited 3,000-5,000 clk for its entries when they were loaded one
+// block ahead). Place p + 128 is `whole` pages and `rest` slots on, without a division.
 template <int D>
-__device__ __forceinline__ BoxAt box_at(const BlockLane<D>& bl, const int* row, int kb, int len,
-                                        int box, const PagedSeqs& p) {
-  BoxAt at{0, 0, false};
-  const int key = kb * 128 + bl.sub * box;
-  if (bl.in && key < len) {
-    const int i = key / p.page_size;
-    at.slot = key - i * p.page_size;
-    at.page = row[i];
-    at.on = true;
+struct BoxWalk {
+  const int* row;
+  int key, len, i, slot;
+  int page_size, whole, rest;
+  int w0, last;       // first entry of the window; the run's last entry
+  int cur, nxt;       // this lane's entries of the window and of the one behind it
+  bool in;
+  __device__ __forceinline__ int entry(int k) const { return k <= last ? row[k] : 0; }
+  // `entries`: the run's first 32 entries from block kb on, when they are in shared memory already.
+  __device__ __forceinline__ void start(const BlockLane<D>& bl, const int* r, int kb, int n, int box,
+                                        int psize, const int* entries = nullptr) {
+    row = r;
+    len = n;
+    in = bl.in;
+    page_size = psize;
+    key = kb * 128 + bl.sub * box;
+    i = key / psize;
+    slot = key - i * psize;
+    whole = 128 / psize;
+    rest = 128 - whole * psize;
+    w0 = __shfl_sync(0xffffffffu, i, 0);
+    last = (n - 1) / psize;
+    cur = entries ? entries[lane_id()] : entry(w0 + (int)lane_id());
+    nxt = entry(w0 + 32 + (int)lane_id());
   }
-  return at;
-}
+  __device__ __forceinline__ BoxAt take() {
+    const int at0 = i - w0;               // lanes' entries lie within two windows of lane 0's
+    const int a = __shfl_sync(0xffffffffu, cur, at0 & 31), c = __shfl_sync(0xffffffffu, nxt, at0 & 31);
+    const BoxAt at{at0 < 32 ? a : c, slot, in && key < len};
+    key += 128;
+    i += whole;
+    slot += rest;
+    if (slot >= page_size) {
+      slot -= page_size;
+      ++i;
+    }
+    if (__shfl_sync(0xffffffffu, i, 0) - w0 >= 32) {
+      w0 += 32;
+      cur = nxt;
+      nxt = entry(w0 + 32 + (int)lane_id());
+    }
+    return at;
+  }
+};
 
 // Issue one block's loads into `dst` ([D/64 chunks][128 rows][128 B], 128-byte swizzle) on
 // `bar`; the whole warp calls it. A bad page number becomes num_pages, which the tensor map
@@ -245,6 +282,15 @@ __device__ __forceinline__ void load_block(uint8_t* dst, const CUtensorMap* tm,
                 bar);
   }
   __syncwarp();
+}
+
+// A 4-byte copy to shared memory that the thread does not wait for, and the arrival (one of the
+// barrier's count) once this thread's copies so far have landed.
+__device__ __forceinline__ void copy_async4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
 // A wait by a whole warp that tests once before it suspends: the phase is often complete already,
