@@ -358,8 +358,8 @@ int lvb_attention_paged(const lvb_paged_desc* d, const void* Q, const void* Kc, 
     }
     DecodeWorkspace dw = {};
     if (st == LVB_OK)
-      st = paged_decode_launch(d, lay, mp.seqs, Q, Kc, Vc, O, lse, pl.prefix_splits > 0, ws + fb,
-                               &dw, s, dev);
+      st = paged_decode_launch(d, lay, mp.seqs, Q, Kc, Vc, O, lse, pl.prefix_splits > 0,
+                               pl.prefix_splits > 0, ws + fb, &dw, s, dev);
     mp.dec_o = dw.part_o;
     mp.dec_ml = dw.part_ml;
     mp.dec_tab = dw.tab;

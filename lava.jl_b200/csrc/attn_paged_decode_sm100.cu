@@ -9,7 +9,7 @@
 // product (the tensor core takes both operands in one 16-bit type); l sums the unrounded p.
 //
 //   * the 128-key blocks of all (sequence, KV head) items, one after the other, are dealt to the
-//     CTAs in equal contiguous runs (an item also counts kItemCost blocks for its start and end), so
+//     CTAs in equal contiguous runs (an item also counts some blocks for its start and end), so
 //     lengths from one key to the whole cache load the SMs evenly. The lengths are on the device:
 //     every CTA sums the block counts itself. An item that a run boundary cuts leaves pieces (O, m,
 //     l in 32 bits) in the workspace, at most two per CTA, and the join kernel adds them in a
@@ -41,13 +41,18 @@ constexpr int kVWarp = 9;                  // the V blocks
 constexpr int kQkWarp = 10;
 constexpr int kPvWarp = 11;
 constexpr int kQueue = 8;                  // items published ahead
-constexpr int kItemCost = 1;               // blocks that an item's start and end count for
+// Blocks that an item's start and end count for when the blocks are dealt out: the time of three
+// 128-wide blocks, six 64-wide ones (measured on ragged batches: drafts over 64-wide heads 42.6 us
+// with 1, 33.7 with 4, 32.3 with 6; 61 sequences of 128-wide heads 107.3 with 1, 103.7 with 3).
+template <int D>
+constexpr int kItemCost = 384 / D;
 constexpr int kChunk = 128 * 128;          // one 64-element chunk of a 128-key block
 constexpr float kLazy = 8.f;               // log2 units a score may exceed the reference maximum
 
 struct DecParams {
   PagedSeqs seqs;
   int Hq, Hkv, group, nrows, causal, box, keep_parts;
+  int late_wait;            // 1: runs beside the kernel before it (see the kernel's start)
   float scale_log2;
   void* O;
   long long o_st, o_sh;
@@ -224,18 +229,21 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 
   // The setup above may run while the stream's previous kernel ends; the join kernel, which reads
-  // this one's results after its own wait, may be scheduled from here on.
-  griddep_wait();
+  // this one's results after its own wait, may be scheduled from here on. When the kernel before
+  // this one is the same call's over the prefix, the two share only inputs, which that kernel has
+  // waited for: this one then takes the SMs as they become free and waits at its end, so that its
+  // own end is that kernel's too.
+  if (!p.late_wait) griddep_wait();
   griddep_launch_dependents();
 
   // ---------------- this CTA's run of blocks ----------------
   // Thread i sums the costs of sequences [i·per, (i+1)·per); a scan over the threads gives the
   // total and the thread whose sequences hold the run's first unit. An item's units are its
-  // kItemCost, then its blocks.
+  // kItemCost<D>, then its blocks.
   const int batch = p.seqs.batch;
   const int per = (batch + kThreads - 1) / kThreads;
   const int sb0 = min((int)threadIdx.x * per, batch), sb1 = min(sb0 + per, batch);
-  auto units_of = [&](int nb) -> int { return nb ? (nb + kItemCost) * p.Hkv : 0; };
+  auto units_of = [&](int nb) -> int { return nb ? (nb + kItemCost<D>) * p.Hkv : 0; };
   const bool kept = batch <= kThreads;     // one sequence per thread: the producer reads them here
   int mine = 0;
   for (int b = sb0; b < sb1; ++b) {
@@ -324,8 +332,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           nb = __shfl_sync(0xffffffffu, nb_lane, b - base);
         }
-        const int hk = (u - off) / (nb + kItemCost);
-        const int o_item = off + hk * (nb + kItemCost) + kItemCost;   // its first block
+        const int hk = (u - off) / (nb + kItemCost<D>);
+        const int o_item = off + hk * (nb + kItemCost<D>) + kItemCost<D>;   // its first block
         const int kb0 = max(0, u - o_item);
         const int kb1 = min(nb, u1 - o_item);
         u = o_item + nb;
@@ -775,6 +783,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
 
+  if (p.late_wait) griddep_wait();
   tc_fence_before();
   __syncthreads();
   if (warp == kQkWarp) {
@@ -825,8 +834,8 @@ size_t paged_decode_workspace(const lvb_paged_desc* d, int sm_count, bool keep_p
 
 int paged_decode_launch(const lvb_paged_desc* d, const PagedLayout& lay, const PagedSeqs& seqs,
                         const void* Q, const void* Kc, const void* Vc, void* O, float* lse,
-                        bool keep_parts, void* ws, DecodeWorkspace* out, cudaStream_t stream,
-                        DeviceState* dev) {
+                        bool keep_parts, bool after_prefix, void* ws, DecodeWorkspace* out,
+                        cudaStream_t stream, DeviceState* dev) {
   const char* op = "lvb_attention_paged";
   DecParams p = {};
   p.seqs = seqs;
@@ -837,6 +846,7 @@ int paged_decode_launch(const lvb_paged_desc* d, const PagedLayout& lay, const P
   p.causal = d->causal ? 1 : 0;
   p.box = paged_box(d->page_size);
   p.keep_parts = keep_parts ? 1 : 0;
+  p.late_wait = after_prefix ? 1 : 0;
   p.scale_log2 = d->scale * 1.4426950408889634f;
   p.O = O;
   p.o_st = lay.o[0];

@@ -781,7 +781,7 @@ int64_t most_items(const lvb_paged_desc* d, int parts) {
 }  // namespace
 
 // Key ranges per tile pair: with fewer items than SMs, as many as fill the SMs once, of at least
-// four blocks of the longest run of keys (the prefix's length; a table's row otherwise).
+// two blocks of the longest run of keys (the prefix's length; a table's row otherwise).
 int paged_flash_splits(const lvb_paged_desc* d, int sm_count, int parts) {
   const int64_t items = std::max<int64_t>(1, most_items(d, parts));
   int64_t keys = 0;
@@ -789,7 +789,7 @@ int paged_flash_splits(const lvb_paged_desc* d, int sm_count, int parts) {
   if (parts & kFlashOwn) keys += d->table_width * d->page_size;
   const int64_t blocks = (keys + 127) / 128;
   int64_t s = std::max(1, sm_count) / items;
-  s = std::min<int64_t>(s, blocks / 4);
+  s = std::min<int64_t>(s, blocks / 2);
   return (int)std::max<int64_t>(1, s);
 }
 

@@ -140,9 +140,11 @@ struct DecodeWorkspace {
 };
 size_t paged_decode_workspace(const lvb_paged_desc* d, int sm_count, bool keep_parts);
 // keep_parts: every item's result stays in the workspace for the join with a prefix's parts.
+// after_prefix: the kernel before it is the same call's flash kernel over the prefix.
 int paged_decode_launch(const lvb_paged_desc* d, const PagedLayout& lay, const PagedSeqs& seqs,
                         const void* Q, const void* Kc, const void* Vc, void* O, float* lse,
-                        bool keep_parts, void* ws, DecodeWorkspace* out, cudaStream_t stream,
+                        bool keep_parts, bool after_prefix, void* ws, DecodeWorkspace* out,
+                        cudaStream_t stream,
                         DeviceState* dev);
 
 // The flash kernel over the prefix's keys, the sequences' own, or both one after the other.
@@ -244,9 +246,15 @@ struct BoxWalk {
     nxt = entry(w0 + 32 + (int)lane_id());
   }
   __device__ __forceinline__ BoxAt take() {
-    const int at0 = i - w0;               // lanes' entries lie within two windows of lane 0's
-    const int a = __shfl_sync(0xffffffffu, cur, at0 & 31), c = __shfl_sync(0xffffffffu, nxt, at0 & 31);
-    const BoxAt at{at0 < 32 ? a : c, slot, in && key < len};
+    // the lanes' entries lie within two windows of lane 0's; the second is only looked at (and so
+    // waited for) once a lane needs it
+    const int at0 = i - w0;
+    int page = __shfl_sync(0xffffffffu, cur, at0 & 31);
+    if (__any_sync(0xffffffffu, at0 >= 32)) {
+      const int c = __shfl_sync(0xffffffffu, nxt, at0 & 31);
+      if (at0 >= 32) page = c;
+    }
+    const BoxAt at{page, slot, in && key < len};
     key += 128;
     i += whole;
     slot += rest;
