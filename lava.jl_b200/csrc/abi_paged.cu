@@ -366,6 +366,9 @@ int lvb_attention_paged(const lvb_paged_desc* d, const void* Q, const void* Kc, 
     mp.dec_rows = dw.rows;
     mp.dec_slots = dw.slots;
     mp.dec_ctas = dw.ctas;
+    // about as many pieces per item as there are CTAs for each, and one more
+    const int pieces = dw.ctas / (int)(d->batch * d->heads_kv) + 2 + pl.prefix_splits;
+    mp.warps_per_row = pieces <= 8 ? 1 : pieces <= 16 ? 2 : 4;
     if (st == LVB_OK) st = merge_launch(mp, (int)d->head_dim, bf16, s, dev);
   } else {
     const int parts = kFlashOwn | (d->prefix_len ? kFlashPrefix : 0);
@@ -374,6 +377,7 @@ int lvb_attention_paged(const lvb_paged_desc* d, const void* Q, const void* Kc, 
       mp.tile_o = fw.tile_o;
       mp.tile_ml = fw.tile_ml;
       mp.tile_splits = pl.splits;
+      mp.warps_per_row = pl.splits <= 8 ? 1 : pl.splits <= 16 ? 2 : 4;
       mp.pairs_per_seq = (int)((d->max_q + 2 * mp.ppt - 1) / (2 * mp.ppt));
       st = merge_launch(mp, (int)d->head_dim, bf16, s, dev);
     }

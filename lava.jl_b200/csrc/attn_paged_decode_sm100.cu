@@ -150,7 +150,8 @@ __device__ __forceinline__ int blocks_of(const SeqInfo& s) {
 template <int D, int NR, int RR, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_decode_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                        const __grid_constant__ CUtensorMap tmV, const DecParams p) {
+                        const __grid_constant__ CUtensorMap tmV,
+                        const __grid_constant__ DecParams p) {
   using C = Cfg<D, NR>;
   constexpr int KR = C::kK, VR = C::kV;
   constexpr uint32_t kFmt = BF16 ? 1 : 0;

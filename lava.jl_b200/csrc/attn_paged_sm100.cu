@@ -650,18 +650,25 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // ----------------------------------------------------------------------------------------
 // The join: O = Σ 2^(m_s - m) O_s / Σ 2^(m_s - m) l_s, m = max m_s, over a row's parts in a fixed
-// order (the prefix's or the tile's key ranges, then the decoding kernel's pieces). One warp per
-// row, D/32 elements per lane. Bound by the latency of its loads (the lists, the item's table
-// entry, the parts), so the parts' rows are loaded beside their (m, l), before their weights are
-// known.
+// order (the prefix's or the tile's key ranges, then the decoding kernel's pieces). One, two or
+// four warps per row, eight parts each at a time, D/32 elements per lane. Bound by the latency of
+// its loads (the lists, the item's table entry, the parts), so the parts' rows are loaded beside
+// their (m, l), before their weights are known, and rows of many parts take several warps.
 // ----------------------------------------------------------------------------------------
+constexpr int kMergeThreads = 128;
+
 template <int D, bool BF16>
-__global__ void __launch_bounds__(256) merge_kernel(const MergeParams p, int rows) {
+__global__ void __launch_bounds__(kMergeThreads) merge_kernel(const MergeParams p, int rows) {
   constexpr int V = D / 32;            // elements per lane
+  __shared__ float2 sh_ml[4];
+  __shared__ float sh_acc[4][D];
   const int lane = lane_id();
+  const int warp = warp_id();
   griddep_launch_dependents();
-  // one row per warp: (sequence, position, head)
-  const int row = blockIdx.x * 8 + warp_id();
+  // row = (sequence, position, head); a row's warps lie side by side
+  const int wpr = p.warps_per_row;
+  const int row = (blockIdx.x * 4 + warp) / wpr;
+  const int sub = warp & (wpr - 1);
   const int bq = row / p.Hq;
   const int h = row - bq * p.Hq;
   const int b = bq / p.seqs.max_q;
@@ -670,54 +677,50 @@ __global__ void __launch_bounds__(256) merge_kernel(const MergeParams p, int row
   // warp waits for it, so that this grid's end is also that kernel's.
   SeqInfo s{0, 0, 0};
   if (row < rows) s = seq_info(p.seqs, b);
-  griddep_wait();
-  if (pos >= s.qlen) return;
+  bool on = pos < s.qlen;
   const long long tok = s.tok0 + pos;
   const int hk = h / p.group, gh = h - hk * p.group;
   // where the parts are
   const int nt = p.tile_splits;
   long long tile0 = 0;
   if (nt) {
-    const long long at = p.pairs_per_seq ? pos : tok;
-    const int in_pair = (int)(at % (2 * p.ppt));
+    const int at = p.pairs_per_seq ? pos : (int)tok;
+    const int in_pair = at % (2 * p.ppt);
     const long long pair = at / (2 * p.ppt) + (long long)b * p.pairs_per_seq;
     const int t = in_pair / p.ppt;
     tile0 = (pair * p.Hkv + hk) * nt * 256 + t * 128 + (in_pair - t * p.ppt) * p.group + gh;
   }
+  griddep_wait();
   int nd = 0, first_slot = 0, next_c = 0;
-  if (p.dec_tab) {
+  if (p.dec_tab && on) {
     const int4 e = p.dec_tab[b * p.Hkv + hk];
     if (e.w == kItemPieces && e.x >= 0 && e.x < p.dec_slots && e.y > 0 && e.z < p.dec_ctas) {
       first_slot = e.x;
       next_c = e.y;
       nd = 1 + max(0, e.z - e.y + 1);
     } else if (e.w != kItemNoKeys || !nt) {
-      return;                            // the decoding kernel has stored the row
+      on = false;                        // the decoding kernel has stored the row
     }
   }
   const int dec_row = pos * p.group + gh;
-  auto row_of = [&](int i) -> long long {    // part i's row: >= 0 in tile_o, else ~row in dec_o
-    if (i < nt) return tile0 + (long long)i * 256;
-    const int k = i - nt;
-    const long long slot = k == 0 ? first_slot : 2 * (next_c + k - 1);
-    return ~(slot * p.dec_rows + dec_row);
-  };
-  const int n = nt + nd;
-  // Part by part in chunks of eight, whose rows are all under way at once, beside their (m, l): a
-  // running maximum m, and sums relative to it. A part without a key has l = 0 and an O that
+  const int n = on ? nt + nd : 0;
+  // A running maximum m, and sums relative to it. A part without a key has l = 0 and an O that
   // nothing wrote: its weight is 0 and its row is dropped.
   float m = -INFINITY, den = 0.f;
   float acc[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) acc[e] = 0.f;
-  for (int i0 = 0; i0 < n; i0 += 8) {
+  for (int i0 = 8 * sub; i0 < n; i0 += 8 * wpr) {
     float v[8][V];
     float2 ml[8];
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
-      const long long r = row_of(min(i0 + q, n - 1));
-      const float* src = (r >= 0 ? p.tile_o + r * D : p.dec_o + ~r * D) + lane * V;
-      ml[q] = *reinterpret_cast<const float2*>(r >= 0 ? p.tile_ml + 2 * r : p.dec_ml + 2 * ~r);
+      const int i = min(i0 + q, n - 1), k = i - nt;
+      const bool tile = k < 0;
+      const long long slot = k <= 0 ? first_slot : 2 * (next_c + k - 1);
+      const long long r = tile ? tile0 + (long long)i * 256 : slot * p.dec_rows + dec_row;
+      ml[q] = *reinterpret_cast<const float2*>((tile ? p.tile_ml : p.dec_ml) + 2 * r);
+      const float* src = (tile ? p.tile_o : p.dec_o) + r * D + lane * V;
       if constexpr (V == 4) {
         const float4 f = *reinterpret_cast<const float4*>(src);
         v[q][0] = f.x, v[q][1] = f.y, v[q][2] = f.z, v[q][3] = f.w;
@@ -744,14 +747,36 @@ __global__ void __launch_bounds__(256) merge_kernel(const MergeParams p, int row
     }
     m = mn;
   }
-  const float mu = m == -INFINITY ? 0.f : m;
+  if (wpr > 1) {
+    // the row's warps: sums relative to the largest of their maxima
+    sh_ml[warp] = make_float2(m, den);
+#pragma unroll
+    for (int e = 0; e < V; ++e) sh_acc[warp][lane * V + e] = acc[e];
+    __syncthreads();
+    if (sub) return;
+    float mn = m;
+    for (int q = 1; q < wpr; ++q) mn = fmaxf(mn, sh_ml[warp + q].x);
+    const float mu = mn == -INFINITY ? 0.f : mn;
+    const float keep = exp2f(m - mu);
+    den *= keep;
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] *= keep;
+    for (int q = 1; q < wpr; ++q) {
+      const float wq = exp2f(sh_ml[warp + q].x - mu);
+      den += wq * sh_ml[warp + q].y;
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] += wq * sh_acc[warp + q][lane * V + e];
+    }
+    m = mn;
+  }
+  if (!on) return;
   const float inv = den == 0.f ? 0.f : 1.f / den;
   uint16_t* dst = reinterpret_cast<uint16_t*>(p.O) + tok * p.o_st + h * p.o_sh + lane * V;
 #pragma unroll
   for (int e = 0; e < V; e += 2)
     *reinterpret_cast<uint32_t*>(dst + e) = pack2<BF16>(acc[e] * inv, acc[e + 1] * inv);
   if (p.lse && lane == 0)
-    p.lse[tok * p.Hq + h] = den == 0.f ? -INFINITY : (mu + log2f(den)) * 0.69314718055994530942f;
+    p.lse[tok * p.Hq + h] = den == 0.f ? -INFINITY : (m + log2f(den)) * 0.69314718055994530942f;
 }
 
 template <int D, bool BF16>
@@ -855,13 +880,13 @@ int paged_flash_launch(const lvb_paged_desc* d, const PagedLayout& lay, const Pa
 int merge_launch(const MergeParams& p, int D, bool bf16, cudaStream_t stream, DeviceState* dev) {
   const char* op = "lvb_attention_paged";
   const int rows = p.seqs.batch * p.seqs.max_q * p.Hq;
-  const dim3 grid((unsigned)((rows + 7) / 8));
+  const dim3 grid((unsigned)(((long long)rows * p.warps_per_row + 3) / 4));
   SmemAttr none;
   if (D == 128)
-    return bf16 ? launch_serial(op, merge_kernel<128, true>, none, dev, grid, 256, 0, stream, p, rows)
-                : launch_serial(op, merge_kernel<128, false>, none, dev, grid, 256, 0, stream, p, rows);
-  return bf16 ? launch_serial(op, merge_kernel<64, true>, none, dev, grid, 256, 0, stream, p, rows)
-              : launch_serial(op, merge_kernel<64, false>, none, dev, grid, 256, 0, stream, p, rows);
+    return bf16 ? launch_serial(op, merge_kernel<128, true>, none, dev, grid, kMergeThreads, 0, stream, p, rows)
+                : launch_serial(op, merge_kernel<128, false>, none, dev, grid, kMergeThreads, 0, stream, p, rows);
+  return bf16 ? launch_serial(op, merge_kernel<64, true>, none, dev, grid, kMergeThreads, 0, stream, p, rows)
+              : launch_serial(op, merge_kernel<64, false>, none, dev, grid, kMergeThreads, 0, stream, p, rows);
 }
 
 }  // namespace lvb

@@ -123,6 +123,7 @@ struct MergeParams {
   const int4* dec_tab;         // [batch·Hkv]; NULL: none
   int dec_rows;
   int dec_slots, dec_ctas;     // bounds of the table's entries
+  int warps_per_row;           // 1, 2 or 4
   void* O;
   long long o_st, o_sh;
   float* lse;
