@@ -432,8 +432,8 @@ int lvb_rope(const lvb_rope_desc* d, const void* Q, const void* K, void* Qo, voi
  * block table. Place p of sequence b is slot p % page_size of page table[b][p / page_size].
  * The new tokens of all sequences are packed: sequence b's rows are cu_q[b] .. cu_q[b+1]-1 of
  * K, V, Q and O ([token][head][head_dim]), and they stand at its last places, seq_lens[b] -
- * q_len .. seq_lens[b] - 1 (seq_lens counts them). Rows behind cu_q[batch] are neither read nor
- * written. table, seq_lens, cu_q and prefix_table are int32 device arrays read by the kernels
+ * q_len .. seq_lens[b] - 1 (seq_lens counts them). Rows behind cu_q[batch] are left as they
+ * were. table, seq_lens, cu_q and prefix_table are int32 device arrays read by the kernels
  * (a captured graph sees what they hold at its replay), so what they hold is checked there and
  * reported through lvb_device_status as LVB_ERR_INVALID_ARG, with the call's effect limited:
  * site 81, a length that is negative or beyond the table's row (counts as 0); site 82, a page

@@ -167,27 +167,22 @@ struct SeqInfo {
   int len;    // keys in the cache
 };
 
-// (LVB_ERR_INVALID_ARG is 1; the check costs a few integer operations per sequence.)
-__device__ __forceinline__ SeqInfo seq_info(const PagedSeqs& p, int b) {
-  SeqInfo s;
-  s.len = p.lens[b];
-  if (p.cu_q) {
-    s.tok0 = p.cu_q[b];
-    const long long q = (long long)p.cu_q[b + 1] - s.tok0;
-    s.qlen = (int)q;
-    if (q < 0 || q > p.max_q || s.tok0 < 0 || s.tok0 + q > p.tokens) {
-      report_bad(p.status, kBadRows, b);
-      s.qlen = 0;
-    }
-  } else {
-    s.tok0 = b * p.max_q;
-    s.qlen = p.max_q;
-  }
-  if (s.len < 0 || s.len > (long long)p.table_width * p.page_size) {
+// Sequence b from its length and row offsets as the lists have them.
+__device__ __forceinline__ SeqInfo seq_checked(const PagedSeqs& p, int b, int len, int row0, int row1) {
+  SeqInfo s{row0, 0, len};
+  const long long q = (long long)row1 - row0;
+  if (q < 0 || q > p.max_q || row0 < 0 || row1 > p.tokens) report_bad(p.status, kBadRows, b);
+  else s.qlen = (int)q;
+  if (len < 0 || len > (long long)p.table_width * p.page_size) {
     report_bad(p.status, kBadLength, b);
     s.len = 0;
   }
   return s;
+}
+__device__ __forceinline__ SeqInfo seq_info(const PagedSeqs& p, int b) {
+  const int row0 = p.cu_q ? p.cu_q[b] : b * p.max_q;
+  const int row1 = p.cu_q ? p.cu_q[b + 1] : row0 + p.max_q;
+  return seq_checked(p, b, p.lens[b], row0, row1);
 }
 
 // ----------------------------------------------------------------------------------------

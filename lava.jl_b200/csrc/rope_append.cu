@@ -19,8 +19,12 @@ namespace lvb {
 namespace {
 
 constexpr int kRotThreads = 256;
+constexpr int kRotCtas = 4;           // per SM: 64 registers a thread
 constexpr int kRotTokens = 16;        // most tokens per CTA
-constexpr int kRotUnroll = 4;         // heads whose loads a thread has in flight
+// Heads that a thread has under way at a time. Two, with four CTAs per SM, against one with five,
+// three or four with three: a video clip's gradient 18.6 us against 22.3, 20.9 and 22.0; prompts into
+// the cache 17.1 against 16.5, 16.3 and 16.3; 268 MB of Q and K 87.0 against 93.2, 88.5 and 86.1.
+constexpr int kRotUnroll = 2;
 
 struct RotArgs {
   int pairs, layout, n_axes, inverse;
@@ -28,13 +32,6 @@ struct RotArgs {
   const double* freqs;
   const int* pos;                     // NULL: the token's place (append)
   long long pos_axis;
-};
-
-// A tensor's rows for one token: base + head·stride.
-struct HeadRows {
-  const uint8_t* src;
-  uint8_t* dst;
-  long long src_h, dst_h;             // bytes
 };
 
 __device__ __forceinline__ int axis_of(const RotArgs& r, int pair) {
@@ -128,34 +125,46 @@ __device__ __forceinline__ void rotate2(uint4& u, uint4& v, const float (&c)[Vec
   v = Vec<T>::pack(b);
 }
 
-// Heads h0 + hl, + step, ... < h1 of one tensor, vectors at element offsets o0 and o1 of a head.
+// A thread's heads h, h + step, ... < h1 of a list of heads (`rows(h)` gives where head h comes from
+// and goes to, and whether it turns), two vectors at element offsets o0 and o1 each, kRotUnroll
+// heads at a time. The first batch is loaded before the CTA works out its angles and places, so
+// that this chain of loads runs beside it.
 template <typename T, bool HALVES>
-__device__ __forceinline__ void walk_heads(const HeadRows& r, int h, int h1, int step, int o0,
-                                           int o1, bool turns, const float (&c)[Vec<T>::N],
-                                           const float (&s)[Vec<T>::N]) {
-  for (; h < h1; h += kRotUnroll * step) {
-    uint4 u[kRotUnroll], v[kRotUnroll];
+struct HeadWalk {
+  uint4 u[kRotUnroll], v[kRotUnroll];
+  int h, h1, step, o0, o1;
+  template <typename Src>
+  __device__ __forceinline__ void load(const Src& src) {
 #pragma unroll
     for (int k = 0; k < kRotUnroll; ++k) {
       const int hk = h + k * step;
       if (hk < h1) {
-        const T* p = reinterpret_cast<const T*>(r.src + hk * r.src_h);
+        const T* p = reinterpret_cast<const T*>(src(hk));
         u[k] = *reinterpret_cast<const uint4*>(p + o0);
         v[k] = *reinterpret_cast<const uint4*>(p + o1);
       }
     }
+  }
+  template <typename Src, typename Dst, typename Turns>
+  __device__ __forceinline__ void finish(const Src& src, const Dst& dst, const Turns& turns,
+                                         const float (&c)[Vec<T>::N], const float (&s)[Vec<T>::N]) {
+    while (true) {
 #pragma unroll
-    for (int k = 0; k < kRotUnroll; ++k) {
-      const int hk = h + k * step;
-      if (hk < h1) {
-        if (turns) rotate2<T, HALVES>(u[k], v[k], c, s);
-        T* p = reinterpret_cast<T*>(r.dst + hk * r.dst_h);
-        *reinterpret_cast<uint4*>(p + o0) = u[k];
-        *reinterpret_cast<uint4*>(p + o1) = v[k];
+      for (int k = 0; k < kRotUnroll; ++k) {
+        const int hk = h + k * step;
+        if (hk < h1) {
+          if (turns(hk)) rotate2<T, HALVES>(u[k], v[k], c, s);
+          T* p = reinterpret_cast<T*>(dst(hk));
+          *reinterpret_cast<uint4*>(p + o0) = u[k];
+          *reinterpret_cast<uint4*>(p + o1) = v[k];
+        }
       }
+      h += kRotUnroll * step;
+      if (h >= h1) break;
+      load(src);
     }
   }
-}
+};
 
 // A thread's place in its CTA: token i of the CTA's, vector pair j of a head, and the first of
 // the heads it walks (step `hpp`).
@@ -213,13 +222,28 @@ struct RopeParams {
 };
 
 template <typename T, bool HALVES>
-__global__ void __launch_bounds__(kRotThreads) rope_kernel(const RopeParams p) {
+__global__ void __launch_bounds__(kRotThreads, kRotCtas) rope_kernel(const RopeParams p) {
   extern __shared__ float2 cs[];      // [n_tok][pairs]
   griddep_wait();
   griddep_launch_dependents();
   const int s0 = blockIdx.x * p.n_tok;
   const int b = blockIdx.z;
   const int pairs = p.rot.pairs;
+  const Lane l(p.n_tok, p.tasks);
+  const long long s = s0 + l.i;
+  const bool on = l.on && s < p.S;
+  // The CTA's heads of the list Q heads, K heads.
+  const int h0 = blockIdx.y * p.heads_per_cta;
+  HeadWalk<T, HALVES> walk;
+  const bool turns = lane_vectors<T, HALVES>(l.j, pairs, walk.o0, walk.o1);
+  walk.h = h0 + l.hl;
+  walk.h1 = on ? min(h0 + p.heads_per_cta, p.Hq + p.Hkv) : 0;
+  walk.step = l.hpp;
+  const long long qs = b * p.q[0] + s * p.q[2], ks = b * p.k[0] + s * p.k[2];
+  const long long qd = b * p.qo[0] + s * p.qo[2], kd = b * p.ko[0] + s * p.ko[2];
+  auto src = [&](int h) { return h < p.Hq ? p.Q + qs + h * p.q[1] : p.K + ks + (h - p.Hq) * p.k[1]; };
+  auto dst = [&](int h) { return h < p.Hq ? p.Qo + qd + h * p.qo[1] : p.Ko + kd + (h - p.Hq) * p.ko[1]; };
+  walk.load(src);
   for (int x = threadIdx.x; x < p.n_tok * pairs; x += kRotThreads) {
     const int i = x / pairs, pr = x - i * pairs;
     if (s0 + i < p.S) {
@@ -229,22 +253,10 @@ __global__ void __launch_bounds__(kRotThreads) rope_kernel(const RopeParams p) {
     }
   }
   __syncthreads();
-  const Lane l(p.n_tok, p.tasks);
-  const long long s = s0 + l.i;
-  if (!l.on || s >= p.S) return;
-  int o0, o1;
-  const bool turns = lane_vectors<T, HALVES>(l.j, pairs, o0, o1);
+  if (!on) return;
   float c[Vec<T>::N], sn[Vec<T>::N];
   lane_angles<T>(cs, l.i, l.j, pairs, turns, c, sn);
-  // The CTA's heads of the list Q heads, K heads.
-  const int h0 = blockIdx.y * p.heads_per_cta;
-  const int h1 = min(h0 + p.heads_per_cta, p.Hq + p.Hkv);
-  const HeadRows rq{p.Q + b * p.q[0] + s * p.q[2], p.Qo + b * p.qo[0] + s * p.qo[2], p.q[1], p.qo[1]};
-  walk_heads<T, HALVES>(rq, h0 + l.hl, min(h1, p.Hq), l.hpp, o0, o1, turns, c, sn);
-  if (h1 > p.Hq) {
-    const HeadRows rk{p.K + b * p.k[0] + s * p.k[2], p.Ko + b * p.ko[0] + s * p.ko[2], p.k[1], p.ko[1]};
-    walk_heads<T, HALVES>(rk, max(h0 - p.Hq, 0) + l.hl, h1 - p.Hq, l.hpp, o0, o1, turns, c, sn);
-  }
+  walk.finish(src, dst, [&](int) { return turns; }, c, sn);
 }
 
 // ----------------------------------------------------------------------------------------
@@ -260,19 +272,32 @@ struct AppendParams {
   long long kc[3], vc[3];                        // of page, slot, head
 };
 
-// Sequence of token t: the number of sequences that end at or before it (one warp).
-__device__ __forceinline__ int sequence_of(const PagedSeqs& p, int t) {
-  if (!p.cu_q) return t / p.max_q;
-  int b = 0;
-  for (int i = 0; i < p.batch; i += 32) {
-    const int k = i + (int)lane_id();
-    b += __popc(__ballot_sync(0xffffffffu, k < p.batch && p.cu_q[k + 1] <= t));
+// The sequence of token t, by one warp: 32 sequences' offsets and lengths at a time, so that a place
+// costs two dependent loads (the lists, then the table). -1: behind the last sequence.
+__device__ __forceinline__ int sequence_of(const PagedSeqs& p, int t, SeqInfo* s) {
+  if (!p.cu_q) {
+    const int b = t / p.max_q;
+    if (b >= p.batch) return -1;
+    *s = seq_info(p, b);
+    return b;
   }
-  return b;
+  for (int i = 0; i < p.batch; i += 32) {
+    const int k = min(i + (int)lane_id(), p.batch - 1);
+    const int row0 = p.cu_q[k], row1 = p.cu_q[k + 1], len = p.lens[k];
+    const unsigned in = __ballot_sync(0xffffffffu, row0 <= t && t < row1);
+    if (in) {
+      const int src = __ffs(in) - 1;
+      const int b = __shfl_sync(0xffffffffu, k, src);
+      *s = seq_checked(p, b, __shfl_sync(0xffffffffu, len, src), __shfl_sync(0xffffffffu, row0, src),
+                       __shfl_sync(0xffffffffu, row1, src));
+      return b;
+    }
+  }
+  return -1;
 }
 
 template <typename T, bool HALVES>
-__global__ void __launch_bounds__(kRotThreads) append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kRotThreads, kRotCtas) append_kernel(const AppendParams p) {
   extern __shared__ float2 cs[];      // [n_tok][pairs]
   __shared__ long long sh_k[kRotTokens], sh_v[kRotTokens];   // cache rows, bytes; -1: left out
   __shared__ int sh_place[kRotTokens];
@@ -280,83 +305,95 @@ __global__ void __launch_bounds__(kRotThreads) append_kernel(const AppendParams 
   griddep_launch_dependents();
   const int t0 = blockIdx.x * p.n_tok;
   const int pairs = p.rot.pairs;
-  for (int i = warp_id(); i < p.n_tok; i += kRotThreads / 32) {
-    const int t = t0 + i;
-    int place = -1;
-    long long ko = -1, vo = -1;
-    if (t < p.T) {
-      const int b = sequence_of(p.seqs, t);
-      if (lane_id() == 0 && b < p.seqs.batch) {
-        const SeqInfo s = seq_info(p.seqs, b);
-        place = t >= s.tok0 && t - s.tok0 < s.qlen ? s.len - s.qlen + (t - s.tok0) : -1;
-        if (place >= 0) {
-          const int pi = place / p.seqs.page_size;
-          const int page = p.seqs.table[b * p.seqs.table_stride + pi];
-          if (page < 0 || page >= p.seqs.num_pages) {
-            report_bad(p.seqs.status, kBadPage, b);
-            place = -1;
-          } else {
-            const int slot = place - pi * p.seqs.page_size;
-            ko = page * p.kc[0] + slot * p.kc[1];
-            vo = page * p.vc[0] + slot * p.vc[1];
+  const Lane l(p.n_tok, p.tasks);
+  const long long t = t0 + l.i;
+  // The CTA's heads of the list Q heads, K heads, V heads.
+  const int h0 = blockIdx.y * p.heads_per_cta;
+  HeadWalk<T, HALVES> walk;
+  const bool turns = lane_vectors<T, HALVES>(l.j, pairs, walk.o0, walk.o1);
+  walk.h = h0 + l.hl;
+  walk.h1 = l.on && t < p.T ? min(h0 + p.heads_per_cta, p.Hq + 2 * p.Hkv) : 0;
+  walk.step = l.hpp;
+  const int hk0 = p.Hq, hv0 = p.Hq + p.Hkv;     // the first K and V heads of the list
+  auto src = [&](int h) {
+    return h < hk0 ? p.Q + t * p.q[0] + h * p.q[1]
+                   : h < hv0 ? p.K + t * p.k[0] + (h - hk0) * p.k[1]
+                             : p.V + t * p.v[0] + (h - hv0) * p.v[1];
+  };
+  walk.load(src);
+  // The first half of the warps looks up the tokens' places; the other, when the positions are given,
+  // works out the angles meanwhile. Positions that count the places have to wait for them.
+  const int half = kRotThreads / 2;
+  auto angles = [&](int first, int step) {
+    for (int x = first; x < p.n_tok * pairs; x += step) {
+      const int i = x / pairs, pr = x - i * pairs;
+      if (t0 + i < p.T) {
+        const int pos = p.rot.pos ? p.rot.pos[axis_of(p.rot, pr) * p.rot.pos_axis + t0 + i]
+                                  : p.seqs.prefix_len + max(sh_place[i], 0);
+        cs[x] = turn(pos, p.rot.freqs[pr], p.rot.inverse);
+      }
+    }
+  };
+  if (threadIdx.x >= half && p.rot.pos) angles(threadIdx.x - half, half);
+  if (threadIdx.x < half)
+    for (int i = warp_id(); i < p.n_tok; i += kRotThreads / 64) {
+      const int ti = t0 + i;
+      int place = -1;
+      long long ko = -1, vo = -1;
+      if (ti < p.T) {
+        SeqInfo s{0, 0, 0};
+        const int b = sequence_of(p.seqs, ti, &s);
+        if (lane_id() == 0 && b >= 0) {
+          // (a sequence whose rows do not fit has none)
+          place = ti - s.tok0 < s.qlen ? s.len - s.qlen + (ti - s.tok0) : -1;
+          if (place >= 0) {
+            const int pi = place / p.seqs.page_size;
+            const int page = p.seqs.table[b * p.seqs.table_stride + pi];
+            if (page < 0 || page >= p.seqs.num_pages) {
+              report_bad(p.seqs.status, kBadPage, b);
+              place = -1;
+            } else {
+              const int slot = place - pi * p.seqs.page_size;
+              ko = page * p.kc[0] + slot * p.kc[1];
+              vo = page * p.vc[0] + slot * p.vc[1];
+            }
           }
         }
       }
+      if (lane_id() == 0) {
+        sh_place[i] = place;
+        sh_k[i] = ko;
+        sh_v[i] = vo;
+      }
     }
-    if (lane_id() == 0) {
-      sh_place[i] = place;
-      sh_k[i] = ko;
-      sh_v[i] = vo;
-    }
-  }
   __syncthreads();
-  for (int x = threadIdx.x; x < p.n_tok * pairs; x += kRotThreads) {
-    const int i = x / pairs, pr = x - i * pairs;
-    if (sh_place[i] >= 0) {
-      const int pos = p.rot.pos ? p.rot.pos[axis_of(p.rot, pr) * p.rot.pos_axis + t0 + i]
-                                : p.seqs.prefix_len + sh_place[i];
-      cs[x] = turn(pos, p.rot.freqs[pr], p.rot.inverse);
-    }
+  if (!p.rot.pos && pairs) {
+    angles(threadIdx.x, kRotThreads);
+    __syncthreads();
   }
-  __syncthreads();
-  const Lane l(p.n_tok, p.tasks);
   if (!l.on || sh_place[l.i] < 0) return;
-  const long long t = t0 + l.i;
-  int o0, o1;
-  const bool turns = lane_vectors<T, HALVES>(l.j, pairs, o0, o1);
   float c[Vec<T>::N], sn[Vec<T>::N];
   lane_angles<T>(cs, l.i, l.j, pairs, turns, c, sn);
-  // The CTA's heads of the list Q heads, K heads, V heads.
-  const int h0 = blockIdx.y * p.heads_per_cta;
-  const int h1 = min(h0 + p.heads_per_cta, p.Hq + 2 * p.Hkv);
-  if (h0 < p.Hq) {
-    const HeadRows r{p.Q + t * p.q[0], p.Qo + t * p.qo[0], p.q[1], p.qo[1]};
-    walk_heads<T, HALVES>(r, h0 + l.hl, min(h1, p.Hq), l.hpp, o0, o1, turns, c, sn);
-  }
-  const int k0 = max(h0 - p.Hq, 0), k1 = min(h1 - p.Hq, p.Hkv);
-  if (k0 < k1) {
-    const HeadRows r{p.K + t * p.k[0], p.Kc + sh_k[l.i], p.k[1], p.kc[2]};
-    walk_heads<T, HALVES>(r, k0 + l.hl, k1, l.hpp, o0, o1, turns, c, sn);
-  }
-  const int v0 = max(h0 - p.Hq - p.Hkv, 0), v1 = h1 - p.Hq - p.Hkv;
-  if (v0 < v1) {
-    const HeadRows r{p.V + t * p.v[0], p.Vc + sh_v[l.i], p.v[1], p.vc[2]};
-    walk_heads<T, HALVES>(r, v0 + l.hl, v1, l.hpp, o0, o1, false, c, sn);
-  }
+  uint8_t* kc = p.Kc + sh_k[l.i];
+  uint8_t* vc = p.Vc + sh_v[l.i];
+  auto dst = [&](int h) {
+    return h < hk0 ? p.Qo + t * p.qo[0] + h * p.qo[1]
+                   : h < hv0 ? kc + (h - hk0) * p.kc[2] : vc + (h - hv0) * p.vc[2];
+  };
+  walk.finish(src, dst, [&](int h) { return turns && h < hv0; }, c, sn);
 }
 
-// Tokens per CTA and heads per CTA: up to `most` tokens, few enough for at least one head per
-// pass over the CTA's threads; the heads split until the grid has about four CTAs per SM (a
-// thread's loads in flight are kRotUnroll heads), never below one pass.
-void rot_grid(long long tokens_per_row, long long rows, int heads, int tasks, int most, int sms,
-              int* n_tok, int* heads_per_cta) {
+// Tokens per CTA and heads per CTA. As many tokens as leave about three CTAs per SM (the angles of a
+// token are worked out once for all its heads, 768 per CTA; the video clip's gradient 18.6 us with
+// 16 tokens, 20.0 with 8, 22.1 with 4); when one token per CTA is too few, its heads are
+// split too, never below one pass of the CTA's threads.
+void rot_grid(long long tokens_per_row, long long rows, int heads, int tasks, int sms, int* n_tok,
+              int* heads_per_cta) {
+  auto ctas = [&](int n) { return rows * ((tokens_per_row + n - 1) / n); };
   int n = 1;
-  while (n < most && 2 * n * tasks <= kRotThreads && n < tokens_per_row) n *= 2;
-  // few tokens: one per CTA, so the heads of a token spread over its threads
-  while (n > 1 && rows * ((tokens_per_row + n - 1) / n) < 2LL * sms) n /= 2;
+  while (2 * n <= kRotTokens && 2 * n * tasks <= kRotThreads && ctas(2 * n) >= 3LL * sms) n *= 2;
   const int hpp = std::max(1, kRotThreads / (n * tasks));
-  const long long ctas = rows * ((tokens_per_row + n - 1) / n);
-  long long split = std::max<long long>(1, (4LL * sms + ctas - 1) / ctas);
+  const long long split = std::max<long long>(1, 4LL * sms / ctas(n));
   int per = (int)((heads + split - 1) / split);
   per = std::min(heads, (per + hpp - 1) / hpp * hpp);
   *n_tok = n;
@@ -406,7 +443,7 @@ int rope_launch(const lvb_rope_desc* d, const long long qs[3], const long long k
     p.ko[i] = kos[i] * es;
   }
   const int heads = p.Hq + p.Hkv;
-  rot_grid(d->seq, d->batch, heads, p.tasks, kRotTokens, dev->sm_count, &p.n_tok, &p.heads_per_cta);
+  rot_grid(d->seq, d->batch, heads, p.tasks, dev->sm_count, &p.n_tok, &p.heads_per_cta);
   const dim3 grid((unsigned)((d->seq + p.n_tok - 1) / p.n_tok),
                   (unsigned)((heads + p.heads_per_cta - 1) / p.heads_per_cta), (unsigned)d->batch);
   const size_t smem = (size_t)p.n_tok * p.rot.pairs * sizeof(float2);
@@ -451,7 +488,7 @@ int append_launch(const lvb_append_desc* d, const PagedLayout& lay, const long l
     p.vc[i] = lay.vc[i] * 2;
   }
   const int heads = p.Hq + 2 * p.Hkv;
-  rot_grid(g.tokens, 1, heads, p.tasks, 4, dev->sm_count, &p.n_tok, &p.heads_per_cta);
+  rot_grid(g.tokens, 1, heads, p.tasks, dev->sm_count, &p.n_tok, &p.heads_per_cta);
   const dim3 grid((unsigned)((g.tokens + p.n_tok - 1) / p.n_tok),
                   (unsigned)((heads + p.heads_per_cta - 1) / p.heads_per_cta));
   const size_t smem = (size_t)p.n_tok * p.rot.pairs * sizeof(float2);
