@@ -486,7 +486,8 @@ int lvb_kv_append(const lvb_append_desc* d, void* Kc, void* Vc, const void* K, c
 typedef enum lvb_paged_kernel {
   LVB_PAGED_FLASH = 0,    /* 128-row tiles of (position, head of the group) rows */
   LVB_PAGED_DECODE = 1    /* group·max_q <= 32: the cache streamed once, its key blocks dealt
-                             evenly to the SMs whatever the lengths */
+                             evenly to the SMs whatever the lengths, or (few or short sequences:
+                             `cluster`) an item's blocks to the CTAs of a cluster */
 } lvb_paged_kernel;
 
 typedef struct lvb_paged_plan {
@@ -495,7 +496,11 @@ typedef struct lvb_paged_plan {
   int32_t prefix_splits;  /* > 0: the prefix is read once for all query rows of a KV head, in
                              this many key ranges, and joined with the sequences' own part;
                              0: no prefix, or (LVB_PAGED_FLASH) read by every sequence's tiles */
+  int32_t cluster;        /* LVB_PAGED_DECODE: CTAs per (sequence, KV head) that join their parts in
+                             shared memory; 0: blocks dealt to all CTAs, parts joined by a second
+                             kernel */
   int32_t launches;       /* kernel launches per call */
+  int32_t reserved;
   int64_t workspace_bytes;
 } lvb_paged_plan;
 

@@ -300,6 +300,9 @@ int lvb_attention_paged_plan_for(const lvb_paged_desc* d, int32_t sm_count, lvb_
     if (d->prefix_len) {
       out->prefix_splits = paged_flash_splits(d, sm_count, kFlashPrefix);
       out->launches = 3;
+    } else if ((out->cluster = paged_decode_cluster(d, sm_count)) > 0) {
+      out->launches = 1;      // no parts in memory
+      return LVB_OK;
     }
     out->workspace_bytes = (int64_t)(flash_bytes(d, *out) +
                                      paged_decode_workspace(d, sm_count, d->prefix_len > 0));
@@ -343,6 +346,11 @@ int lvb_attention_paged(const lvb_paged_desc* d, const void* Q, const void* Kc, 
   mp.o_sh = lay.o[1];
   mp.lse = lse;
   uint8_t* ws = nullptr;
+  if (pl.cluster > 0) {
+    DecodeWorkspace none = {};
+    return paged_decode_launch(d, lay, mp.seqs, Q, Kc, Vc, O, lse, false, false, pl.cluster, ws, &none,
+                               s, dev);
+  }
   cudaError_t e = workspace_alloc(dev, reinterpret_cast<void**>(&ws), (size_t)pl.workspace_bytes, s);
   if (e != cudaSuccess) return fail_cuda(e, op, "workspace allocation");
   FlashWorkspace fw = {};
@@ -359,7 +367,7 @@ int lvb_attention_paged(const lvb_paged_desc* d, const void* Q, const void* Kc, 
     DecodeWorkspace dw = {};
     if (st == LVB_OK)
       st = paged_decode_launch(d, lay, mp.seqs, Q, Kc, Vc, O, lse, pl.prefix_splits > 0,
-                               pl.prefix_splits > 0, ws + fb, &dw, s, dev);
+                               pl.prefix_splits > 0, 0, ws + fb, &dw, s, dev);
     mp.dec_o = dw.part_o;
     mp.dec_ml = dw.part_ml;
     mp.dec_tab = dw.tab;

@@ -194,13 +194,32 @@ __global__ void __launch_bounds__(kThreads, 1)
     int base = 0;        // the lanes hold runs base .. base+31 ...
     long long done = 0;  // ... whose first item has this number
     SeqInfo sq{0, 0, 0};
+    int run = 0;         // the lane's run: the 32 stand in order of falling length, so that the
+                         // items taken last, when the CTAs finish, are short ones
     long long incl = 0;  // items of the lanes' runs up to and with this lane's
     auto fetch = [&]() {
+      run = base + (int)lane;
       sq = SeqInfo{0, 0, 0};
       if (p.all_rows) {
         if (base + (int)lane == 0) sq.qlen = p.seqs.tokens;
       } else if (base + (int)lane < runs) {
         sq = seq_info(p.seqs, base + lane);
+      }
+      if (runs > 1) {
+        const int key = sq.qlen > 0 ? sq.len : -1;
+        int rank = 0, from = 0;
+#pragma unroll 4
+        for (int o = 0; o < 32; ++o) {
+          const int other = __shfl_sync(0xffffffffu, key, o);
+          rank += other > key || (other == key && o < (int)lane);
+        }
+#pragma unroll 4
+        for (int o = 0; o < 32; ++o)
+          if (__shfl_sync(0xffffffffu, rank, o) == (int)lane) from = o;
+        run = __shfl_sync(0xffffffffu, run, from);
+        sq.tok0 = __shfl_sync(0xffffffffu, sq.tok0, from);
+        sq.qlen = __shfl_sync(0xffffffffu, sq.qlen, from);
+        sq.len = __shfl_sync(0xffffffffu, sq.len, from);
       }
       incl = (long long)((sq.qlen + rows2 - 1) / rows2) * p.Hkv * p.splits;
 #pragma unroll
@@ -246,14 +265,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       im.tok0 = __shfl_sync(0xffffffffu, sq.tok0, src);
       im.qlen = __shfl_sync(0xffffffffu, sq.qlen, src);
       im.len = __shfl_sync(0xffffffffu, sq.len, src);
-      const int b = base + src;
-      // within a run: KV head by KV head, a head's heaviest causal pair first
+      const int b = __shfl_sync(0xffffffffu, run, src);
+      // Within a run the heaviest causal pairs first: pair by pair over the KV heads, whose keys stay
+      // in L2, or KV head by KV head when there are more pairs than a few rounds of the CTAs.
       const int x = (int)(item - done - before);
       const int n_pairs = (im.qlen + rows2 - 1) / rows2;
       const int split = x % p.splits;
       const int y = x / p.splits;
-      im.hk = y / n_pairs;
-      const int pair = n_pairs - 1 - (y - im.hk * n_pairs);
+      int pair;
+      if (n_pairs <= 2 * (int)gridDim.x) {
+        pair = y / p.Hkv;
+        im.hk = y - pair * p.Hkv;
+      } else {
+        im.hk = y / n_pairs;
+        pair = y - im.hk * n_pairs;
+      }
+      pair = n_pairs - 1 - pair;
       im.pos0 = pair * rows2;
       int n0 = blocks_upto(p, npb, im.len, im.qlen, min(im.pos0 + p.ppt, im.qlen));
       int n1 = im.pos0 + p.ppt < im.qlen
@@ -805,8 +832,10 @@ int64_t most_items(const lvb_paged_desc* d, int parts) {
 
 }  // namespace
 
-// Key ranges per tile pair: with fewer items than SMs, as many as fill the SMs once, of at least
-// two blocks of the longest run of keys (the prefix's length; a table's row otherwise).
+// Key ranges per tile pair: with fewer items than SMs, as many as fill the SMs once, down to one
+// block of the longest run of keys (the prefix's length; a table's row otherwise). (At least one,
+// two, four, eight blocks: a prefix of 500 keys 13.5, 14.8, 18.4, 18.4 us, of 4,099 keys over 64-wide
+// heads 30.4, 32.1, 30.5, 34.5 us.)
 int paged_flash_splits(const lvb_paged_desc* d, int sm_count, int parts) {
   const int64_t items = std::max<int64_t>(1, most_items(d, parts));
   int64_t keys = 0;
@@ -814,7 +843,7 @@ int paged_flash_splits(const lvb_paged_desc* d, int sm_count, int parts) {
   if (parts & kFlashOwn) keys += d->table_width * d->page_size;
   const int64_t blocks = (keys + 127) / 128;
   int64_t s = std::max(1, sm_count) / items;
-  s = std::min<int64_t>(s, blocks / 2);
+  s = std::min<int64_t>(s, blocks);
   return (int)std::max<int64_t>(1, s);
 }
 

@@ -25,16 +25,22 @@ struct SmemAttr {
 
 // Launch with programmatic stream serialization: the kernel may be scheduled while the stream's
 // previous kernel ends, and calls griddep_wait() before it touches global memory.
+// cluster: CTAs per cluster (above 8 needs the function's leave too).
 template <typename... P, typename... A>
-int launch_serial(const char* op, void (*kern)(P...), SmemAttr& attr, DeviceState* dev, dim3 grid,
-                  int threads, size_t smem, cudaStream_t stream, const A&... args) {
-  if (smem > 48 * 1024) {
+int launch_cluster(const char* op, void (*kern)(P...), SmemAttr& attr, DeviceState* dev, dim3 grid,
+                   int threads, size_t smem, int cluster, cudaStream_t stream, const A&... args) {
+  if (smem > 48 * 1024 || cluster > 8) {
     const int dv = dev->device;
     const bool known = dv >= 0 && dv < SmemAttr::kMaxDevices;
     if (!known || !attr.set[dv].load(std::memory_order_acquire)) {
       const cudaError_t e =
           cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
       if (e != cudaSuccess) return fail_cuda(e, op, "cudaFuncSetAttribute");
+      if (cluster > 0) {
+        const cudaError_t e2 =
+            cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e2 != cudaSuccess) return fail_cuda(e2, op, "cudaFuncSetAttribute");
+      }
       if (known) attr.set[dv].store(true, std::memory_order_release);
     }
   }
@@ -43,13 +49,22 @@ int launch_serial(const char* op, void (*kern)(P...), SmemAttr& attr, DeviceStat
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)cluster;
+  at[1].val.clusterDim.y = 1;
+  at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
   return e == cudaSuccess ? LVB_OK : fail_cuda(e, op, "kernel launch");
+}
+template <typename... P, typename... A>
+int launch_serial(const char* op, void (*kern)(P...), SmemAttr& attr, DeviceState* dev, dim3 grid,
+                  int threads, size_t smem, cudaStream_t stream, const A&... args) {
+  return launch_cluster(op, kern, attr, dev, grid, threads, smem, 0, stream, args...);
 }
 
 // Sites of bad device data in the status word (code LVB_ERR_INVALID_ARG).
@@ -139,13 +154,15 @@ struct DecodeWorkspace {
   int4* tab;
   int rows, slots, ctas;
 };
+// CTAs per item when its blocks are split over a cluster, 0 when they are dealt to all CTAs.
+int paged_decode_cluster(const lvb_paged_desc* d, int sm_count);
 size_t paged_decode_workspace(const lvb_paged_desc* d, int sm_count, bool keep_parts);
 // keep_parts: every item's result stays in the workspace for the join with a prefix's parts.
 // after_prefix: the kernel before it is the same call's flash kernel over the prefix.
 int paged_decode_launch(const lvb_paged_desc* d, const PagedLayout& lay, const PagedSeqs& seqs,
                         const void* Q, const void* Kc, const void* Vc, void* O, float* lse,
-                        bool keep_parts, bool after_prefix, void* ws, DecodeWorkspace* out,
-                        cudaStream_t stream,
+                        bool keep_parts, bool after_prefix, int cluster, void* ws,
+                        DecodeWorkspace* out, cudaStream_t stream,
                         DeviceState* dev);
 
 // The flash kernel over the prefix's keys, the sequences' own, or both one after the other.
@@ -295,6 +312,26 @@ __device__ __forceinline__ void copy_async4(void* dst, const void* src) {
 }
 __device__ __forceinline__ void copy_async_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// Loads from a CTA of the cluster (a shared::cluster address, see mapa_shared).
+__device__ __forceinline__ float ld_cluster_f32(uint32_t a) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster_f32x2(uint32_t a) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t a) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(a)
+               : "memory");
+  return v;
 }
 
 // A wait by a whole warp that tests once before it suspends: the phase is often complete already,

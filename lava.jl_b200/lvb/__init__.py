@@ -170,7 +170,8 @@ class lvb_append_desc(C.Structure):
 
 class lvb_paged_plan(C.Structure):
     _fields_ = [("kernel", C.c_int32), ("splits", C.c_int32), ("prefix_splits", C.c_int32),
-                ("launches", C.c_int32), ("workspace_bytes", C.c_int64)]
+                ("cluster", C.c_int32), ("launches", C.c_int32), ("reserved", C.c_int32),
+                ("workspace_bytes", C.c_int64)]
 
 
 class lvb_comm_id(C.Structure):

@@ -218,9 +218,11 @@ def run_attention(lvb, torch, c, Hq, qlens, causal=True, scale=None, cu=True, sp
     return Q, O, lse
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("T,D", [("bf16", 128), ("fp16", 128), ("bf16", 64), ("fp16", 64)])
 @pytest.mark.parametrize("page,Hq,Hkv,lens,qlens,causal", [
     (16, 1, 1, [1], [1], True),                                   # one key
+    (16, 32, 8, [3000], [1], True),                               # one sequence over all SMs
     (8, 8, 8, [1, 7, 8, 9, 127, 128, 129, 700], [1] * 8, True),   # ends around a page and a block
     (64, 64, 8, [0, 1000, 64, 0, 3], [1] * 5, True),              # sequences without a key
     (48, 12, 4, [500, 2, 131], [3, 1, 2], True),                  # pages that no block divides
@@ -230,10 +232,14 @@ def run_attention(lvb, torch, c, Hq, qlens, causal=True, scale=None, cu=True, sp
     (24, 6, 2, [20000], [2], True),                               # one long sequence: split
     (128, 4, 4, [3000, 40, 2500, 1, 900, 128, 129] * 5, [1] * 35, True),
 ])
-def test_decode(lvb, torch_cuda, T, D, page, Hq, Hkv, lens, qlens, causal):
-    assert lvb.attention_paged_plan(len(lens), Hq, Hkv, sum(qlens), max(qlens), page, 9,
-                                    D=D).kernel == lvb.PAGED_DECODE
-    c = Cache(torch_cuda, T, Hkv, D, page, lens, seed=page + Hq)
+def test_decode(lvb, torch_cuda, T, D, page, Hq, Hkv, lens, qlens, causal, wide):
+    """With a table as wide as the lengths (short or few sequences: clusters of CTAs join an item in
+    shared memory) and with one for 100,000 keys (the blocks are dealt to all CTAs)."""
+    c = Cache(torch_cuda, T, Hkv, D, page, lens, seed=page + Hq, width_more=100000 // page if wide else 2)
+    plan = lvb.attention_paged_plan(len(lens), Hq, Hkv, sum(qlens), max(qlens), page, c.table.shape[1], D=D)
+    assert plan.kernel == lvb.PAGED_DECODE
+    if wide:
+        assert plan.cluster == (16 if len(lens) == 1 and Hkv == 8 else 0)
     run_attention(lvb, torch_cuda, c, Hq, qlens, causal, spare_rows=2)
 
 
