@@ -244,6 +244,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (!p.late_wait) griddep_wait();
   griddep_launch_dependents();
 
+  // A cluster's item is given by its number: the producer reads its sequence at once.
+  const int c_id = p.cluster ? blockIdx.x / p.cluster : 0, c_b = c_id / p.Hkv;
+  SeqInfo c_seq{0, 0, 0};
+  if (p.cluster && warp == kTmaWarp) {
+    c_seq = seq_info(p.seqs, c_b);
+    if (lane == 0) {
+      sStart[0] = c_seq.tok0;      // for the join
+      sStart[1] = c_seq.qlen;
+    }
+  }
+
   // ---------------- this CTA's run of blocks ----------------
   // Thread i sums the costs of sequences [i·per, (i+1)·per); a scan over the threads gives the
   // total and the thread whose sequences hold the run's first unit. An item's units are its
@@ -254,7 +265,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto units_of = [&](int nb) -> int { return nb ? (nb + kItemCost<D>) * p.Hkv : 0; };
   const bool kept = batch <= kThreads;     // one sequence per thread: the producer reads them here
   int mine = 0;
-  // (a cluster's item is given by its number)
   for (int b = p.cluster ? sb1 : sb0; b < sb1; ++b) {
     const SeqInfo s = seq_info(p.seqs, b);
     if (kept) sSeq[b] = s;
@@ -301,6 +311,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   // columns: S of warpgroup w at w·NR, its O buffers at (2 + 2w + ob)·NR
   const WaitGuard g{p.seqs.status, abort_flag, p.timeout_ns};
 
+  auto load_q = [&](int qb, int hk, int tok0) {
+    bar_arrive_expect_tx(&q_full[qb], C::kCh * p.nrows * 128);
+    for (int c = 0; c < C::kCh; ++c)
+      tma_load_3d(sQ + qb * C::kQ + c * NR * 128, &tmQ, c * 64, hk * p.group, tok0, &q_full[qb]);
+  };
+
   if (warp == kTmaWarp) {
     // ---------------- producer: items, Q, K and V blocks ----------------
     const BlockLane<D> bl((int)lane, p.box);
@@ -328,9 +344,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       Item& im = items[qi];
       bool found = false;
       if (p.cluster && pub == 0) {
-        const int id = blockIdx.x / p.cluster, rank = blockIdx.x - id * p.cluster;
-        const int cb = id / p.Hkv;
-        const SeqInfo c = seq_info(p.seqs, cb);
+        const SeqInfo& c = c_seq;
+        const int rank = blockIdx.x - c_id * p.cluster;
         const int nb = blocks_of(c);
         const int kb0 = (int)((long long)nb * rank / p.cluster);
         const int kb1 = (int)((long long)nb * (rank + 1) / p.cluster);
@@ -338,10 +353,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (found) {
           const int entry = kb0 * 128 / p.seqs.page_size + (int)lane;
           if (entry <= (c.len - 1) / p.seqs.page_size)
-            copy_async4(&im.entries[lane], p.seqs.table + cb * p.seqs.table_stride + entry);
+            copy_async4(&im.entries[lane], p.seqs.table + c_b * p.seqs.table_stride + entry);
           if (lane == 0) {
-            im.b = cb;
-            im.hk = id - cb * p.Hkv;
+            im.b = c_b;
+            im.hk = c_id - c_b * p.Hkv;
             im.kb0 = kb0;
             im.nblk = kb1 - kb0;
             im.len = c.len;
@@ -433,14 +448,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                  p.seqs.page_size, im.entries);
       __syncwarp();
       if (lane == 0) bar_arrive(&i_empty[qi]);
-      const int qb = it & 1;
-      if (!wait_soon_warp(&q_empty[qb], (uint32_t)((it >> 1) & 1) ^ 1, g, 51, it)) { ok = false; break; }
-      if (lane == 0) {
-        bar_arrive_expect_tx(&q_full[qb], C::kCh * p.nrows * 128);
-        for (int c = 0; c < C::kCh; ++c)
-          tma_load_3d(sQ + qb * C::kQ + c * NR * 128, &tmQ, c * 64, hk * p.group, tok0, &q_full[qb]);
+      if (it > 0) {        // (the first item's Q comes from the V warp, beside the first K block)
+        const int qb = it & 1;
+        if (!wait_soon_warp(&q_empty[qb], (uint32_t)((it >> 1) & 1) ^ 1, g, 51, it)) { ok = false; break; }
+        if (lane == 0) load_q(qb, hk, tok0);
+        __syncwarp();
       }
-      __syncwarp();
       for (int j = 0; j < nblk; ++j, ++n) {
         const BoxAt at = walk.take();
         const int s = n % KR;
@@ -475,6 +488,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!wait_soon_warp(&i_full[qi], (uint32_t)((it / kQueue) & 1), g, 74, it)) { ok = false; break; }
       const Item& im = items[qi];
       const int last = im.last, hk = im.hk, nblk = im.nblk;
+      if (it == 0 && !last && lane == 0) load_q(0, hk, im.tok0);
       BoxWalk<D> walk;
       if (!last)
         walk.start(bl, p.seqs.table + im.b * p.seqs.table_stride, im.kb0, im.len, p.box,
@@ -492,6 +506,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!ok && lane == 0)
       for (int i = max(0, n - VR); i < n; ++i)
         drain_wait(&v_full[i % VR], (uint32_t)((i / VR) & 1), p.timeout_ns);
+    if (!ok && lane == 0 && n > 0) drain_wait(&q_full[0], 0, p.timeout_ns);
     __syncwarp();
   } else if (warp == kQkWarp || warp == kPvWarp) {
     // ---------------- MMA issuers: the warp waits, one elected lane issues ----------------
@@ -838,48 +853,56 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool bad = *abort_flag != 0;
     if (bad && threadIdx.x < NR) sJml[2 * threadIdx.x + 1] = -1.f;   // after a wait gave up: store nothing
     cluster_sync_all();
-    const int id = blockIdx.x / p.cluster, rank = blockIdx.x - id * p.cluster;
-    const int b = id / p.Hkv, hk = id - b * p.Hkv;
-    const SeqInfo s = seq_info(p.seqs, b);
-    const int n_rows = min(p.nrows, s.qlen * p.group);
+    const int rank = blockIdx.x - c_id * p.cluster, hk = c_id - c_b * p.Hkv;
+    const int tok0 = sStart[0], n_rows = min(p.nrows, sStart[1] * p.group);
     constexpr int V = D / 32;
     const uint32_t j_addr = smem_u32(sJ) + lane * V * 4, ml_addr = smem_u32(sJml);
     for (int r = rank + (int)warp * p.cluster; r < n_rows; r += p.cluster * (kThreads / 32)) {
       float pm = -INFINITY, pl = 0.f;            // lane k: part k's m and l
       if ((int)lane < p.cluster) {
-        const uint32_t a = mapa_shared(ml_addr + r * 8, lane);
-        pm = ld_cluster_f32(a);
-        pl = ld_cluster_f32(a + 4);
+        const float2 x = ld_cluster_f32x2(mapa_shared(ml_addr + r * 8, lane));
+        pm = x.x;
+        pl = x.y;
+      }
+      // all parts' rows under way at once (of a part without a key: whatever its ring holds)
+      float o[16][V];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        if (k < p.cluster) {
+          const uint32_t a = mapa_shared(j_addr + r * D * 4, k);
+          if constexpr (V == 4) {
+            const float4 f = ld_cluster_f32x4(a);
+            o[k][0] = f.x, o[k][1] = f.y, o[k][2] = f.z, o[k][3] = f.w;
+          } else {
+            const float2 f = ld_cluster_f32x2(a);
+            o[k][0] = f.x, o[k][1] = f.y;
+          }
+        }
       }
       const bool gave_up = __any_sync(0xffffffffu, pl < 0.f);
       const bool some = pl != 0.f;
       float mx = some ? pm : -INFINITY;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      for (int o2 = 16; o2 > 0; o2 >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o2));
       const float mu = mx == -INFINITY ? 0.f : mx;
       const float pw = some ? fast_exp2(pm - mu) : 0.f;
       float den = some ? pw * pl : 0.f;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
+      for (int o2 = 16; o2 > 0; o2 >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o2);
       const unsigned parts = __ballot_sync(0xffffffffu, some);
       float acc[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) acc[e] = 0.f;
-      for (unsigned rest = parts; rest; rest &= rest - 1) {
-        const int k = __ffs(rest) - 1;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
         const float wk = __shfl_sync(0xffffffffu, pw, k);
-        const uint32_t a = mapa_shared(j_addr + r * D * 4, k);
-        if constexpr (V == 4) {
-          const float4 f = ld_cluster_f32x4(a);
-          acc[0] += wk * f.x, acc[1] += wk * f.y, acc[2] += wk * f.z, acc[3] += wk * f.w;
-        } else {
-          const float2 f = ld_cluster_f32x2(a);
-          acc[0] += wk * f.x, acc[1] += wk * f.y;
-        }
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (parts >> k & 1) acc[e] += wk * o[k][e];
       }
       if (gave_up) continue;
       const int pos = r / p.group;
-      const long long tok = s.tok0 + pos;
+      const long long tok = tok0 + pos;
       const int h = hk * p.group + r - pos * p.group;
       const float inv = den == 0.f ? 0.f : 1.f / den;
       uint16_t* dst = reinterpret_cast<uint16_t*>(p.O) + tok * p.o_st + h * p.o_sh + lane * V;
