@@ -26,7 +26,8 @@
  *    it has completed (griddepcontrol.wait), and they let the next kernel be scheduled
  *    early. A caller's kernel launched after a GEMM with that same attribute must wait
  *    (griddepcontrol.wait) before reading the GEMM's output; other kernels see plain stream
- *    order.
+ *    order. The kernels of lvb_rope, lvb_kv_append and lvb_attention_paged are launched the same
+ *    way.
  *  - The library never frees caller memory and holds no pointer past a call.
  */
 #ifndef LVB_H
@@ -482,7 +483,10 @@ int lvb_kv_append(const lvb_append_desc* d, void* Kc, void* Vc, const void* K, c
 /* Attention of the packed queries over the paged cache, the same operation as lvb_attention_fwd
  * per sequence: O = softmax(scale·Q·Kᵀ + mask)·V over the prefix's keys and the sequence's own,
  * fp32 softmax, P rounded to the cache's type, GQA by head grouping; rows that see no key give
- * O = 0 and lse = -inf. `lse` (nullable) is fp32 [token][heads_q]. */
+ * O = 0 and lse = -inf. `lse` (nullable) is fp32 [token][heads_q]. What the pages hold behind a
+ * sequence's last place, and the table behind its last page, plays no part, whatever it is; among
+ * a sequence's own places (and the prefix's) an infinite or NaN value reaches every row of the call
+ * whose products include its block, also where the causal mask gives it the weight 0. */
 typedef enum lvb_paged_kernel {
   LVB_PAGED_FLASH = 0,    /* 128-row tiles of (position, head of the group) rows */
   LVB_PAGED_DECODE = 1    /* group·max_q <= 32: the cache streamed once, its key blocks dealt

@@ -15,6 +15,9 @@ through Vulkan.
   Keywords `bias`, `residual`, `activation` fuse the epilogue `act(A·B + bias + residual)`.
 * `attention!(O, Q, K, V; causal, scale)` — Q/O `(E, Lq, Hq, B)`, K/V `(E, Lk, Hkv, B)`
   column-major (Lava's layout, src/device/sharedmemory.jl:73-76); GQA by head grouping.
+* `rope!`, `kv_append!`, `attention_paged!` — rotation of queries and keys by position, new tokens
+  into a paged KV cache, and the attention of ragged batches over it (with a prefix that all
+  sequences share).
 * `B200Array` — an owning device buffer (`lvb_malloc`/`lvb_free`); any value with
   `pointer` and `size` (e.g. `Lava.LavaDeviceArray`, a non-owning `(ptr, dims)`,
   src/device/devicearray.jl:35-38) is accepted by the ops.
@@ -33,7 +36,7 @@ using LinearAlgebra: Transpose, transpose
 # on `backend::KI.Backend` and call `caps(backend)`; B200Backend subtypes it so they resolve.
 import KernelInterface as KI
 
-export B200Backend, B200Array, gemm!, attention!, device_status, caps_raw, matrix_shapes_raw,
+export B200Backend, B200Array, gemm!, attention!, rope!, kv_append!, attention_paged!, device_status, caps_raw, matrix_shapes_raw,
        pe_program, PeProgram, pe_ifelse, pe_eq, pe_rsqrt, pe_erf,
        LavaB200Error, BFloat16, shard_range, comm_unique_id, Comm, allgather!
 
@@ -145,6 +148,38 @@ struct AttnDesc
     scale::Float32; reserved::Int32
     q_stride::NTuple{3,Int64}; k_stride::NTuple{3,Int64}
     v_stride::NTuple{3,Int64}; o_stride::NTuple{3,Int64}
+end
+
+struct Rotation
+    pairs::Int32; layout::Int32; n_axes::Int32; inverse::Int32
+    sections::NTuple{4,Int32}
+end
+
+struct RopeDesc
+    dtype::Int32; reserved::Int32
+    batch::Int64; heads_q::Int64; heads_kv::Int64; seq::Int64; head_dim::Int64
+    q_stride::NTuple{3,Int64}; k_stride::NTuple{3,Int64}
+    qo_stride::NTuple{3,Int64}; ko_stride::NTuple{3,Int64}
+    pos_stride::NTuple{3,Int64}
+    rot::Rotation
+end
+
+struct PagedDesc
+    dtype::Int32; causal::Int32
+    batch::Int64; heads_q::Int64; heads_kv::Int64; head_dim::Int64
+    tokens::Int64; max_q::Int64
+    page_size::Int64; num_pages::Int64; table_width::Int64; table_stride::Int64
+    prefix_len::Int64
+    kc_stride::NTuple{3,Int64}; vc_stride::NTuple{3,Int64}
+    q_stride::NTuple{2,Int64}; o_stride::NTuple{2,Int64}
+    scale::Float32; reserved::Int32
+end
+
+struct AppendDesc
+    paged::PagedDesc
+    k_stride::NTuple{2,Int64}; v_stride::NTuple{2,Int64}
+    pos_stride::Int64
+    rot::Rotation
 end
 
 # ---- capabilities ----------------------------------------------------------------------
@@ -356,6 +391,135 @@ function attention!(O, Q, K, V; causal::Bool = true, scale::Real = inv(sqrt(size
     check(ccall(sym(:lvb_attention_fwd), Cint,
                 (Ref{AttnDesc}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}),
                 d, pointer(Q), pointer(K), pointer(V), pointer(O), pl, stream))
+    return O
+end
+
+# ---- position rotation, paged KV cache -----------------------------------------------------
+const ROPE_LAYOUTS = Dict{Symbol,Int32}(:halves => 0, :pairs => 1)
+
+function rotation(pairs::Integer, sections, layout::Symbol, inverse::Bool)
+    haskey(ROPE_LAYOUTS, layout) || throw(ArgumentError("layout: :halves or :pairs"))
+    s = sections === nothing ? (pairs,) : Tuple(sections)
+    1 <= length(s) <= 4 || throw(ArgumentError("sections: 1 to 4 axes"))
+    return Rotation(pairs, ROPE_LAYOUTS[layout], length(s), Int32(inverse),
+                    ntuple(i -> i <= length(s) ? Int32(s[i]) : Int32(0), 4))
+end
+
+"""
+    rope!(Qo, Q, pos, freqs; Ko = nothing, K = nothing, sections = nothing, layout = :halves,
+          inverse = false, stream = C_NULL)
+
+Rotate queries (and keys) `(E, L, H, B)` by their positions; a result may be its input. Pair `i` of a
+head turns by `pos * freqs[i]`: `freqs` a device vector of Float64, one per pair; `pos` Int32 `(L, B)`
+on the device, or `(L, B, axes)` with `sections` the pairs of each axis. `layout`: pair `i` (0-based)
+is elements `i` and `i + pairs` (`:halves`) or `2i` and `2i + 1` (`:pairs`). `inverse` turns back, which is the
+gradient.
+"""
+function rope!(Qo, Q, pos, freqs; Ko = nothing, K = nothing, sections = nothing,
+               layout::Symbol = :halves, inverse::Bool = false, stream::Ptr{Cvoid} = C_NULL)
+    E, L, Hq, Bq = size(Q, 1), size(Q, 2), size(Q, 3), size(Q, 4)
+    size(Qo) == size(Q) || throw(DimensionMismatch("rope!: Q $(size(Q)) Qo $(size(Qo))"))
+    (K === nothing) == (Ko === nothing) || throw(ArgumentError("rope!: K and Ko come together"))
+    Hkv = K === nothing ? 0 : size(K, 3)
+    K === nothing || (size(Ko) == size(K) && size(K) == (E, L, Hkv, Bq)) ||
+        throw(DimensionMismatch("rope!: K $(size(K)) Ko $(size(Ko))"))
+    rot = rotation(length(freqs), sections, layout, inverse)
+    (size(pos, 1), size(pos, 2), length(pos)) == (L, Bq, L * Bq * rot.n_axes) ||
+        throw(DimensionMismatch("rope!: pos is (L, B) or (L, B, axes)"))
+    (eltype(pos) === Int32 && eltype(freqs) === Float64) ||
+        throw(ArgumentError("rope!: pos is Int32, freqs Float64"))
+    z = (0, 0, 0)
+    d = RopeDesc(dtype(eltype(Q)), 0, Bq, Hq, Hkv, L, E, z, z, z, z, (L * Bq, L, 1), rot)
+    check(ccall(sym(:lvb_rope), Cint,
+                (Ref{RopeDesc}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid},
+                 Ptr{Cvoid}),
+                d, pointer(Q), ptr_or_null(K), pointer(Qo), ptr_or_null(Ko), pointer(pos),
+                pointer(freqs), stream))
+    return Qo
+end
+
+ptr_or_null(x) = x === nothing ? C_NULL : Ptr{Cvoid}(pointer(x))
+
+function paged_desc(Kc, Vc, table, seq_lens, cu_q, max_q, T, Hq, prefix_len, causal, scale)
+    E, Hkv, page, pages = size(Kc, 1), size(Kc, 2), size(Kc, 3), size(Kc, 4)
+    size(Vc) == size(Kc) || throw(DimensionMismatch("caches $(size(Kc)) and $(size(Vc))"))
+    width, B = size(table, 1), size(table, 2)
+    (eltype(table) === Int32 && eltype(seq_lens) === Int32) ||
+        throw(ArgumentError("the block table and seq_lens are Int32"))
+    length(seq_lens) == B || throw(DimensionMismatch("seq_lens has $(length(seq_lens)) entries, the table $B columns"))
+    cu_q === nothing || (eltype(cu_q) === Int32 && length(cu_q) == B + 1) ||
+        throw(DimensionMismatch("cu_q needs $(B + 1) Int32 entries"))
+    (cu_q === nothing || max_q !== nothing) || throw(ArgumentError("cu_q without max_q"))
+    mq = max_q === nothing ? (B == 0 ? 0 : T ÷ B) : max_q
+    (cu_q !== nothing || B * mq == T) || throw(DimensionMismatch("$T rows for $B sequences of $mq"))
+    z3, z2 = (0, 0, 0), (0, 0)
+    return PagedDesc(dtype(eltype(Kc)), Int32(causal), B, Hq, Hkv, E, T, mq, page, pages, width, 0,
+                     prefix_len, z3, z3, z2, z2, Float32(scale), 0)
+end
+
+"""
+    kv_append!(Kc, Vc, K, V, table, seq_lens; cu_q = nothing, max_q = nothing, Q = nothing,
+               Qo = nothing, pos = nothing, freqs = nothing, sections = nothing, layout = :halves,
+               prefix_len = 0, stream = C_NULL)
+
+Write new keys and values `(E, Hkv, T)` into a paged cache `(E, Hkv, page_size, pages)`: sequence `b`'s
+rows are `cu_q[b]+1 : cu_q[b+1]` (0-based offsets, Int32 on the device) and become its last places, up to
+`seq_lens[b]`; `table` is Int32 `(pages per sequence, B)` of 0-based page numbers. With `freqs` the keys
+are rotated on the way (`rope!`; `pos` Int32 `(T)` or `(T, axes)`, by default the place) and `Q`
+`(E, Hq, T)` beside them into `Qo`.
+"""
+function kv_append!(Kc, Vc, K, V, table, seq_lens; cu_q = nothing, max_q = nothing, Q = nothing,
+                    Qo = nothing, pos = nothing, freqs = nothing, sections = nothing,
+                    layout::Symbol = :halves, prefix_len::Integer = 0, stream::Ptr{Cvoid} = C_NULL)
+    T = size(K, 3)
+    (size(K) == (size(Kc, 1), size(Kc, 2), T) && size(V) == size(K)) ||
+        throw(DimensionMismatch("kv_append!: K $(size(K)) V $(size(V))"))
+    (Q === nothing) == (Qo === nothing) || throw(ArgumentError("kv_append!: Q and Qo come together"))
+    Hq = Q === nothing ? 0 : size(Q, 2)
+    Q === nothing || (size(Q) == (size(Kc, 1), Hq, T) && size(Qo) == size(Q)) ||
+        throw(DimensionMismatch("kv_append!: Q $(size(Q)) Qo $(size(Qo))"))
+    rot = freqs === nothing ? rotation(0, nothing, layout, false) :
+          rotation(length(freqs), sections, layout, false)
+    pos === nothing || (eltype(pos) === Int32 && length(pos) == T * rot.n_axes) ||
+        throw(DimensionMismatch("kv_append!: pos is Int32 (T) or (T, axes)"))
+    d = AppendDesc(paged_desc(Kc, Vc, table, seq_lens, cu_q, max_q, T, Hq, prefix_len, true, 1),
+                   (0, 0), (0, 0), T, rot)
+    check(ccall(sym(:lvb_kv_append), Cint,
+                (Ref{AppendDesc}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid},
+                 Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}),
+                d, pointer(Kc), pointer(Vc), pointer(K), pointer(V), ptr_or_null(Q), ptr_or_null(Qo),
+                pointer(table), pointer(seq_lens), ptr_or_null(cu_q), ptr_or_null(pos),
+                ptr_or_null(freqs), stream))
+    return Kc, Vc
+end
+
+"""
+    attention_paged!(O, Q, Kc, Vc, table, seq_lens; cu_q = nothing, max_q = nothing, causal = true,
+                     scale = 1/sqrt(E), lse = nothing, prefix_table = nothing, prefix_len = 0,
+                     stream = C_NULL)
+
+Attention of packed queries `(E, Hq, T)` over a paged cache (the arguments of `kv_append!`; `seq_lens` counts
+the queries' own tokens). `prefix_table` (Int32, 0-based page numbers) and `prefix_len`: keys that
+stand before every sequence's own, read once for all. `lse` Float32 `(Hq, T)`.
+"""
+function attention_paged!(O, Q, Kc, Vc, table, seq_lens; cu_q = nothing, max_q = nothing,
+                          causal::Bool = true, scale::Real = inv(sqrt(size(Q, 1))), lse = nothing,
+                          prefix_table = nothing, prefix_len::Integer = 0,
+                          stream::Ptr{Cvoid} = C_NULL)
+    E, Hq, T = size(Q, 1), size(Q, 2), size(Q, 3)
+    (size(O) == size(Q) && E == size(Kc, 1)) ||
+        throw(DimensionMismatch("attention_paged!: Q $(size(Q)) O $(size(O)) cache $(size(Kc))"))
+    prefix_len == 0 || (prefix_table !== nothing && eltype(prefix_table) === Int32 &&
+                        length(prefix_table) >= cld(prefix_len, size(Kc, 3))) ||
+        throw(ArgumentError("attention_paged!: prefix_table must list the prefix's pages"))
+    lse === nothing || (eltype(lse) === Float32 && size(lse) == (Hq, T)) ||
+        throw(DimensionMismatch("attention_paged!: lse is Float32 (Hq, T)"))
+    d = paged_desc(Kc, Vc, table, seq_lens, cu_q, max_q, T, Hq, prefix_len, causal, scale)
+    check(ccall(sym(:lvb_attention_paged), Cint,
+                (Ref{PagedDesc}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid},
+                 Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}),
+                d, pointer(Q), pointer(Kc), pointer(Vc), pointer(table), pointer(seq_lens),
+                ptr_or_null(cu_q), ptr_or_null(prefix_table), pointer(O), ptr_or_null(lse), stream))
     return O
 end
 

@@ -26,6 +26,11 @@ using LinearAlgebra
         @test err isa LavaB200Error && err.operation == "lvb_gemm"
     end
 
+    @testset "paged-cache structs have the C sizes (no GPU)" begin
+        @test sizeof(LavaB200.Rotation) == 32 && sizeof(LavaB200.RopeDesc) == 200
+        @test sizeof(LavaB200.PagedDesc) == 184 && sizeof(LavaB200.AppendDesc) == 256
+    end
+
     @testset "B200Backend is a KernelInterface.Backend (no GPU)" begin
         @test B200Backend() isa LavaB200.KI.Backend
     end
@@ -143,6 +148,31 @@ using LinearAlgebra
                 ref = v * (p ./ sum(p; dims = 1))
                 @test maximum(abs.(O[:, :, h, 1] .- ref)) <= 1e-2
             end
+        end
+        @testset "rope!, kv_append!, attention_paged! (GPU)" begin
+            E, Hq, Hkv, page, L = 128, 4, 2, 16, 40
+            K = Float16.(randn(Float32, E, Hkv, L)); V = Float16.(randn(Float32, E, Hkv, L))
+            Q = Float16.(randn(Float32, E, Hq, 1))
+            Kc = B200Array(zeros(Float16, E, Hkv, page, 5)); Vc = B200Array(zeros(Float16, E, Hkv, page, 5))
+            table = B200Array(reshape(Int32[4, 0, 2], 3, 1)); lens = B200Array(Int32[L])
+            kv_append!(Kc, Vc, B200Array(K), B200Array(V), table, lens)
+            dO = B200Array{Float16}(undef, E, Hq, 1)
+            attention_paged!(dO, B200Array(Q), Kc, Vc, table, lens)
+            O = Float64.(Array(dO))
+            for h in 1:Hq
+                k = Float64.(K[:, (h + 1) ÷ 2, :]); v = Float64.(V[:, (h + 1) ÷ 2, :])
+                s = (k' * Float64.(Q[:, h, 1])) ./ sqrt(E)
+                p = exp.(s .- maximum(s))
+                @test maximum(abs.(O[:, h, 1] .- v * (p ./ sum(p)))) <= 1e-2
+            end
+            x = randn(Float32, 64, 3, 1, 1)
+            pos = B200Array(reshape(Int32[0, 7, 100], 3, 1)); f = B200Array([10.0^(-i / 32) for i in 0:31])
+            y = B200Array{Float32}(undef, 64, 3, 1, 1)
+            rope!(y, B200Array(x), pos, f)
+            @test Array(y)[:, 1, 1, 1] == x[:, 1, 1, 1]
+            rope!(y, y, pos, f; inverse = true)
+            @test maximum(abs.(Array(y) .- x)) <= 1e-5
+            @test device_status() == (0, 0, 0)
         end
     else
         @info "no GPU visible: GPU tier not run"

@@ -700,8 +700,11 @@ class PreparedCall:
         self._device = next(t for t in keep if t is not None).device.index
 
     def __call__(self, stream=None):
-        s = (_torch()._C._cuda_getCurrentRawStream(self._device) if stream is None
-             else _stream_ptr(stream))
+        c = _torch()._C
+        if c._cuda_getDevice() != self._device:
+            raise LavaError(LVB_ERR_INVALID_ARG, "lvb: the call's tensors are on "
+                            f"cuda:{self._device}, the current device is cuda:{c._cuda_getDevice()}")
+        s = c._cuda_getCurrentRawStream(self._device) if stream is None else _stream_ptr(stream)
         st = self._fn(*self._args, s)
         if st:
             check(st)
