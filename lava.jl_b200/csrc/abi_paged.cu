@@ -309,6 +309,8 @@ int lvb_attention_paged_plan_for(const lvb_paged_desc* d, int32_t sm_count, lvb_
     return LVB_OK;
   }
   out->kernel = LVB_PAGED_FLASH;
+  if (paged_flash_items(d, kFlashOwn) > INT32_MAX - 65536)
+    return fail(LVB_ERR_UNSUPPORTED, op, "more than 2^31 query tiles", "split the batch");
   out->splits = paged_flash_splits(d, sm_count, kFlashOwn | (d->prefix_len ? kFlashPrefix : 0));
   out->launches = out->splits > 1 ? 2 : 1;
   out->workspace_bytes = (int64_t)flash_bytes(d, *out);

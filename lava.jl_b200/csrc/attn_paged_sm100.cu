@@ -172,11 +172,23 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const WaitGuard g{p.seqs.status, abort_flag, p.timeout_ns};
+  // (only into L2, so what the list holds in the end is what is read)
+  if (p.prefix && warp == kTmaWarp)
+    for (int i = lane * 32; i < (p.prefix + p.seqs.page_size - 1) / p.seqs.page_size; i += 32 * 32)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(p.seqs.prefix_table + i));
   // The setup above may run while the stream's previous kernel ends; what reads this kernel's
   // results after its own wait may be scheduled from here on.
   griddep_wait();
   griddep_launch_dependents();
   const int npb = (p.prefix + 127) / 128;
+
+  auto load_q = [&](const Item& im) {
+    bar_arrive_expect_tx(q_full, (uint32_t)(2 * kCh * p.ppt * p.group * 128));
+    for (int t = 0; t < 2; ++t)
+      for (int c = 0; c < kCh; ++c)
+        tma_load_3d(sQ + t * C::kTileBytes + c * kChunk, &tmQ, c * 64, im.hk * p.group,
+                    im.tok0 + im.pos0 + t * p.ppt, q_full);
+  };
 
   if (warp == kTmaWarp) {
     // ---------------- scheduler + TMA producer (the whole warp) ----------------
@@ -192,11 +204,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     int qi = 0;          // Q tiles issued
     bool ok = true;
     int base = 0;        // the lanes hold runs base .. base+31 ...
-    long long done = 0;  // ... whose first item has this number
+    int done = 0;        // ... whose first item has this number
     SeqInfo sq{0, 0, 0};
     int run = 0;         // the lane's run: the 32 stand in order of falling length, so that the
                          // items taken last, when the CTAs finish, are short ones
-    long long incl = 0;  // items of the lanes' runs up to and with this lane's
+    int incl = 0;        // items of the lanes' runs up to and with this lane's
     auto fetch = [&]() {
       run = base + (int)lane;
       sq = SeqInfo{0, 0, 0};
@@ -221,20 +233,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         sq.qlen = __shfl_sync(0xffffffffu, sq.qlen, from);
         sq.len = __shfl_sync(0xffffffffu, sq.len, from);
       }
-      incl = (long long)((sq.qlen + rows2 - 1) / rows2) * p.Hkv * p.splits;
+      incl = (sq.qlen + rows2 - 1) / rows2 * p.Hkv * p.splits;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
         if ((int)lane >= o) incl += v;
       }
     };
     fetch();
-    long long item = blockIdx.x;
+    int item = blockIdx.x;
     for (int k = 0; ok; ++k) {
       if (p.counter) {
-        int take = 0;
-        if (lane == 0) take = atomicAdd(p.counter, 1);
-        item = __shfl_sync(0xffffffffu, take, 0);
+        if (lane == 0) item = atomicAdd(p.counter, 1);
+        item = __shfl_sync(0xffffffffu, item, 0);
       } else if (k > 0) {
         item += gridDim.x;
       }
@@ -260,7 +271,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         break;
       }
       const int src = __ffs(__ballot_sync(0xffffffffu, item - done < incl)) - 1;
-      const long long before = src == 0 ? 0 : __shfl_sync(0xffffffffu, incl, max(src - 1, 0));
+      const int before = src == 0 ? 0 : __shfl_sync(0xffffffffu, incl, max(src - 1, 0));
       Item im;
       im.tok0 = __shfl_sync(0xffffffffu, sq.tok0, src);
       im.qlen = __shfl_sync(0xffffffffu, sq.qlen, src);
@@ -268,7 +279,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int b = __shfl_sync(0xffffffffu, run, src);
       // Within a run the heaviest causal pairs first: pair by pair over the KV heads, whose keys stay
       // in L2, or KV head by KV head when there are more pairs than a few rounds of the CTAs.
-      const int x = (int)(item - done - before);
+      const int x = item - done - before;
       const int n_pairs = (im.qlen + rows2 - 1) / rows2;
       const int split = x % p.splits;
       const int y = x / p.splits;
@@ -286,8 +297,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       int n1 = im.pos0 + p.ppt < im.qlen
                    ? blocks_upto(p, npb, im.len, im.qlen, min(im.pos0 + rows2, im.qlen)) : 0;
       const int n = max(n0, n1);
-      im.kb0 = (int)((long long)n * split / p.splits);
-      im.n_blocks = (int)((long long)n * (split + 1) / p.splits) - im.kb0;
+      // (n < 2^25 blocks, splits <= SMs: the products fit in 32 bits without a sign)
+      im.kb0 = (int)((unsigned)n * split / p.splits);
+      im.n_blocks = (int)((unsigned)n * (split + 1) / p.splits) - im.kb0;
       im.n_tile0 = min(max(n0 - im.kb0, 0), im.n_blocks);
       im.n_tile1 = min(max(n1 - im.kb0, 0), im.n_blocks);
       im.part = ((b * p.pairs_per_seq + pair) * p.Hkv + im.hk) * p.splits + split;
@@ -298,16 +310,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
       if (im.n_blocks == 0) continue;
-      // Q of this item once the previous item's last QK has read the old one.
-      if (!wait_bar_warp(q_empty, (uint32_t)(qi & 1) ^ 1, g, 11, k)) { ok = false; break; }
-      if (lane == 0) {
-        bar_arrive_expect_tx(q_full, (uint32_t)(2 * kCh * p.ppt * p.group * 128));
-        for (int t = 0; t < 2; ++t)
-          for (int c = 0; c < kCh; ++c)
-            tma_load_3d(sQ + t * C::kTileBytes + c * kChunk, &tmQ, c * 64, im.hk * p.group,
-                        im.tok0 + im.pos0 + t * p.ppt, q_full);
+      // Q of this item once the previous item's last QK has read the old one (the first item's Q
+      // comes from the P·V warp, beside the first K block).
+      if (qi > 0) {
+        if (!wait_bar_warp(q_empty, (uint32_t)(qi & 1) ^ 1, g, 11, k)) { ok = false; break; }
+        if (lane == 0) load_q(im);
+        __syncwarp();
       }
-      __syncwarp();
       ++qi;
       const int* row = p.seqs.table + b * p.seqs.table_stride;
       // the prefix's blocks, then the sequence's own
@@ -345,7 +354,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     if (!ok && lane == 0) {
-      // Let every copy this warp started land before the CTA's shared memory goes away.
+      // Let every copy in flight land before the CTA's shared memory goes away.
       if (qi > 0) drain_wait(q_full, (uint32_t)((qi - 1) & 1), p.timeout_ns);
       for (int i = max(0, rn - R); i < rn; ++i)
         drain_wait(&ring_full[i % R], (uint32_t)((i / R) & 1), p.timeout_ns);
@@ -375,6 +384,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (elect_one()) bar_arrive(&i_empty[islot]);
       if (it.last) break;
       if (it.n_blocks == 0) continue;
+      if (!qk_role && qi == 0 && lane == 0) load_q(it);
+      __syncwarp();
       const int nt[2] = {it.n_tile0, it.n_tile1};
       const int nb = it.n_blocks;
       int ring_seen = -1;     // this warp's ring slots of the item already waited for
@@ -826,18 +837,20 @@ int64_t tile_pairs(const lvb_paged_desc* d, int parts) {
   const int64_t rows2 = 2 * positions_per_tile(d);
   return (rows + rows2 - 1) / rows2;
 }
-int64_t most_items(const lvb_paged_desc* d, int parts) {
-  return tile_pairs(d, parts) * d->heads_kv * (parts == kFlashPrefix ? 1 : d->batch);
-}
 
 }  // namespace
+
+// Items without the splits, at most.
+int64_t paged_flash_items(const lvb_paged_desc* d, int parts) {
+  return tile_pairs(d, parts) * d->heads_kv * (parts == kFlashPrefix ? 1 : d->batch);
+}
 
 // Key ranges per tile pair: with fewer items than SMs, as many as fill the SMs once, down to one
 // block of the longest run of keys (the prefix's length; a table's row otherwise). (At least one,
 // two, four, eight blocks: a prefix of 500 keys 13.5, 14.8, 18.4, 18.4 us, of 4,099 keys over 64-wide
 // heads 30.4, 32.1, 30.5, 34.5 us.)
 int paged_flash_splits(const lvb_paged_desc* d, int sm_count, int parts) {
-  const int64_t items = std::max<int64_t>(1, most_items(d, parts));
+  const int64_t items = std::max<int64_t>(1, paged_flash_items(d, parts));
   int64_t keys = 0;
   if (parts & kFlashPrefix) keys += d->prefix_len;
   if (parts & kFlashOwn) keys += d->table_width * d->page_size;
@@ -849,7 +862,7 @@ int paged_flash_splits(const lvb_paged_desc* d, int sm_count, int parts) {
 
 size_t paged_flash_workspace(const lvb_paged_desc* d, int splits, int parts) {
   const bool store = splits > 1 || parts == kFlashPrefix;
-  return kCounterBytes + (store ? (size_t)most_items(d, parts) * splits * 256 * (d->head_dim + 2) * sizeof(float) : 0);
+  return kCounterBytes + (store ? (size_t)paged_flash_items(d, parts) * splits * 256 * (d->head_dim + 2) * sizeof(float) : 0);
 }
 
 int paged_flash_launch(const lvb_paged_desc* d, const PagedLayout& lay, const PagedSeqs& seqs,
@@ -877,7 +890,7 @@ int paged_flash_launch(const lvb_paged_desc* d, const PagedLayout& lay, const Pa
   p.o_sh = lay.o[1];
   p.lse = lse;
   p.timeout_ns = wait_timeout_ns();
-  const int64_t items = most_items(d, parts) * splits;
+  const int64_t items = paged_flash_items(d, parts) * splits;
   p.tile_o = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(ws) + kCounterBytes);
   p.tile_ml = p.tile_o + (p.store_parts ? (size_t)items * 256 * d->head_dim : 0);
   *out = FlashWorkspace{p.tile_o, p.tile_ml};

@@ -171,6 +171,7 @@ struct FlashWorkspace {
   float* tile_ml;
 };
 enum { kFlashOwn = 1, kFlashPrefix = 2 };
+int64_t paged_flash_items(const lvb_paged_desc* d, int parts);
 int paged_flash_splits(const lvb_paged_desc* d, int sm_count, int parts);
 size_t paged_flash_workspace(const lvb_paged_desc* d, int splits, int parts);
 int paged_flash_launch(const lvb_paged_desc* d, const PagedLayout& lay, const PagedSeqs& seqs,
