@@ -500,15 +500,15 @@ typedef struct lvb_paged_plan {
   int32_t prefix_splits;  /* > 0: the prefix is read once for all query rows of a KV head, in
                              this many key ranges, and joined with the sequences' own part;
                              0: no prefix, or (LVB_PAGED_FLASH) read by every sequence's tiles */
-  int32_t cluster;        /* LVB_PAGED_DECODE: CTAs per (sequence, KV head) that join their parts in
-                             shared memory; 0: blocks dealt to all CTAs, parts joined by a second
-                             kernel */
+  int32_t cluster;        /* CTAs of a (sequence, KV head), or of a split tile pair, that join their
+                             parts in shared memory; 0: no such clusters */
   int32_t launches;       /* kernel launches per call */
   int32_t reserved;
   int64_t workspace_bytes;
 } lvb_paged_plan;
 
 int lvb_attention_paged_check(const lvb_paged_desc* d);
+/* (How many clusters a GPU runs at once differs from chip to chip; the plan takes a usual one's.) */
 int lvb_attention_paged_plan_for(const lvb_paged_desc* d, int32_t sm_count, lvb_paged_plan* out);
 /* Enqueue it. cu_q may be NULL (max_q rows per sequence). prefix_table: the prefix's pages
  * ((prefix_len + page_size - 1) / page_size entries; NULL without one). */

@@ -4,6 +4,7 @@
 #include <cstring>
 
 #include <algorithm>
+#include <mutex>
 
 #include "paged.cuh"
 
@@ -153,11 +154,103 @@ bool use_decode(const lvb_paged_desc* d) {
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
+// The numbers of clusters as measured on a B200, for a plan without a device, scaled to `sm_count`.
+PagedRoom static_room(int sm_count) {
+  static const int k148[kMostCluster + 1] = {0, 148, 74, 45, 33, 26, 22, 15, 15, 15, 11, 7, 7, 7, 7, 7, 7};
+  PagedRoom r;
+  r.sms = sm_count;
+  for (int c = 0; c <= kMostCluster; ++c) r.clusters[c] = (int)((int64_t)k148[c] * sm_count / 148);
+  return r;
+}
+
+__global__ void cluster_probe_kernel() {}
+
+// The device's own numbers, asked once.
+int device_room(DeviceState* dev, PagedRoom* out, const char* op) {
+  struct Asked {
+    std::once_flag once;
+    PagedRoom room;
+  };
+  static Asked asked[64];
+  if (dev->device < 0 || dev->device >= 64) {
+    *out = static_room(dev->sm_count);
+    return LVB_OK;
+  }
+  Asked& a = asked[dev->device];
+  std::call_once(a.once, [&] {
+    a.room = static_room(dev->sm_count);
+    const int smem = 220 * 1024;
+    if (cudaFuncSetAttribute(cluster_probe_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+        cudaFuncSetAttribute(cluster_probe_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+      cudaGetLastError();
+      return;
+    }
+    for (int c = 2; c <= kMostCluster; ++c) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(c);
+      cfg.blockDim = dim3(384);
+      cfg.dynamicSmemBytes = smem;
+      cudaLaunchAttribute at[1];
+      at[0].id = cudaLaunchAttributeClusterDimension;
+      at[0].val.clusterDim.x = (unsigned)c;
+      at[0].val.clusterDim.y = 1;
+      at[0].val.clusterDim.z = 1;
+      cfg.attrs = at;
+      cfg.numAttrs = 1;
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, cluster_probe_kernel, &cfg) == cudaSuccess) {
+        a.room.clusters[c] = n;
+      } else {
+        cudaGetLastError();
+        a.room.clusters[c] = 0;      // such clusters are not used
+      }
+    }
+  });
+  *out = a.room;
+  return LVB_OK;
+}
+
+FlashSplit flash_split(const lvb_paged_plan& pl) {
+  if (pl.kernel == LVB_PAGED_FLASH) return FlashSplit{pl.splits, std::max(1, pl.cluster)};
+  return FlashSplit{pl.prefix_splits, 1};
+}
+
 // Workspace of a planned call: the flash kernel's, then the decoding kernel's.
 size_t flash_bytes(const lvb_paged_desc* d, const lvb_paged_plan& pl) {
   if (pl.kernel == LVB_PAGED_FLASH)
-    return up256(paged_flash_workspace(d, pl.splits, kFlashOwn | (d->prefix_len ? kFlashPrefix : 0)));
-  return pl.prefix_splits ? up256(paged_flash_workspace(d, pl.prefix_splits, kFlashPrefix)) : 0;
+    return up256(paged_flash_workspace(d, flash_split(pl), kFlashOwn | (d->prefix_len ? kFlashPrefix : 0)));
+  return pl.prefix_splits ? up256(paged_flash_workspace(d, flash_split(pl), kFlashPrefix)) : 0;
+}
+
+int plan_paged(const lvb_paged_desc* d, const PagedRoom& room, lvb_paged_plan* out) {
+  const char* op = "lvb_attention_paged";
+  std::memset(out, 0, sizeof *out);
+  out->splits = 1;
+  if (d->batch == 0 || d->tokens == 0 || d->max_q == 0 || d->heads_q == 0) return LVB_OK;
+  if (use_decode(d)) {
+    out->kernel = LVB_PAGED_DECODE;
+    out->launches = 2;
+    if (d->prefix_len) {
+      out->prefix_splits = paged_flash_split(d, room, kFlashPrefix).splits;
+      out->launches = 3;
+    } else if ((out->cluster = paged_decode_cluster(d, room)) > 0) {
+      out->launches = 1;      // no parts in memory
+      return LVB_OK;
+    }
+    out->workspace_bytes = (int64_t)(flash_bytes(d, *out) +
+                                     paged_decode_workspace(d, room.sms, d->prefix_len > 0));
+    return LVB_OK;
+  }
+  out->kernel = LVB_PAGED_FLASH;
+  const int parts = kFlashOwn | (d->prefix_len ? kFlashPrefix : 0);
+  if (paged_flash_items(d, parts) > INT32_MAX - 65536)
+    return fail(LVB_ERR_UNSUPPORTED, op, "more than 2^31 query tiles", "split the batch");
+  const FlashSplit fs = paged_flash_split(d, room, parts);
+  out->splits = fs.splits;
+  out->cluster = fs.cluster > 1 ? fs.cluster : 0;
+  out->launches = fs.splits > fs.cluster ? 2 : 1;
+  out->workspace_bytes = (int64_t)flash_bytes(d, *out);
+  return LVB_OK;
 }
 
 }  // namespace
@@ -290,31 +383,7 @@ int lvb_attention_paged_plan_for(const lvb_paged_desc* d, int32_t sm_count, lvb_
   int st = lvb_attention_paged_check(d);
   if (st) return st;
   if (!out) return fail(LVB_ERR_INVALID_ARG, op, "plan is NULL");
-  if (sm_count <= 0) sm_count = 148;
-  std::memset(out, 0, sizeof *out);
-  out->splits = 1;
-  if (d->batch == 0 || d->tokens == 0 || d->max_q == 0 || d->heads_q == 0) return LVB_OK;
-  if (use_decode(d)) {
-    out->kernel = LVB_PAGED_DECODE;
-    out->launches = 2;
-    if (d->prefix_len) {
-      out->prefix_splits = paged_flash_splits(d, sm_count, kFlashPrefix);
-      out->launches = 3;
-    } else if ((out->cluster = paged_decode_cluster(d, sm_count)) > 0) {
-      out->launches = 1;      // no parts in memory
-      return LVB_OK;
-    }
-    out->workspace_bytes = (int64_t)(flash_bytes(d, *out) +
-                                     paged_decode_workspace(d, sm_count, d->prefix_len > 0));
-    return LVB_OK;
-  }
-  out->kernel = LVB_PAGED_FLASH;
-  if (paged_flash_items(d, kFlashOwn) > INT32_MAX - 65536)
-    return fail(LVB_ERR_UNSUPPORTED, op, "more than 2^31 query tiles", "split the batch");
-  out->splits = paged_flash_splits(d, sm_count, kFlashOwn | (d->prefix_len ? kFlashPrefix : 0));
-  out->launches = out->splits > 1 ? 2 : 1;
-  out->workspace_bytes = (int64_t)flash_bytes(d, *out);
-  return LVB_OK;
+  return plan_paged(d, static_room(sm_count > 0 ? sm_count : 148), out);
 }
 
 int lvb_attention_paged(const lvb_paged_desc* d, const void* Q, const void* Kc, const void* Vc,
@@ -334,7 +403,8 @@ int lvb_attention_paged(const lvb_paged_desc* d, const void* Q, const void* Kc, 
   DeviceState* dev = current_device_state(op);
   if (!dev) return LVB_ERR_NO_DEVICE;
   lvb_paged_plan pl;
-  if ((st = lvb_attention_paged_plan_for(d, dev->sm_count, &pl))) return st;
+  PagedRoom room;
+  if ((st = device_room(dev, &room, op)) || (st = plan_paged(d, room, &pl))) return st;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const PagedLayout lay = paged_layout(*d);
   MergeParams mp = {};
@@ -348,7 +418,7 @@ int lvb_attention_paged(const lvb_paged_desc* d, const void* Q, const void* Kc, 
   mp.o_sh = lay.o[1];
   mp.lse = lse;
   uint8_t* ws = nullptr;
-  if (pl.cluster > 0) {
+  if (pl.kernel == LVB_PAGED_DECODE && pl.cluster > 0) {
     DecodeWorkspace none = {};
     return paged_decode_launch(d, lay, mp.seqs, Q, Kc, Vc, O, lse, false, false, pl.cluster, ws, &none,
                                s, dev);
@@ -360,7 +430,7 @@ int lvb_attention_paged(const lvb_paged_desc* d, const void* Q, const void* Kc, 
   const size_t fb = flash_bytes(d, pl);
   if (pl.kernel == LVB_PAGED_DECODE) {
     if (pl.prefix_splits) {
-      st = paged_flash_launch(d, lay, mp.seqs, Q, Kc, Vc, O, lse, kFlashPrefix, pl.prefix_splits, ws,
+      st = paged_flash_launch(d, lay, mp.seqs, Q, Kc, Vc, O, lse, kFlashPrefix, flash_split(pl), ws,
                               &fw, s, dev);
       mp.tile_o = fw.tile_o;
       mp.tile_ml = fw.tile_ml;
@@ -377,17 +447,18 @@ int lvb_attention_paged(const lvb_paged_desc* d, const void* Q, const void* Kc, 
     mp.dec_slots = dw.slots;
     mp.dec_ctas = dw.ctas;
     // about as many pieces per item as there are CTAs for each, and one more
-    const int pieces = dw.ctas / (int)(d->batch * d->heads_kv) + 2 + pl.prefix_splits;
+    const int pieces = dw.ctas / (int)(d->batch * d->heads_kv) + 2 + mp.tile_splits;
     mp.warps_per_row = pieces <= 8 ? 1 : pieces <= 16 ? 2 : 4;
     if (st == LVB_OK) st = merge_launch(mp, (int)d->head_dim, bf16, s, dev);
   } else {
     const int parts = kFlashOwn | (d->prefix_len ? kFlashPrefix : 0);
-    st = paged_flash_launch(d, lay, mp.seqs, Q, Kc, Vc, O, lse, parts, pl.splits, ws, &fw, s, dev);
-    if (st == LVB_OK && pl.splits > 1) {
+    st = paged_flash_launch(d, lay, mp.seqs, Q, Kc, Vc, O, lse, parts, flash_split(pl), ws, &fw, s, dev);
+    const int groups = pl.splits / std::max(1, pl.cluster);
+    if (st == LVB_OK && groups > 1) {
       mp.tile_o = fw.tile_o;
       mp.tile_ml = fw.tile_ml;
-      mp.tile_splits = pl.splits;
-      mp.warps_per_row = pl.splits <= 8 ? 1 : pl.splits <= 16 ? 2 : 4;
+      mp.tile_splits = groups;
+      mp.warps_per_row = groups <= 8 ? 1 : groups <= 16 ? 2 : 4;
       mp.pairs_per_seq = (int)((d->max_q + 2 * mp.ppt - 1) / (2 * mp.ppt));
       st = merge_launch(mp, (int)d->head_dim, bf16, s, dev);
     }

@@ -960,19 +960,16 @@ size_t decode_slots(const lvb_paged_desc* d, int sm_count, bool keep_parts) {
 
 }  // namespace
 
-// As many CTAs per item as fill the SMs once (a power of two up to 16; a cluster lies in one GPC, of
-// which 16 CTAs leave about two SMs idle and 8 one). Taken when a full table gives a CTA at most
-// eight blocks (so unequal lengths cost no more than that), or when one sequence fills at least
-// four fifths of the SMs.
-int paged_decode_cluster(const lvb_paged_desc* d, int sm_count) {
+// As many CTAs per item as run at once, and no more than shorten the longest CTA's run. Taken when a
+// full table gives a CTA at most eight blocks, so that unequal lengths cost no more than that.
+int paged_decode_cluster(const lvb_paged_desc* d, const PagedRoom& room) {
   const int64_t items = d->batch * d->heads_kv;
-  const int64_t blocks = (d->table_width * d->page_size + 127) / 128;
-  int cs = 16;
-  while (cs > 0 && sm_count / (cs + cs / 8) < items) cs /= 2;
-  while (cs > 1 && cs / 2 >= blocks) cs /= 2;      // no CTA without a block
-  if (cs == 0) return 0;
-  if (blocks <= 8LL * cs) return cs;
-  return d->batch == 1 && items * cs * 5 >= 4LL * sm_count ? cs : 0;
+  const int64_t blocks = std::max<int64_t>(1, (d->table_width * d->page_size + 127) / 128);
+  int c = kMostCluster;
+  while (c > 0 && (c == 1 ? room.sms : room.clusters[c]) < items) --c;
+  if (c == 0 || blocks > 8LL * c) return 0;
+  const int64_t longest = (blocks + c - 1) / c;
+  return (int)((blocks + longest - 1) / longest);
 }
 
 size_t paged_decode_workspace(const lvb_paged_desc* d, int sm_count, bool keep_parts) {

@@ -14,8 +14,11 @@
 //   * an item = (sequence, KV head, pair of tiles, key range) is worked out from the lengths on
 //     the device by the TMA warp, which publishes all of it through the item queue;
 //   * with few items (a small chunk over a long cache, a prefix) the key blocks of a tile pair
-//     are split over several CTAs, and each leaves (O, m, l) in 32 bits for the join.
+//     are split over several CTAs, which join their O, m and l (in 32 bits) in a cluster through
+//     distributed shared memory, or leave them in memory for the join kernel (the rule is at
+//     paged_flash_split).
 #include <algorithm>
+#include <climits>
 #include <cmath>
 
 #include "paged.cuh"
@@ -38,6 +41,7 @@ struct FlashParams {
   int all_rows;                // 1: one run of rows, tokens 0..tokens-1 (prefix only)
   int splits, pairs_per_seq;   // pairs_per_seq: rows of the parts' index per sequence
   int store_parts;
+  int cluster;                 // CTAs per cluster (of a pair's splits), one item per CTA; 0: none
   int* counter;                // items are taken from it; NULL: item blockIdx.x, + gridDim.x, ...
   float scale_log2;
   void* O;
@@ -181,6 +185,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   griddep_wait();
   griddep_launch_dependents();
   const int npb = (p.prefix + 127) / 128;
+  float part_m = -INFINITY, part_l = 0.f;      // a softmax thread's row of its CTA's part (clusters)
+  int part_nt = 0;
 
   auto load_q = [&](const Item& im) {
     bar_arrive_expect_tx(q_full, (uint32_t)(2 * kCh * p.ppt * p.group * 128));
@@ -243,7 +249,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     fetch();
     int item = blockIdx.x;
     for (int k = 0; ok; ++k) {
-      if (p.counter) {
+      if (p.cluster && k > 0) {
+        item = INT_MAX;            // the one item of this CTA is done
+      } else if (p.counter) {
         if (lane == 0) item = atomicAdd(p.counter, 1);
         item = __shfl_sync(0xffffffffu, item, 0);
       } else if (k > 0) {
@@ -302,7 +310,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       im.n_blocks = (int)((unsigned)n * (split + 1) / p.splits) - im.kb0;
       im.n_tile0 = min(max(n0 - im.kb0, 0), im.n_blocks);
       im.n_tile1 = min(max(n1 - im.kb0, 0), im.n_blocks);
-      im.part = ((b * p.pairs_per_seq + pair) * p.Hkv + im.hk) * p.splits + split;
+      im.part = (b * p.pairs_per_seq + pair) * p.Hkv + im.hk;
+      im.part = p.cluster ? im.part * (p.splits / p.cluster) + split / p.cluster
+                          : im.part * p.splits + split;
       im.last = 0;
       if (lane == 0) {
         items[slot] = im;
@@ -618,7 +628,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const long long tok = it.tok0 + pos;
       const int h = it.hk * p.group + row_head;
-      if (p.store_parts) {
+      if (p.cluster) {
+        // O stays in TMEM until the CTA's products are done (below)
+        part_m = m_ref;
+        part_l = l;
+        part_nt = nt;
+      } else if (p.store_parts) {
         const long long at = (long long)it.part * 256 + t * 128 + r;
         if (row_ok) {
           p.tile_ml[at * 2] = m_ref;
@@ -678,6 +693,108 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
 
+  if (p.cluster) {
+    // The cluster's join. Each CTA copies its O, and m and l, into shared memory over Q and the ring
+    // (16-byte unit c of row r at c ^ (r % 8): the threads of a store lie in different banks); row r
+    // of the pair is then joined by CTA r % cluster.
+    constexpr int V = D / 32;
+    float* sO = reinterpret_cast<float*>(smem);               // [256][D]
+    float2* sMl = reinterpret_cast<float2*>(smem + 256 * D * 4);
+    tc_fence_before();
+    __syncthreads();          // every product and copy of this CTA is done
+    tc_fence_after();
+    const bool bad = *abort_flag != 0;
+    if (warp != kQkWarp && warp != kPvWarp && warp != kTmaWarp) {
+      const int t = (warp - 2) >> 2, wl = warp & 3, r = t * 128 + wl * 32 + lane;
+      const uint32_t tO = tmem + ((uint32_t)(wl * 32) << 16) + 256 + 128 * t;
+      sMl[r] = make_float2(part_m, bad ? -1.f : part_l);      // after a wait gave up: store nothing
+      if (part_nt > 0) {
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(tO + 32 * c, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            st_shared_v4(smem_u32(sO) + r * D * 4 + (((8 * c + e) ^ (r & 7)) << 4), o[4 * e],
+                         o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+        }
+      }
+    }
+    cluster_sync_all();
+    const Item& im = items[0];
+    const int rank = blockIdx.x % p.cluster;
+    const int rows = im.last ? 0 : 256;
+    const uint32_t o_addr = smem_u32(sO), ml_addr = smem_u32(sMl);
+    for (int r = rank + (int)warp * p.cluster; r < rows; r += p.cluster * (kThreads / 32)) {
+      const int t = r >> 7, row_pos = (r & 127) / p.group;
+      const int pos = im.pos0 + t * p.ppt + row_pos;
+      if (row_pos >= p.ppt || pos >= im.qlen) continue;
+      float pm = -INFINITY, pl = 0.f;            // lane k: part k's m and l
+      if ((int)lane < p.cluster) {
+        const float2 x = ld_cluster_f32x2(mapa_shared(ml_addr + r * 8, lane));
+        pm = x.x;
+        pl = x.y;
+      }
+      // all parts' rows under way at once (of a part without a key: whatever lies there)
+      const uint32_t col = V == 4 ? ((lane ^ (r & 7)) << 4) : (((lane >> 1) ^ (r & 7)) << 4) + (lane & 1) * 8;
+      float o[16][V];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        if (k < p.cluster) {
+          const uint32_t a = mapa_shared(o_addr + r * D * 4 + col, k);
+          if constexpr (V == 4) {
+            const float4 f = ld_cluster_f32x4(a);
+            o[k][0] = f.x, o[k][1] = f.y, o[k][2] = f.z, o[k][3] = f.w;
+          } else {
+            const float2 f = ld_cluster_f32x2(a);
+            o[k][0] = f.x, o[k][1] = f.y;
+          }
+        }
+      }
+      const bool gave_up = __any_sync(0xffffffffu, pl < 0.f);
+      const bool some = pl != 0.f;
+      float mx = some ? pm : -INFINITY;
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+      const float mu = mx == -INFINITY ? 0.f : mx;
+      const float pw = some ? fast_exp2(pm - mu) : 0.f;
+      float den = some ? pw * pl : 0.f;
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) den += __shfl_xor_sync(0xffffffffu, den, x);
+      const unsigned parts = __ballot_sync(0xffffffffu, some);
+      float acc[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] = 0.f;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const float wk = __shfl_sync(0xffffffffu, pw, k);
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (parts >> k & 1) acc[e] += wk * o[k][e];
+      }
+      if (gave_up) continue;
+      if (p.store_parts) {
+        // one part for the join with the sequences' own
+        const long long at = (long long)im.part * 256 + r;
+        if (lane == 0) *reinterpret_cast<float2*>(&p.tile_ml[at * 2]) = make_float2(mu, den);
+        float* dst = p.tile_o + at * D + lane * V;
+        if constexpr (V == 4) *reinterpret_cast<float4*>(dst) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        else *reinterpret_cast<float2*>(dst) = make_float2(acc[0], acc[1]);
+      } else {
+        const long long tok = im.tok0 + pos;
+        const int h = im.hk * p.group + (r & 127) - row_pos * p.group;
+        const float inv = den == 0.f ? 0.f : 1.f / den;
+        uint16_t* dst = reinterpret_cast<uint16_t*>(p.O) + tok * p.o_st + h * p.o_sh + lane * V;
+#pragma unroll
+        for (int e = 0; e < V; e += 2)
+          *reinterpret_cast<uint32_t*>(dst + e) = pack2<BF16>(acc[e] * inv, acc[e + 1] * inv);
+        if (p.lse && lane == 0)
+          p.lse[tok * p.Hq + h] = den == 0.f ? -INFINITY : (mu + log2f(den)) * 0.69314718055994530942f;
+      }
+    }
+    cluster_sync_all();      // no CTA leaves while another reads its part
+  }
   tc_fence_before();
   __syncthreads();
   if (warp == kQkWarp) {
@@ -821,8 +938,8 @@ template <int D, bool BF16>
 int launch_flash(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                  const FlashParams& p, int ctas, cudaStream_t stream, DeviceState* dev) {
   static SmemAttr attr;
-  return launch_serial("lvb_attention_paged", paged_flash_kernel<D, BF16>, attr, dev, ctas, kThreads,
-                       Cfg<D>::kSmem, stream, tq, tk, tv, p);
+  return launch_cluster("lvb_attention_paged", paged_flash_kernel<D, BF16>, attr, dev, ctas, kThreads,
+                        Cfg<D>::kSmem, std::max(1, p.cluster), stream, tq, tk, tv, p);
 }
 
 constexpr size_t kCounterBytes = 256;   // the item counter, before the 32-byte stores' parts
@@ -845,29 +962,48 @@ int64_t paged_flash_items(const lvb_paged_desc* d, int parts) {
   return tile_pairs(d, parts) * d->heads_kv * (parts == kFlashPrefix ? 1 : d->batch);
 }
 
-// Key ranges per tile pair: with fewer items than SMs, as many as fill the SMs once, down to one
-// block of the longest run of keys (the prefix's length; a table's row otherwise). (At least one,
-// two, four, eight blocks: a prefix of 500 keys 13.5, 14.8, 18.4, 18.4 us, of 4,099 keys over 64-wide
-// heads 30.4, 32.1, 30.5, 34.5 us.)
-int paged_flash_splits(const lvb_paged_desc* d, int sm_count, int parts) {
+// With fewer items than SMs: key ranges (of the prefix's length; of a table's row otherwise), by the
+// cost of a CTA's blocks (1.8 us each) and of a part that goes through memory (0.45 us with its
+// share of the join; of a prefix's, that are joined while more is going on, a tenth: 4,099 keys over
+// 64-wide heads in 16 ranges 31.0 us, in 11 34.5). The sequences' own ranges meet in clusters where that spares the join kernel
+// or most of its work (a cluster's join 1.5 us, the kernel 4 us): 64 new tokens of one sequence over
+// 1,000, 4,000 and 16,000 keys 14.8, 20.3 and 35.4 us with clusters, 21.6, 26.9 and 38.9 without. A
+// prefix's do not: the decoding kernel fills the SMs as its CTAs end, and the join kernel runs
+// anyway (16,384 keys before 64 sequences 87.2 us with clusters, 84.9 without).
+FlashSplit paged_flash_split(const lvb_paged_desc* d, const PagedRoom& room, int parts) {
   const int64_t items = std::max<int64_t>(1, paged_flash_items(d, parts));
   int64_t keys = 0;
   if (parts & kFlashPrefix) keys += d->prefix_len;
   if (parts & kFlashOwn) keys += d->table_width * d->page_size;
-  const int64_t blocks = (keys + 127) / 128;
-  int64_t s = std::max(1, sm_count) / items;
-  s = std::min<int64_t>(s, blocks);
-  return (int)std::max<int64_t>(1, s);
+  const int64_t blocks = std::max<int64_t>(1, (keys + 127) / 128);
+  FlashSplit best{1, 1};
+  if (2 * items > room.sms) return best;
+  double least = 1e30;
+  for (int c = 1; c <= (parts == kFlashPrefix ? 1 : kMostCluster); ++c) {
+    const int64_t most = (c == 1 ? room.sms : room.clusters[c]) / items;   // groups that run at once
+    for (int64_t g = 1; g <= most && g * c <= blocks; ++g) {
+      const double cost = 1.8 * (double)((blocks + g * c - 1) / (g * c)) +
+                          (parts == kFlashPrefix ? 0.05 : 0.45) * (double)g +
+                          (c > 1 ? 1.5 : 0.0) + (parts != kFlashPrefix && g > 1 ? 4.0 : 0.0);
+      if (cost < least - 1e-9) {
+        least = cost;
+        best = FlashSplit{(int)(g * c), c};
+      }
+    }
+  }
+  return best;
 }
 
-size_t paged_flash_workspace(const lvb_paged_desc* d, int splits, int parts) {
-  const bool store = splits > 1 || parts == kFlashPrefix;
-  return kCounterBytes + (store ? (size_t)paged_flash_items(d, parts) * splits * 256 * (d->head_dim + 2) * sizeof(float) : 0);
+size_t paged_flash_workspace(const lvb_paged_desc* d, FlashSplit fs, int parts) {
+  const int groups = fs.splits / fs.cluster;
+  const bool store = parts == kFlashPrefix || groups > 1;
+  return kCounterBytes + (store ? (size_t)paged_flash_items(d, parts) * groups * 256 *
+                                      (d->head_dim + 2) * sizeof(float) : 0);
 }
 
 int paged_flash_launch(const lvb_paged_desc* d, const PagedLayout& lay, const PagedSeqs& seqs,
                        const void* Q, const void* Kc, const void* Vc, void* O, float* lse, int parts,
-                       int splits, void* ws, FlashWorkspace* out, cudaStream_t stream,
+                       FlashSplit fs, void* ws, FlashWorkspace* out, cudaStream_t stream,
                        DeviceState* dev) {
   const char* op = "lvb_attention_paged";
   FlashParams p = {};
@@ -881,18 +1017,20 @@ int paged_flash_launch(const lvb_paged_desc* d, const PagedLayout& lay, const Pa
   p.own = (parts & kFlashOwn) ? 1 : 0;
   p.prefix = (parts & kFlashPrefix) ? (int)d->prefix_len : 0;
   p.all_rows = parts == kFlashPrefix ? 1 : 0;
-  p.splits = splits;
+  p.splits = fs.splits;
   p.pairs_per_seq = (int)tile_pairs(d, parts);
-  p.store_parts = splits > 1 || p.all_rows ? 1 : 0;
+  p.cluster = fs.cluster > 1 ? fs.cluster : 0;
+  p.store_parts = p.all_rows || fs.splits > fs.cluster ? 1 : 0;
   p.scale_log2 = d->scale * 1.4426950408889634f;
   p.O = O;
   p.o_st = lay.o[0];
   p.o_sh = lay.o[1];
   p.lse = lse;
   p.timeout_ns = wait_timeout_ns();
-  const int64_t items = paged_flash_items(d, parts) * splits;
+  const int64_t items = paged_flash_items(d, parts) * fs.splits;
   p.tile_o = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(ws) + kCounterBytes);
-  p.tile_ml = p.tile_o + (p.store_parts ? (size_t)items * 256 * d->head_dim : 0);
+  const size_t stored = (size_t)(items / fs.cluster);
+  p.tile_ml = p.tile_o + (p.store_parts ? stored * 256 * d->head_dim : 0);
   *out = FlashWorkspace{p.tile_o, p.tile_ml};
   CUtensorMap tq, tk, tv;
   {
@@ -904,10 +1042,10 @@ int paged_flash_launch(const lvb_paged_desc* d, const PagedLayout& lay, const Pa
   }
   int st = paged_kv_maps(&tk, &tv, d, lay, Kc, Vc, op);
   if (st) return st;
-  const int ctas = (int)std::min<int64_t>(items, std::max(1, dev->sm_count));
+  const int ctas = p.cluster ? (int)items : (int)std::min<int64_t>(items, std::max(1, dev->sm_count));
   // Items of different length are taken from a counter (zeroed on the stream before the launch);
   // a prefix's are alike and dealt in order.
-  if (!p.all_rows) {
+  if (!p.all_rows && !p.cluster) {
     p.counter = reinterpret_cast<int*>(ws);
     cudaError_t e = cudaMemsetAsync(ws, 0, sizeof(int), stream);
     if (e != cudaSuccess) return fail_cuda(e, op, "work counter reset");

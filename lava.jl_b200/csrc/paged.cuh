@@ -104,6 +104,14 @@ int paged_kv_maps(CUtensorMap* tk, CUtensorMap* tv, const lvb_paged_desc* d, con
 void paged_seqs(PagedSeqs* p, const lvb_paged_desc& d, const int32_t* table,
                 const int32_t* seq_lens, const int32_t* cu_q, const int32_t* prefix_table,
                 DeviceState* dev);
+// How many CTAs with most of an SM's shared memory run at once: clusters of a size lie in one GPC, so
+// their number depends on the chip's (measured here: 33 clusters of 4, 15 of 9, 7 of 16).
+constexpr int kMostCluster = 16;
+struct PagedRoom {
+  int sms;
+  int clusters[kMostCluster + 1];   // [size]
+};
+
 // Slots per TMA box: min(128, the largest power of two dividing the page size).
 inline int paged_box(int64_t page_size) {
   int b = 8;
@@ -155,7 +163,7 @@ struct DecodeWorkspace {
   int rows, slots, ctas;
 };
 // CTAs per item when its blocks are split over a cluster, 0 when they are dealt to all CTAs.
-int paged_decode_cluster(const lvb_paged_desc* d, int sm_count);
+int paged_decode_cluster(const lvb_paged_desc* d, const PagedRoom& room);
 size_t paged_decode_workspace(const lvb_paged_desc* d, int sm_count, bool keep_parts);
 // keep_parts: every item's result stays in the workspace for the join with a prefix's parts.
 // after_prefix: the kernel before it is the same call's flash kernel over the prefix.
@@ -172,11 +180,15 @@ struct FlashWorkspace {
 };
 enum { kFlashOwn = 1, kFlashPrefix = 2 };
 int64_t paged_flash_items(const lvb_paged_desc* d, int parts);
-int paged_flash_splits(const lvb_paged_desc* d, int sm_count, int parts);
-size_t paged_flash_workspace(const lvb_paged_desc* d, int splits, int parts);
+// Key ranges per tile pair, and how many of them form a cluster (1: none).
+struct FlashSplit {
+  int splits, cluster;
+};
+FlashSplit paged_flash_split(const lvb_paged_desc* d, const PagedRoom& room, int parts);
+size_t paged_flash_workspace(const lvb_paged_desc* d, FlashSplit fs, int parts);
 int paged_flash_launch(const lvb_paged_desc* d, const PagedLayout& lay, const PagedSeqs& seqs,
                        const void* Q, const void* Kc, const void* Vc, void* O, float* lse, int parts,
-                       int splits, void* ws, FlashWorkspace* out, cudaStream_t stream,
+                       FlashSplit fs, void* ws, FlashWorkspace* out, cudaStream_t stream,
                        DeviceState* dev);
 
 struct SeqInfo {

@@ -258,12 +258,12 @@ def test_plans(lvb):
     assert (p.kernel, p.prefix_splits, p.launches) == (lvb.PAGED_DECODE, 0, 2)
     assert p.workspace_bytes == 64 * 16 + 2 * 148 * 16 * 130 * 4
     p = lvb.attention_paged_plan(8, 64, 8, 8, 1, 64, 256, prefix_len=16384)
-    assert (p.kernel, p.prefix_splits, p.launches) == (lvb.PAGED_DECODE, 18, 3)
+    assert (p.kernel, p.prefix_splits, p.cluster, p.launches) == (lvb.PAGED_DECODE, 16, 0, 3)
+    assert lvb.attention_paged_plan(4, 32, 8, 4, 1, 16, 4, prefix_len=500).prefix_splits == 4
     # few or short sequences: clusters of CTAs, one launch, no workspace
-    for args, cluster in [((1, 32, 8, 1, 1, 16, 49), 8), ((1, 32, 8, 1, 1, 16, 100), 16),
-                          ((1, 32, 8, 1, 1, 16, 1 << 16), 16),     # one sequence, all SMs
-                          ((1, 32, 4, 1, 1, 16, 1 << 16), 0),      # it would leave half of them idle
-                          ((2, 32, 8, 2, 1, 16, 512), 8), ((2, 32, 8, 2, 1, 16, 513), 0),
+    for args, cluster in [((1, 32, 8, 1, 1, 16, 49), 7), ((1, 32, 8, 1, 1, 16, 100), 7),
+                          ((1, 32, 8, 1, 1, 16, 640), 10), ((1, 32, 8, 1, 1, 16, 641), 0),
+                          ((1, 32, 8, 1, 1, 16, 1), 1), ((2, 32, 8, 2, 1, 16, 512), 0),
                           ((8, 32, 8, 8, 1, 16, 64), 2), ((16, 32, 8, 16, 1, 16, 64), 1),
                           ((32, 32, 8, 32, 1, 16, 64), 0)]:
         p = lvb.attention_paged_plan(*args)
@@ -272,11 +272,11 @@ def test_plans(lvb):
     assert lvb.attention_paged_plan(8, 64, 8, 32, 4, 64, 256).kernel == lvb.PAGED_DECODE    # 32 rows
     assert lvb.attention_paged_plan(8, 64, 8, 40, 5, 64, 256).kernel == lvb.PAGED_FLASH     # 40 rows
     p = lvb.attention_paged_plan(1, 32, 8, 64, 64, 64, 1000)
-    assert (p.kernel, p.splits, p.launches) == (lvb.PAGED_FLASH, 18, 2)
+    assert (p.kernel, p.splits, p.cluster, p.launches) == (lvb.PAGED_FLASH, 18, 2, 2)
     p = lvb.attention_paged_plan(1, 32, 8, 64, 64, 64, 4)             # two blocks of keys
-    assert (p.splits, p.launches) == (2, 2)
+    assert (p.splits, p.cluster, p.launches) == (2, 2, 1)
     p = lvb.attention_paged_plan(1, 32, 8, 64, 64, 64, 2)             # one: no split
-    assert (p.splits, p.launches) == (1, 1)
+    assert (p.splits, p.cluster, p.launches) == (1, 0, 1)
     p = lvb.attention_paged_plan(16, 32, 8, 16384, 2048, 64, 1000, prefix_len=500)
     assert (p.kernel, p.splits, p.prefix_splits, p.launches) == (lvb.PAGED_FLASH, 1, 0, 1)
     assert lvb.attention_paged_plan(0, 32, 8, 0, 1, 64, 4).launches == 0
