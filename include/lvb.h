@@ -489,7 +489,7 @@ int lvb_kv_append(const lvb_append_desc* d, void* Kc, void* Vc, const void* K, c
  * whose products include its block, also where the causal mask gives it the weight 0. */
 typedef enum lvb_paged_kernel {
   LVB_PAGED_FLASH = 0,    /* 128-row tiles of (position, head of the group) rows */
-  LVB_PAGED_DECODE = 1    /* group·max_q <= 32: the cache streamed once, its key blocks dealt
+  LVB_PAGED_DECODE = 1    /* group·max_q <= 16: the cache streamed once, its key blocks dealt
                              evenly to the SMs whatever the lengths, or (few or short sequences:
                              `cluster`) an item's blocks to the CTAs of a cluster */
 } lvb_paged_kernel;

@@ -148,8 +148,11 @@ int check_lists(const char* op, const lvb_paged_desc* d, const int32_t* table,
   return LVB_OK;
 }
 
+// The decoding kernel's products hold 16 rows. (More rows in wider products, with twice the softmax
+// per key, took 125 us at 24 rows over 8·8 times 16,384 keys, the flash kernel 106; 28 and 21 over
+// 1,000 keys, 15.8 and 10.6 over 300; at 16 rows 97 and 103, 16.3 and 20.1, 9.6 and 10.7.)
 bool use_decode(const lvb_paged_desc* d) {
-  return (d->heads_q / d->heads_kv) * d->max_q <= 32;
+  return (d->heads_q / d->heads_kv) * d->max_q <= 16;
 }
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
@@ -210,16 +213,11 @@ int device_room(DeviceState* dev, PagedRoom* out, const char* op) {
   return LVB_OK;
 }
 
-FlashSplit flash_split(const lvb_paged_plan& pl) {
-  if (pl.kernel == LVB_PAGED_FLASH) return FlashSplit{pl.splits, std::max(1, pl.cluster)};
-  return FlashSplit{pl.prefix_splits, 1};
-}
-
-// Workspace of a planned call: the flash kernel's, then the decoding kernel's.
-size_t flash_bytes(const lvb_paged_desc* d, const lvb_paged_plan& pl) {
-  if (pl.kernel == LVB_PAGED_FLASH)
-    return up256(paged_flash_workspace(d, flash_split(pl), kFlashOwn | (d->prefix_len ? kFlashPrefix : 0)));
-  return pl.prefix_splits ? up256(paged_flash_workspace(d, flash_split(pl), kFlashPrefix)) : 0;
+// Workspace of a planned call: the flash kernel's over the prefix, then what the sequences' own
+// keys need.
+size_t prefix_bytes(const lvb_paged_desc* d, const lvb_paged_plan& pl) {
+  if (!pl.prefix_splits) return 0;
+  return up256(paged_flash_workspace(d, FlashSplit{pl.prefix_splits, 1}, kFlashPrefix, true));
 }
 
 int plan_paged(const lvb_paged_desc* d, const PagedRoom& room, lvb_paged_plan* out) {
@@ -227,29 +225,33 @@ int plan_paged(const lvb_paged_desc* d, const PagedRoom& room, lvb_paged_plan* o
   std::memset(out, 0, sizeof *out);
   out->splits = 1;
   if (d->batch == 0 || d->tokens == 0 || d->max_q == 0 || d->heads_q == 0) return LVB_OK;
-  if (use_decode(d)) {
-    out->kernel = LVB_PAGED_DECODE;
-    out->launches = 2;
-    if (d->prefix_len) {
-      out->prefix_splits = paged_flash_split(d, room, kFlashPrefix).splits;
-      out->launches = 3;
-    } else if ((out->cluster = paged_decode_cluster(d, room)) > 0) {
+  const bool decode = use_decode(d);
+  out->kernel = decode ? LVB_PAGED_DECODE : LVB_PAGED_FLASH;
+  if (paged_flash_items(d, kFlashOwn) > INT32_MAX - 65536)
+    return fail(LVB_ERR_UNSUPPORTED, op, "more than 2^31 query tiles", "split the batch");
+  if (d->prefix_len && (decode || paged_flash_gathers(d, room)))
+    out->prefix_splits = paged_flash_split(d, room, kFlashPrefix, true).splits;
+  const bool joined = out->prefix_splits > 0;
+  if (decode) {
+    if (!joined && (out->cluster = paged_decode_cluster(d, room)) > 0) {
       out->launches = 1;      // no parts in memory
       return LVB_OK;
     }
-    out->workspace_bytes = (int64_t)(flash_bytes(d, *out) +
-                                     paged_decode_workspace(d, room.sms, d->prefix_len > 0));
+    // (rows of the join, counted in 32 bits)
+    if ((double)d->batch * (double)d->max_q * (double)d->heads_q > (double)(INT32_MAX / 4))
+      return fail(LVB_ERR_UNSUPPORTED, op, "more than 2^29 query rows", "split the batch");
+    out->launches = joined ? 3 : 2;
+    out->workspace_bytes =
+        (int64_t)(prefix_bytes(d, *out) + paged_decode_workspace(d, room.sms, joined));
     return LVB_OK;
   }
-  out->kernel = LVB_PAGED_FLASH;
-  const int parts = kFlashOwn | (d->prefix_len ? kFlashPrefix : 0);
-  if (paged_flash_items(d, parts) > INT32_MAX - 65536)
-    return fail(LVB_ERR_UNSUPPORTED, op, "more than 2^31 query tiles", "split the batch");
-  const FlashSplit fs = paged_flash_split(d, room, parts);
+  const int parts = kFlashOwn | (d->prefix_len && !joined ? kFlashPrefix : 0);
+  const FlashSplit fs = paged_flash_split(d, room, parts, joined);
   out->splits = fs.splits;
   out->cluster = fs.cluster > 1 ? fs.cluster : 0;
-  out->launches = fs.splits > fs.cluster ? 2 : 1;
-  out->workspace_bytes = (int64_t)flash_bytes(d, *out);
+  out->launches = joined ? 3 : fs.splits > fs.cluster ? 2 : 1;
+  out->workspace_bytes =
+      (int64_t)(prefix_bytes(d, *out) + paged_flash_workspace(d, fs, parts, joined));
   return LVB_OK;
 }
 
@@ -425,43 +427,59 @@ int lvb_attention_paged(const lvb_paged_desc* d, const void* Q, const void* Kc, 
   }
   cudaError_t e = workspace_alloc(dev, reinterpret_cast<void**>(&ws), (size_t)pl.workspace_bytes, s);
   if (e != cudaSuccess) return fail_cuda(e, op, "workspace allocation");
-  FlashWorkspace fw = {};
   const bool bf16 = d->dtype == LVB_BF16;
-  const size_t fb = flash_bytes(d, pl);
+  const bool joined = pl.prefix_splits > 0;
+  uint8_t* own_ws = ws + prefix_bytes(d, pl);
+  // (before the prefix's kernel, so that nothing stands between it and the one behind it)
+  if (pl.kernel == LVB_PAGED_FLASH && pl.cluster == 0) {
+    e = cudaMemsetAsync(own_ws, 0, sizeof(int), s);
+    if (e != cudaSuccess) st = fail_cuda(e, op, "work counter reset");
+  }
+  FlashWorkspace fw = {};
+  if (joined && st == LVB_OK) {
+    st = paged_flash_launch(d, lay, mp.seqs, Q, Kc, Vc, O, lse, kFlashPrefix, true,
+                            FlashSplit{pl.prefix_splits, 1}, ws, &fw, s, dev);
+    mp.tile_o = fw.tile_o;
+    mp.tile_ml = fw.tile_ml;
+    mp.tile_splits = pl.prefix_splits;
+  }
+  int pieces = mp.tile_splits;      // parts of a row, about
   if (pl.kernel == LVB_PAGED_DECODE) {
-    if (pl.prefix_splits) {
-      st = paged_flash_launch(d, lay, mp.seqs, Q, Kc, Vc, O, lse, kFlashPrefix, flash_split(pl), ws,
-                              &fw, s, dev);
-      mp.tile_o = fw.tile_o;
-      mp.tile_ml = fw.tile_ml;
-      mp.tile_splits = pl.prefix_splits;
-    }
     DecodeWorkspace dw = {};
     if (st == LVB_OK)
-      st = paged_decode_launch(d, lay, mp.seqs, Q, Kc, Vc, O, lse, pl.prefix_splits > 0,
-                               pl.prefix_splits > 0, 0, ws + fb, &dw, s, dev);
-    mp.dec_o = dw.part_o;
-    mp.dec_ml = dw.part_ml;
+      st = paged_decode_launch(d, lay, mp.seqs, Q, Kc, Vc, O, lse, joined, joined, 0, own_ws, &dw, s,
+                               dev);
+    mp.own_o = dw.part_o;
+    mp.own_ml = dw.part_ml;
     mp.dec_tab = dw.tab;
     mp.dec_rows = dw.rows;
     mp.dec_slots = dw.slots;
     mp.dec_ctas = dw.ctas;
     // about as many pieces per item as there are CTAs for each, and one more
-    const int pieces = dw.ctas / (int)(d->batch * d->heads_kv) + 2 + mp.tile_splits;
-    mp.warps_per_row = pieces <= 8 ? 1 : pieces <= 16 ? 2 : 4;
-    if (st == LVB_OK) st = merge_launch(mp, (int)d->head_dim, bf16, s, dev);
+    pieces += dw.ctas / (int)(d->batch * d->heads_kv) + 2;
   } else {
-    const int parts = kFlashOwn | (d->prefix_len ? kFlashPrefix : 0);
-    st = paged_flash_launch(d, lay, mp.seqs, Q, Kc, Vc, O, lse, parts, flash_split(pl), ws, &fw, s, dev);
-    const int groups = pl.splits / std::max(1, pl.cluster);
-    if (st == LVB_OK && groups > 1) {
+    const int parts = kFlashOwn | (d->prefix_len && !joined ? kFlashPrefix : 0);
+    const FlashSplit fs{pl.splits, std::max(1, pl.cluster)};
+    if (st == LVB_OK)
+      st = paged_flash_launch(d, lay, mp.seqs, Q, Kc, Vc, O, lse, parts, joined, fs, own_ws, &fw, s, dev);
+    const int groups = fs.splits / fs.cluster;
+    const int pairs = (int)((d->max_q + 2 * mp.ppt - 1) / (2 * mp.ppt));
+    if (joined) {
+      mp.own_o = fw.tile_o;
+      mp.own_ml = fw.tile_ml;
+      mp.own_splits = groups;
+      mp.own_pairs = pairs;
+    } else {
       mp.tile_o = fw.tile_o;
       mp.tile_ml = fw.tile_ml;
       mp.tile_splits = groups;
-      mp.warps_per_row = groups <= 8 ? 1 : groups <= 16 ? 2 : 4;
-      mp.pairs_per_seq = (int)((d->max_q + 2 * mp.ppt - 1) / (2 * mp.ppt));
-      st = merge_launch(mp, (int)d->head_dim, bf16, s, dev);
+      mp.pairs_per_seq = pairs;
     }
+    pieces += groups;
+  }
+  if (pl.kernel == LVB_PAGED_DECODE || joined || mp.tile_splits > 1) {
+    mp.warps_per_row = pieces <= 8 ? 1 : pieces <= 16 ? 2 : 4;
+    if (st == LVB_OK) st = merge_launch(mp, (int)d->head_dim, bf16, s, dev);
   }
   e = cudaFreeAsync(ws, s);
   if (st == LVB_OK && e != cudaSuccess) return fail_cuda(e, op, "workspace free");

@@ -1,10 +1,10 @@
-// attn_paged_decode_sm100.cu — attention of few query rows per KV head (group·max_q <= 32) over
+// attn_paged_decode_sm100.cu — attention of few query rows per KV head (group·max_q <= 16) over
 // the paged KV cache, B200 (sm_100a).
 //
 // O = softmax(scale·Q·Kᵀ + mask)·V with one pass over the keys: S of a 128-key block, a running
 // reference maximum m per row, p = 2^(s·log2e - m), O += P·V, l += Σp. The cache is read once at
 // HBM speed, and the products are turned so that the keys fill the tensor core's 128 rows:
-//   Sᵀ (128 keys × NR rows) = K_j·Qᵀ,   Oᵀ (D × NR) += V_jᵀ·P_jᵀ,   NR = 16 or 32 rows
+//   Sᵀ (128 keys × kRows) = K_j·Qᵀ,   Oᵀ (D × kRows) += V_jᵀ·P_jᵀ,   kRows = 16
 // (rows = position·group + head of the group). P is rounded to the cache's type for the second
 // product (the tensor core takes both operands in one 16-bit type); l sums the unrounded p.
 //
@@ -44,6 +44,7 @@ constexpr int kTmaWarp = 8;                // the items, Q and the K blocks
 constexpr int kVWarp = 9;                  // the V blocks
 constexpr int kQkWarp = 10;
 constexpr int kPvWarp = 11;
+constexpr int kRows = 16;                  // rows of the products
 constexpr int kQueue = 8;                  // items published ahead
 // Blocks that an item's start and end count for when the blocks are dealt out: the time of three
 // 128-wide blocks, six 64-wide ones (measured on ragged batches: drafts over 64-wide heads 42.6 us
@@ -62,24 +63,24 @@ struct DecParams {
   void* O;
   long long o_st, o_sh;
   float* lse;
-  float* part_o;            // [slot][NR][D]
-  float* part_ml;           // [slot][NR][2]
+  float* part_o;            // [slot][kRows][D]
+  float* part_ml;           // [slot][kRows][2]
   int4* tab;                // [batch·Hkv]
   unsigned long long timeout_ns;
 };
 
-template <int D, int NR>
+template <int D>
 struct Cfg {
   static constexpr int kCh = D / 64;
   static constexpr int kBlock = kCh * kChunk;
   static constexpr int kK = D == 64 ? 6 : 3;             // K ring slots
-  static constexpr int kV = D == 64 ? 6 : NR == 16 ? 3 : 2;   // V ring slots
+  static constexpr int kV = D == 64 ? 6 : 3;             // V ring slots
   static constexpr int kRing = kK + kV;
-  static constexpr int kQ = kCh * NR * 128;            // Q of an item
-  static constexpr int kP = 2 * NR * 128;              // P of a block: two 64-key chunks
-  static constexpr int kTmemCols = NR == 16 ? 128 : 256;   // S and two O per warpgroup
+  static constexpr int kQ = kCh * kRows * 128;            // Q of an item
+  static constexpr int kP = 2 * kRows * 128;              // P of a block: two 64-key chunks
+  static constexpr int kTmemCols = 128;               // S and two O per warpgroup
   static constexpr int kSmem =
-      kRing * kBlock + 2 * kQ + 2 * kP + 2 * 4 * NR * 4 + 3 * NR * 8 + 2048 +
+      kRing * kBlock + 2 * kQ + 2 * kP + 2 * 4 * kRows * 4 + 3 * kRows * 8 + 2048 +
       kThreads * 12 + 1024;
 };
 
@@ -104,16 +105,14 @@ __device__ __forceinline__ void ld_cols(uint32_t taddr, uint32_t (&r)[N]) {
   if constexpr (N == 1) tmem_ld1(taddr, r);
   else if constexpr (N == 4) tmem_ld4(taddr, r);
   else if constexpr (N == 8) tmem_ld8(taddr, r);
-  else if constexpr (N == 16) tmem_ld16(taddr, r);
-  else tmem_ld32(taddr, r);
+  else tmem_ld16(taddr, r);
 }
 template <int N>
 __device__ __forceinline__ void st_cols(uint32_t taddr, uint32_t (&r)[N]) {
   if constexpr (N == 1) tmem_st1(taddr, r);
   else if constexpr (N == 4) tmem_st4(taddr, r);
   else if constexpr (N == 8) tmem_st8(taddr, r);
-  else if constexpr (N == 16) tmem_st16(taddr, r);
-  else tmem_st32(taddr, r);
+  else tmem_st16(taddr, r);
 }
 
 __device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity, uint64_t timeout_ns) {
@@ -150,30 +149,30 @@ __device__ __forceinline__ int blocks_of(const SeqInfo& s) {
   return s.qlen > 0 ? (s.len + 127) >> 7 : 0;
 }
 
-// RR <= NR: the rows that the softmax works on (the smallest of 1, 4, 8, 16, 32 that holds the
+// RR <= kRows: the rows that the softmax works on (the smallest of 1, 4, 8, 16 that holds the
 // query rows); the products' other columns are computed and never read.
-template <int D, int NR, int RR, bool BF16>
+template <int D, int RR, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_decode_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                         const __grid_constant__ CUtensorMap tmV,
                         const __grid_constant__ DecParams p) {
-  using C = Cfg<D, NR>;
+  using C = Cfg<D>;
   constexpr int KR = C::kK, VR = C::kV;
   constexpr uint32_t kFmt = BF16 ? 1 : 0;
-  constexpr uint32_t kIdescQK = make_idesc(1, kFmt, kFmt, 0, 0, 128, NR);
-  constexpr uint32_t kIdescPV = make_idesc(1, kFmt, kFmt, 1, 0, 128, NR);
+  constexpr uint32_t kIdescQK = make_idesc(1, kFmt, kFmt, 0, 0, 128, kRows);
+  constexpr uint32_t kIdescPV = make_idesc(1, kFmt, kFmt, 1, 0, 128, kRows);
   constexpr float kShift = BF16 ? 0.f : 6.f;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align_1024(smem_raw);
   uint8_t* sRing = smem;                                  // [KR + VR][D/64 chunks][128 keys][128 B]
-  uint8_t* sQ = sRing + C::kRing * C::kBlock;                    // [2][D/64 chunks][NR rows][128 B]
-  uint8_t* sP = sQ + 2 * C::kQ;                           // [2][2 chunks][NR rows][128 B]
-  float* sXml = reinterpret_cast<float*>(sP + 2 * C::kP); // [2 warpgroups][NR][2] deposited m, l
-  float* sJml = sXml + 2 * NR * 2;                        // [NR][2] this CTA's part's m and l
-  float* sRed = sJml + NR * 2;                            // [2 warpgroups][4 warps][NR]
-  float* sJ = reinterpret_cast<float*>(sRing);            // [NR][D] its O, when the ring is done with
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sRed + 2 * 4 * NR);
+  uint8_t* sQ = sRing + C::kRing * C::kBlock;                    // [2][D/64 chunks][kRows rows][128 B]
+  uint8_t* sP = sQ + 2 * C::kQ;                           // [2][2 chunks][kRows rows][128 B]
+  float* sXml = reinterpret_cast<float*>(sP + 2 * C::kP); // [2 warpgroups][kRows][2] deposited m, l
+  float* sJml = sXml + 2 * kRows * 2;                        // [kRows][2] this CTA's part's m and l
+  float* sRed = sJml + kRows * 2;                            // [2 warpgroups][4 warps][kRows]
+  float* sJ = reinterpret_cast<float*>(sRing);            // [kRows][D] its O, when the ring is done with
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sRed + 2 * 4 * kRows);
   uint64_t* k_full = bars;               // [KR]
   uint64_t* k_empty = k_full + KR;       // [KR]
   uint64_t* v_full = k_empty + KR;       // [VR]
@@ -288,7 +287,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int u0 = min((int)blockIdx.x, total / share + 1) * share;   // (no product above 2·total + share)
   const int u1 = min(u0 + share, total);
   const int first = before + incl - mine;
-  if (p.cluster && threadIdx.x < NR) {
+  if (p.cluster && threadIdx.x < kRows) {
     sJml[2 * threadIdx.x] = 0.f;
     sJml[2 * threadIdx.x + 1] = 0.f;       // no part yet
   }
@@ -308,13 +307,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // columns: S of warpgroup w at w·NR, its O buffers at (2 + 2w + ob)·NR
+  // columns: S of warpgroup w at w·kRows, its O buffers at (2 + 2w + ob)·kRows
   const WaitGuard g{p.seqs.status, abort_flag, p.timeout_ns};
 
   auto load_q = [&](int qb, int hk, int tok0) {
     bar_arrive_expect_tx(&q_full[qb], C::kCh * p.nrows * 128);
     for (int c = 0; c < C::kCh; ++c)
-      tma_load_3d(sQ + qb * C::kQ + c * NR * 128, &tmQ, c * 64, hk * p.group, tok0, &q_full[qb]);
+      tma_load_3d(sQ + qb * C::kQ + c * kRows * 128, &tmQ, c * 64, hk * p.group, tok0, &q_full[qb]);
   };
 
   if (warp == kTmaWarp) {
@@ -540,8 +539,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint64_t bd = q_desc + (uint64_t)((qb * C::kQ) >> 4);
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk)
-              mma_f16_ss(tmem + NR * w, ad + (((kk >> 2) * kChunk + (kk & 3) * 32) >> 4),
-                         bd + (((kk >> 2) * NR * 128 + (kk & 3) * 32) >> 4), kIdescQK, kk > 0 ? 1u : 0u);
+              mma_f16_ss(tmem + kRows * w, ad + (((kk >> 2) * kChunk + (kk & 3) * 32) >> 4),
+                         bd + (((kk >> 2) * kRows * 128 + (kk & 3) * 32) >> 4), kIdescQK, kk > 0 ? 1u : 0u);
             mma_commit(&s_full[w]);
             mma_commit(&k_empty[sk]);                    // K_j read
             if (j == nb - 1) mma_commit(&q_empty[qb]);   // the item's Q read for the last time
@@ -565,8 +564,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint64_t bd = p_desc + (uint64_t)((w * C::kP) >> 4);
 #pragma unroll
             for (int kk = 0; kk < 8; ++kk)   // 16 keys per MMA
-              mma_f16_ss(tmem + NR * (2 + 2 * w + ob), ad + ((kk * 16 * 128) >> 4),
-                         bd + (((kk >> 2) * NR * 128 + (kk & 3) * 32) >> 4), kIdescPV,
+              mma_f16_ss(tmem + kRows * (2 + 2 * w + ob), ad + ((kk * 16 * 128) >> 4),
+                         bd + (((kk >> 2) * kRows * 128 + (kk & 3) * 32) >> 4), kIdescPV,
                          (j < 2 && kk == 0) ? 0u : 1u);
             mma_commit(&p_empty[w]);
             mma_commit(&v_empty[sv]);                    // V_j read
@@ -588,10 +587,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int t = threadIdx.x & 127;                    // key within the block / Oᵀ lane (d)
     const int wl = warp & 3;
     const uint32_t lane_off = (uint32_t)(wl * 32) << 16;
-    const uint32_t tS = tmem + lane_off + NR * w;
+    const uint32_t tS = tmem + lane_off + kRows * w;
     const int bar_id = 1 + w;
-    float* red = sRed + w * 4 * NR;
-    uint8_t* pt = sP + w * C::kP + (t >> 6) * NR * 128 + (t & 7) * 2;   // Pᵀ: this key's column
+    float* red = sRed + w * 4 * kRows;
+    uint8_t* pt = sP + w * C::kP + (t >> 6) * kRows * 128 + (t & 7) * 2;   // Pᵀ: this key's column
     const float NEG_INF = -INFINITY;
     const float sl = p.scale_log2;
 
@@ -614,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
 
-    // r / group by a product: exact for r < 32 and group <= 32
+    // r / group by a product: exact for r < 16 and group <= 16
     const uint32_t inv_group = 65536u / (uint32_t)p.group + 1u;
     auto row_pos = [&](int r) -> int { return (int)((uint32_t)r * inv_group >> 16); };
     int gb = 0;       // blocks before this item
@@ -646,7 +645,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int n_rows = min(p.nrows, qlen * p.group);   // rows r < n_rows are real
       // Row r = position·group + head of the group sees keys up to lim0 + position.
       const int lim0 = p.causal ? len - qlen : len - 1;
-      const uint32_t tO = tmem + lane_off + NR * (2 + 2 * w + (wi & 1));
+      const uint32_t tO = tmem + lane_off + kRows * (2 + 2 * w + (wi & 1));
       float m_ref[RR], l_part[RR];
 #pragma unroll
       for (int r = 0; r < RR; ++r) {
@@ -690,14 +689,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             float v = x[r];
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-            if (lane == 0) red[wl * NR + r] = v;
+            if (lane == 0) red[wl * kRows + r] = v;
           }
           named_barrier_sync(bar_id, 128);
           bool resc = false;
           float alpha[RR];
 #pragma unroll
           for (int r = 0; r < RR; ++r) {
-            const float bm = fmaxf(fmaxf(red[r], red[NR + r]), fmaxf(red[2 * NR + r], red[3 * NR + r]));
+            const float bm = fmaxf(fmaxf(red[r], red[kRows + r]), fmaxf(red[2 * kRows + r], red[3 * kRows + r]));
             alpha[r] = 1.f;
             if (bm > m_ref[r] + kLazy) {
               if (m_ref[r] != NEG_INF) {
@@ -747,7 +746,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         float v = l_part[r];
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-        if (lane == 0) red[wl * NR + r] = v;
+        if (lane == 0) red[wl * kRows + r] = v;
       }
       if (depositor == w) {
         if (!wait_bar(&x_empty[w], (uint32_t)(x_before & 1) ^ 1, g, 65, it)) ok = false;
@@ -755,8 +754,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int r = 0; r < RR; ++r)
           if (t == r) {
-            sXml[(w * NR + r) * 2] = m_ref[r];
-            sXml[(w * NR + r) * 2 + 1] = (red[r] + red[NR + r]) + (red[2 * NR + r] + red[3 * NR + r]);
+            sXml[(w * kRows + r) * 2] = m_ref[r];
+            sXml[(w * kRows + r) * 2 + 1] = (red[r] + red[kRows + r]) + (red[2 * kRows + r] + red[3 * kRows + r]);
           }
         __syncwarp();
         if (lane == 0) bar_arrive(&x_full[w]);
@@ -774,17 +773,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         float l[RR], m[RR];
 #pragma unroll
         for (int r = 0; r < RR; ++r) {
-          l[r] = (red[r] + red[NR + r]) + (red[2 * NR + r] + red[3 * NR + r]);
+          l[r] = (red[r] + red[kRows + r]) + (red[2 * kRows + r] + red[3 * kRows + r]);
           m[r] = fmaxf(m_ref[r], -3.0e38f);      // finite: 2^(m - m') is 0 or 1, not NaN
         }
         if (both) {
           // the two warpgroups' sums over the larger of their references
           uint32_t o2[RR];
-          ld_cols<RR>(tmem + lane_off + NR * (2 + 2 * ww + (wo & 1)), o2);
+          ld_cols<RR>(tmem + lane_off + kRows * (2 + 2 * ww + (wo & 1)), o2);
           tmem_wait_ld();
 #pragma unroll
           for (int r = 0; r < RR; ++r) {
-            const float2 x2 = *reinterpret_cast<const float2*>(&sXml[(ww * NR + r) * 2]);
+            const float2 x2 = *reinterpret_cast<const float2*>(&sXml[(ww * kRows + r) * 2]);
             const float m2 = fmaxf(x2.x, -3.0e38f);
             const float mm = fmaxf(m[r], m2);
             const float a1 = fast_exp2(m[r] - mm), a2 = fast_exp2(m2 - mm);
@@ -830,7 +829,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         } else {
-          const long long at = (long long)slot * NR;
+          const long long at = (long long)slot * kRows;
 #pragma unroll
           for (int r = 0; r < RR; ++r) {
             if (r < n_rows && t < D) p.part_o[(at + r) * D + t] = __uint_as_float(o[r]);
@@ -851,7 +850,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // A part without a key has l = 0, and its O is not read.
     __syncthreads();
     const bool bad = *abort_flag != 0;
-    if (bad && threadIdx.x < NR) sJml[2 * threadIdx.x + 1] = -1.f;   // after a wait gave up: store nothing
+    if (bad && threadIdx.x < kRows) sJml[2 * threadIdx.x + 1] = -1.f;   // after a wait gave up: store nothing
     cluster_sync_all();
     const int rank = blockIdx.x - c_id * p.cluster, hk = c_id - c_b * p.Hkv;
     const int tok0 = sStart[0], n_rows = min(p.nrows, sStart[1] * p.group);
@@ -925,26 +924,21 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <int D, int NR, int RR, bool BF16>
+template <int D, int RR, bool BF16>
 int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const DecParams& p,
            int ctas, cudaStream_t stream, DeviceState* dev) {
   static SmemAttr attr;
-  return launch_cluster("lvb_attention_paged", paged_decode_kernel<D, NR, RR, BF16>, attr, dev, ctas,
-                        kThreads, Cfg<D, NR>::kSmem, std::max(1, p.cluster), stream, tq, tk, tv, p);
+  return launch_cluster("lvb_attention_paged", paged_decode_kernel<D, RR, BF16>, attr, dev, ctas,
+                        kThreads, Cfg<D>::kSmem, std::max(1, p.cluster), stream, tq, tk, tv, p);
 }
 
 template <int D, bool BF16>
 int launch_rows(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                 const DecParams& p, int ctas, cudaStream_t stream, DeviceState* dev) {
-  if (p.nrows == 1) return launch<D, 16, 1, BF16>(tq, tk, tv, p, ctas, stream, dev);
-  if (p.nrows <= 4) return launch<D, 16, 4, BF16>(tq, tk, tv, p, ctas, stream, dev);
-  if (p.nrows <= 8) return launch<D, 16, 8, BF16>(tq, tk, tv, p, ctas, stream, dev);
-  if (p.nrows <= 16) return launch<D, 16, 16, BF16>(tq, tk, tv, p, ctas, stream, dev);
-  return launch<D, 32, 32, BF16>(tq, tk, tv, p, ctas, stream, dev);
-}
-
-int product_rows(const lvb_paged_desc* d) {
-  return (d->heads_q / d->heads_kv) * d->max_q <= 16 ? 16 : 32;
+  if (p.nrows == 1) return launch<D, 1, BF16>(tq, tk, tv, p, ctas, stream, dev);
+  if (p.nrows <= 4) return launch<D, 4, BF16>(tq, tk, tv, p, ctas, stream, dev);
+  if (p.nrows <= 8) return launch<D, 8, BF16>(tq, tk, tv, p, ctas, stream, dev);
+  return launch<D, 16, BF16>(tq, tk, tv, p, ctas, stream, dev);
 }
 
 // One CTA per SM; fewer when even full tables would not give every CTA a block.
@@ -974,7 +968,7 @@ int paged_decode_cluster(const lvb_paged_desc* d, const PagedRoom& room) {
 
 size_t paged_decode_workspace(const lvb_paged_desc* d, int sm_count, bool keep_parts) {
   return (size_t)(d->batch * d->heads_kv) * sizeof(int4) +
-         decode_slots(d, sm_count, keep_parts) * product_rows(d) * (d->head_dim + 2) * sizeof(float);
+         decode_slots(d, sm_count, keep_parts) * kRows * (d->head_dim + 2) * sizeof(float);
 }
 
 int paged_decode_launch(const lvb_paged_desc* d, const PagedLayout& lay, const PagedSeqs& seqs,
@@ -999,15 +993,14 @@ int paged_decode_launch(const lvb_paged_desc* d, const PagedLayout& lay, const P
   p.o_sh = lay.o[1];
   p.lse = lse;
   p.timeout_ns = wait_timeout_ns();
-  const int rows = product_rows(d);
   int ctas = (int)(d->batch * d->heads_kv) * cluster;
   if (!cluster) {
     const size_t slots = decode_slots(d, dev->sm_count, keep_parts);
     p.tab = reinterpret_cast<int4*>(ws);
     p.part_o = reinterpret_cast<float*>(p.tab + d->batch * d->heads_kv);
-    p.part_ml = p.part_o + slots * rows * d->head_dim;
+    p.part_ml = p.part_o + slots * kRows * d->head_dim;
     ctas = decode_ctas(d, dev->sm_count);
-    *out = DecodeWorkspace{p.part_o, p.part_ml, p.tab, rows, (int)slots, ctas};
+    *out = DecodeWorkspace{p.part_o, p.part_ml, p.tab, kRows, (int)slots, ctas};
   }
   CUtensorMap tq, tk, tv;
   {

@@ -42,6 +42,7 @@ struct FlashParams {
   int splits, pairs_per_seq;   // pairs_per_seq: rows of the parts' index per sequence
   int store_parts;
   int cluster;                 // CTAs per cluster (of a pair's splits), one item per CTA; 0: none
+  int late_wait;               // 1: runs beside the kernel before it (see the kernel's start)
   int* counter;                // items are taken from it; NULL: item blockIdx.x, + gridDim.x, ...
   float scale_log2;
   void* O;
@@ -182,7 +183,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       asm volatile("prefetch.global.L2 [%0];" ::"l"(p.seqs.prefix_table + i));
   // The setup above may run while the stream's previous kernel ends; what reads this kernel's
   // results after its own wait may be scheduled from here on.
-  griddep_wait();
+  // Behind the same call's kernel over the prefix it starts at once: that one has waited for the
+  // stream's earlier work before it let this one start, and shares nothing with it but inputs and
+  // disjoint workspace; it waits before it ends, so that its end is also that kernel's.
+  if (!p.late_wait) griddep_wait();
   griddep_launch_dependents();
   const int npb = (p.prefix + 127) / 128;
   float part_m = -INFINITY, part_l = 0.f;      // a softmax thread's row of its CTA's part (clusters)
@@ -801,6 +805,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+  if (p.late_wait) griddep_wait();
 }
 
 // ----------------------------------------------------------------------------------------
@@ -845,8 +850,15 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const MergeParams 
     const int t = in_pair / p.ppt;
     tile0 = (pair * p.Hkv + hk) * nt * 256 + t * 128 + (in_pair - t * p.ppt) * p.group + gh;
   }
+  long long own0 = 0;
+  if (p.own_splits) {
+    const int in_pair = pos % (2 * p.ppt);
+    const long long pair = pos / (2 * p.ppt) + (long long)b * p.own_pairs;
+    const int t = in_pair / p.ppt;
+    own0 = (pair * p.Hkv + hk) * p.own_splits * 256 + t * 128 + (in_pair - t * p.ppt) * p.group + gh;
+  }
   griddep_wait();
-  int nd = 0, first_slot = 0, next_c = 0;
+  int nd = p.own_splits, first_slot = 0, next_c = 0;
   if (p.dec_tab && on) {
     const int4 e = p.dec_tab[b * p.Hkv + hk];
     if (e.w == kItemPieces && e.x >= 0 && e.x < p.dec_slots && e.y > 0 && e.z < p.dec_ctas) {
@@ -873,9 +885,10 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const MergeParams 
       const int i = min(i0 + q, n - 1), k = i - nt;
       const bool tile = k < 0;
       const long long slot = k <= 0 ? first_slot : 2 * (next_c + k - 1);
-      const long long r = tile ? tile0 + (long long)i * 256 : slot * p.dec_rows + dec_row;
-      ml[q] = *reinterpret_cast<const float2*>((tile ? p.tile_ml : p.dec_ml) + 2 * r);
-      const float* src = (tile ? p.tile_o : p.dec_o) + r * D + lane * V;
+      const long long r = tile ? tile0 + (long long)i * 256
+                          : p.own_splits ? own0 + (long long)k * 256 : slot * p.dec_rows + dec_row;
+      ml[q] = *reinterpret_cast<const float2*>((tile ? p.tile_ml : p.own_ml) + 2 * r);
+      const float* src = (tile ? p.tile_o : p.own_o) + r * D + lane * V;
       if constexpr (V == 4) {
         const float4 f = *reinterpret_cast<const float4*>(src);
         v[q][0] = f.x, v[q][1] = f.y, v[q][2] = f.z, v[q][3] = f.w;
@@ -944,6 +957,10 @@ int launch_flash(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap
 
 constexpr size_t kCounterBytes = 256;   // the item counter, before the 32-byte stores' parts
 
+constexpr double kBlockUs = 1.8;        // a key block of a tile pair
+constexpr double kJoinUs = 4.0;         // the join kernel
+constexpr double kPassUs = 16.0;        // a prefix's own pass: two more starts and ends
+
 int positions_per_tile(const lvb_paged_desc* d) {
   return (int)(128 / (d->heads_q / d->heads_kv));
 }
@@ -964,47 +981,62 @@ int64_t paged_flash_items(const lvb_paged_desc* d, int parts) {
 
 // With fewer items than SMs: key ranges (of the prefix's length; of a table's row otherwise), by the
 // cost of a CTA's blocks (1.8 us each) and of a part that goes through memory (0.45 us with its
-// share of the join; of a prefix's, that are joined while more is going on, a tenth: 4,099 keys over
-// 64-wide heads in 16 ranges 31.0 us, in 11 34.5). The sequences' own ranges meet in clusters where that spares the join kernel
-// or most of its work (a cluster's join 1.5 us, the kernel 4 us): 64 new tokens of one sequence over
-// 1,000, 4,000 and 16,000 keys 14.8, 20.3 and 35.4 us with clusters, 21.6, 26.9 and 38.9 without. A
-// prefix's do not: the decoding kernel fills the SMs as its CTAs end, and the join kernel runs
-// anyway (16,384 keys before 64 sequences 87.2 us with clusters, 84.9 without).
-FlashSplit paged_flash_split(const lvb_paged_desc* d, const PagedRoom& room, int parts) {
+// share of the join). Ranges meet in clusters where that spares the join kernel or most of its work
+// (a cluster's join 1.5 us, the kernel 4 us): 64 new tokens of one sequence over 1,000, 4,000 and
+// 16,000 keys 14.8, 20.3 and 35.4 us with clusters, 21.6, 26.9 and 38.9 without. Parts that are
+// joined anyway (a prefix's and those beside it) do not: the kernel behind it fills the SMs as the
+// CTAs end (16,384 keys before 64 sequences 87.2 us with clusters, 84.9 without), and cost a tenth
+// in the join, as more is going on (4,099 keys over 64-wide heads in 16 ranges 31.0 us, in 11 34.5).
+FlashSplit paged_flash_split(const lvb_paged_desc* d, const PagedRoom& room, int parts, bool joined) {
   const int64_t items = std::max<int64_t>(1, paged_flash_items(d, parts));
   int64_t keys = 0;
   if (parts & kFlashPrefix) keys += d->prefix_len;
   if (parts & kFlashOwn) keys += d->table_width * d->page_size;
   const int64_t blocks = std::max<int64_t>(1, (keys + 127) / 128);
-  FlashSplit best{1, 1};
+  FlashSplit best{1, 1, kBlockUs * (double)blocks * (double)((items + room.sms - 1) / room.sms)};
   if (2 * items > room.sms) return best;
-  double least = 1e30;
-  for (int c = 1; c <= (parts == kFlashPrefix ? 1 : kMostCluster); ++c) {
+  best.us = 1e30;
+  for (int c = 1; c <= (joined ? 1 : kMostCluster); ++c) {
     const int64_t most = (c == 1 ? room.sms : room.clusters[c]) / items;   // groups that run at once
     for (int64_t g = 1; g <= most && g * c <= blocks; ++g) {
-      const double cost = 1.8 * (double)((blocks + g * c - 1) / (g * c)) +
-                          (parts == kFlashPrefix ? 0.05 : 0.45) * (double)g +
-                          (c > 1 ? 1.5 : 0.0) + (parts != kFlashPrefix && g > 1 ? 4.0 : 0.0);
-      if (cost < least - 1e-9) {
-        least = cost;
-        best = FlashSplit{(int)(g * c), c};
-      }
+      const double cost = kBlockUs * (double)((blocks + g * c - 1) / (g * c)) +
+                          (joined ? 0.05 : 0.45) * (double)g + (c > 1 ? 1.5 : 0.0) +
+                          (!joined && g > 1 ? kJoinUs : 0.0);
+      if (cost < best.us - 1e-9) best = FlashSplit{(int)(g * c), c, cost};
     }
   }
   return best;
 }
 
-size_t paged_flash_workspace(const lvb_paged_desc* d, FlashSplit fs, int parts) {
+// Whether the prefix is read in a pass of its own, whose tiles hold the rows of all sequences, and
+// joined with the sequences' own parts, or by every sequence's tiles in front of its own keys.
+// The first has fewer tiles where a sequence's rows do not fill one, but its parts go through
+// memory (twice a row's D fp32, written and read) and into a join, and each pass has its start: of
+// 32 sequences with 4 tokens, 64 heads on 8, and 300 own keys behind 16,384 the first takes 94.1 us,
+// the second 372.8; of 16 with 8, 32 and 64 tokens, 32 heads on 8, 100 keys behind 4,096 the first
+// 45.3, 67.9 and 70.4, the second 61.0, 61.6 and 70.0.
+bool paged_flash_gathers(const lvb_paged_desc* d, const PagedRoom& room) {
+  if (d->prefix_len == 0) return false;
+  const FlashSplit pre = paged_flash_split(d, room, kFlashPrefix, true);
+  const FlashSplit own = paged_flash_split(d, room, kFlashOwn, true);
+  const double rows = (double)d->batch * (double)d->max_q * (double)d->heads_q;   // of the join
+  if (rows > (double)(1 << 24)) return false;
+  const double parts_us = rows * (double)(pre.splits + own.splits) * (double)(d->head_dim + 2) * 8.0 / 5e6;
+  return pre.us + own.us + parts_us + kJoinUs + kPassUs <
+         paged_flash_split(d, room, kFlashOwn | kFlashPrefix, false).us;
+}
+
+size_t paged_flash_workspace(const lvb_paged_desc* d, FlashSplit fs, int parts, bool joined) {
   const int groups = fs.splits / fs.cluster;
-  const bool store = parts == kFlashPrefix || groups > 1;
+  const bool store = joined || groups > 1;
   return kCounterBytes + (store ? (size_t)paged_flash_items(d, parts) * groups * 256 *
                                       (d->head_dim + 2) * sizeof(float) : 0);
 }
 
 int paged_flash_launch(const lvb_paged_desc* d, const PagedLayout& lay, const PagedSeqs& seqs,
                        const void* Q, const void* Kc, const void* Vc, void* O, float* lse, int parts,
-                       FlashSplit fs, void* ws, FlashWorkspace* out, cudaStream_t stream,
-                       DeviceState* dev) {
+                       bool joined, FlashSplit fs, void* ws, FlashWorkspace* out,
+                       cudaStream_t stream, DeviceState* dev) {
   const char* op = "lvb_attention_paged";
   FlashParams p = {};
   p.seqs = seqs;
@@ -1020,7 +1052,8 @@ int paged_flash_launch(const lvb_paged_desc* d, const PagedLayout& lay, const Pa
   p.splits = fs.splits;
   p.pairs_per_seq = (int)tile_pairs(d, parts);
   p.cluster = fs.cluster > 1 ? fs.cluster : 0;
-  p.store_parts = p.all_rows || fs.splits > fs.cluster ? 1 : 0;
+  p.late_wait = joined && !p.all_rows ? 1 : 0;
+  p.store_parts = joined || fs.splits > fs.cluster ? 1 : 0;
   p.scale_log2 = d->scale * 1.4426950408889634f;
   p.O = O;
   p.o_st = lay.o[0];
@@ -1043,13 +1076,9 @@ int paged_flash_launch(const lvb_paged_desc* d, const PagedLayout& lay, const Pa
   int st = paged_kv_maps(&tk, &tv, d, lay, Kc, Vc, op);
   if (st) return st;
   const int ctas = p.cluster ? (int)items : (int)std::min<int64_t>(items, std::max(1, dev->sm_count));
-  // Items of different length are taken from a counter (zeroed on the stream before the launch);
-  // a prefix's are alike and dealt in order.
-  if (!p.all_rows && !p.cluster) {
-    p.counter = reinterpret_cast<int*>(ws);
-    cudaError_t e = cudaMemsetAsync(ws, 0, sizeof(int), stream);
-    if (e != cudaSuccess) return fail_cuda(e, op, "work counter reset");
-  }
+  // Items of different length are taken from a counter (the caller has zeroed it); a prefix's are
+  // alike and dealt in order.
+  if (!p.all_rows && !p.cluster) p.counter = reinterpret_cast<int*>(ws);
   if (d->head_dim == 128)
     return d->dtype == LVB_BF16 ? launch_flash<128, true>(tq, tk, tv, p, ctas, stream, dev)
                                 : launch_flash<128, false>(tq, tk, tv, p, ctas, stream, dev);

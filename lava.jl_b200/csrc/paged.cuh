@@ -140,9 +140,12 @@ struct MergeParams {
   int tile_splits;             // 0: none
   int ppt;                     // positions per 128-row tile
   int pairs_per_seq;           // 0: pairs run over the tokens of the whole batch (the prefix)
-  // The pieces of the decoding kernel: [slot][rows][D], and where each item's pieces are.
-  const float* dec_o;
-  const float* dec_ml;
+  // The parts of a sequence's own keys beside a prefix's: the flash kernel's tiles again (laid out
+  // as above, `own_pairs` per sequence), or the pieces of the decoding kernel: [slot][rows][D],
+  // and where each item's pieces are.
+  const float* own_o;
+  const float* own_ml;
+  int own_splits, own_pairs;   // own_splits 0: the decoding kernel's
   const int4* dec_tab;         // [batch·Hkv]; NULL: none
   int dec_rows;
   int dec_slots, dec_ctas;     // bounds of the table's entries
@@ -180,16 +183,21 @@ struct FlashWorkspace {
 };
 enum { kFlashOwn = 1, kFlashPrefix = 2 };
 int64_t paged_flash_items(const lvb_paged_desc* d, int parts);
-// Key ranges per tile pair, and how many of them form a cluster (1: none).
+// Key ranges per tile pair, how many of them form a cluster (1: none), and the time this may take.
 struct FlashSplit {
   int splits, cluster;
+  double us;
 };
-FlashSplit paged_flash_split(const lvb_paged_desc* d, const PagedRoom& room, int parts);
-size_t paged_flash_workspace(const lvb_paged_desc* d, FlashSplit fs, int parts);
+// joined: the parts go to the join kernel in any case.
+FlashSplit paged_flash_split(const lvb_paged_desc* d, const PagedRoom& room, int parts, bool joined);
+bool paged_flash_gathers(const lvb_paged_desc* d, const PagedRoom& room);
+size_t paged_flash_workspace(const lvb_paged_desc* d, FlashSplit fs, int parts, bool joined);
+// The first 4 bytes of `ws` are a counter that the caller zeroes on the stream (not for the prefix
+// alone). The own pass of a joined call stands behind the prefix's and runs beside it.
 int paged_flash_launch(const lvb_paged_desc* d, const PagedLayout& lay, const PagedSeqs& seqs,
                        const void* Q, const void* Kc, const void* Vc, void* O, float* lse, int parts,
-                       FlashSplit fs, void* ws, FlashWorkspace* out, cudaStream_t stream,
-                       DeviceState* dev);
+                       bool joined, FlashSplit fs, void* ws, FlashWorkspace* out,
+                       cudaStream_t stream, DeviceState* dev);
 
 struct SeqInfo {
   int tok0;   // first query row

@@ -269,8 +269,14 @@ def test_plans(lvb):
         p = lvb.attention_paged_plan(*args)
         assert p.cluster == cluster, (args, p.cluster)
         assert (p.launches, p.workspace_bytes == 0) == ((1, True) if cluster else (2, False))
-    assert lvb.attention_paged_plan(8, 64, 8, 32, 4, 64, 256).kernel == lvb.PAGED_DECODE    # 32 rows
-    assert lvb.attention_paged_plan(8, 64, 8, 40, 5, 64, 256).kernel == lvb.PAGED_FLASH     # 40 rows
+    assert lvb.attention_paged_plan(8, 64, 8, 16, 2, 64, 256).kernel == lvb.PAGED_DECODE    # 16 rows
+    assert lvb.attention_paged_plan(8, 64, 8, 24, 3, 64, 256).kernel == lvb.PAGED_FLASH     # 24 rows
+    # ... behind a long prefix: its keys once for the rows of all sequences, then theirs beside them
+    p = lvb.attention_paged_plan(32, 64, 8, 128, 4, 64, 5, prefix_len=16384)
+    assert (p.kernel, p.splits, p.cluster, p.launches) == (lvb.PAGED_FLASH, 1, 0, 3)
+    assert p.prefix_splits == 4
+    parts = 4 * 8 * 4 * 256 * 130 * 4 + 256                       # four tile pairs, eight KV heads
+    assert p.workspace_bytes == parts + 32 * 8 * 256 * 130 * 4 + 256
     p = lvb.attention_paged_plan(1, 32, 8, 64, 64, 64, 1000)
     assert (p.kernel, p.splits, p.cluster, p.launches) == (lvb.PAGED_FLASH, 18, 2, 2)
     p = lvb.attention_paged_plan(1, 32, 8, 64, 64, 64, 4)             # two blocks of keys

@@ -226,9 +226,9 @@ def run_attention(lvb, torch, c, Hq, qlens, causal=True, scale=None, cu=True, sp
     (8, 8, 8, [1, 7, 8, 9, 127, 128, 129, 700], [1] * 8, True),   # ends around a page and a block
     (64, 64, 8, [0, 1000, 64, 0, 3], [1] * 5, True),              # sequences without a key
     (48, 12, 4, [500, 2, 131], [3, 1, 2], True),                  # pages that no block divides
-    (256, 32, 1, [300, 5000], [1, 1], True),                      # 32 rows per KV head
-    (32, 16, 2, [77, 1, 260], [4, 2, 0], True),                   # rows that see no key, no rows
-    (16, 16, 4, [90, 300], [5, 5], False),                        # no causal mask
+    (256, 16, 1, [300, 5000], [1, 1], True),                      # 16 rows per KV head
+    (32, 8, 2, [77, 1, 260], [4, 2, 0], True),                    # rows that see no key, no rows
+    (16, 12, 4, [90, 300], [5, 5], False),                        # no causal mask
     (24, 6, 2, [20000], [2], True),                               # one long sequence: split
     (128, 4, 4, [3000, 40, 2500, 1, 900, 128, 129] * 5, [1] * 35, True),
 ])
@@ -246,6 +246,9 @@ def test_decode(lvb, torch_cuda, T, D, page, Hq, Hkv, lens, qlens, causal, wide)
 @pytest.mark.parametrize("T,D", [("bf16", 128), ("fp16", 128), ("bf16", 64), ("fp16", 64)])
 @pytest.mark.parametrize("page,Hq,Hkv,lens,qlens,causal", [
     (16, 8, 1, [40], [5], True),                          # 40 rows of one tile
+    (256, 32, 1, [300, 5000], [1, 1], True),              # 32 rows of a token
+    (32, 16, 2, [77, 1, 260], [4, 2, 0], True),           # rows that see no key, no rows
+    (16, 16, 4, [90, 300], [5, 5], False),                # 20 rows, no causal mask
     (64, 2, 2, [256, 300], [256, 40], True),              # one head per KV head
     (8, 6, 2, [700, 0, 333, 130], [200, 0, 333, 1], True),   # groups of 3: 42 positions a tile
     (48, 10, 2, [1000, 90], [130, 80], True),             # groups of 5
@@ -275,6 +278,25 @@ def test_chunks(lvb, torch_cuda, T, D, page, Hq, Hkv, lens, qlens, causal):
 def test_shared_prefix(lvb, torch_cuda, T, D, page, Hq, Hkv, prefix, lens, qlens):
     c = Cache(torch_cuda, T, Hkv, D, page, lens, prefix=prefix, seed=prefix)
     run_attention(lvb, torch_cuda, c, Hq, qlens, spare_rows=3)
+
+
+@pytest.mark.parametrize("T,D", [("bf16", 128), ("fp16", 64)])
+@pytest.mark.parametrize("page,Hq,Hkv,prefix,lens,qlens,splits", [
+    (16, 64, 8, 2003, [33, 0, 200, 3, 129] * 4, [3, 1, 2, 0, 3] * 4, 1),
+    (64, 24, 8, 8193, [1500, 60, 7] * 3, [9, 1, 7] * 3, 2),       # own keys in ranges too
+    (32, 6, 1, 20000, [30, 0, 2] * 20, [20, 3, 3] * 20, 1),       # rows of several tile pairs
+    (32, 20, 4, 6000, [0] * 30, [5] * 30, 1),                     # no own keys at all
+])
+def test_shared_prefix_gathered(lvb, torch_cuda, T, D, page, Hq, Hkv, prefix, lens, qlens, splits):
+    """More rows than the decoding kernel takes: the prefix read once for the rows of all sequences,
+    and joined with the flash kernel's parts over their own keys."""
+    c = Cache(torch_cuda, T, Hkv, D, page, lens, prefix=prefix, seed=prefix)
+    p = lvb.attention_paged_plan(len(lens), Hq, Hkv, sum(qlens) + 3, max(qlens), page, c.table.shape[1], D=D,
+                                 prefix_len=prefix)
+    assert p.kernel == lvb.PAGED_FLASH and p.prefix_splits > 0 and p.launches == 3
+    assert (p.splits > 1) == (splits > 1)
+    run_attention(lvb, torch_cuda, c, Hq, qlens, spare_rows=3)
+    run_attention(lvb, torch_cuda, c, Hq, qlens, causal=False)
 
 
 @pytest.mark.parametrize("Hq,lens,qlens,prefix", [(8, [3000, 700, 5], [1, 1, 1], 0),
@@ -312,7 +334,7 @@ def test_many_sequences(lvb, torch_cuda):
 
 def test_repeatable(lvb, torch_cuda):
     torch = torch_cuda
-    for qlens, prefix in ([1] * 9, 0), ([1] * 9, 700), ([40] * 9, 0):
+    for qlens, prefix in ([1] * 9, 0), ([1] * 9, 700), ([40] * 9, 0), ([9] * 9, 6000):
         c = Cache(torch, "bf16", 2, 128, 32, [2000, 3, 900, 50, 128, 4000, 77, 1, 600], prefix=prefix, seed=3)
         if qlens[0] > 1:
             c.seq_lens = c.seq_lens.clamp(min=0)
