@@ -360,6 +360,8 @@ def test_repeatable(lvb, torch_cuda):
     (64, 0, 3, [65, 64], [2, 1], 0, None, "halves", 0),           # no rotation, no queries
     (64, 0, 3, [65, 64], [2, 1], 32, None, "pairs", 1000),        # keys only, behind a prefix
     (32, 64, 8, [33] * 70, [1] * 70, 32, None, "halves", 0),
+    (16, 2, 1, [20, 3, 9, 50, 1] * 300, [1, 0, 3, 0, 1] * 300, 32, None, "halves", 0),   # 1,500 entries
+    (16, 2, 1, [0] * 700 + [70, 900] + [4] * 800, [0] * 700 + [70, 600] + [0] * 800, 16, None, "pairs", 0),
 ])
 def test_append(lvb, torch_cuda, T, D, page, Hq, Hkv, lens, qlens, pairs, sections, layout, prefix):
     torch = torch_cuda
