@@ -491,7 +491,8 @@ typedef enum lvb_paged_kernel {
   LVB_PAGED_FLASH = 0,    /* 128-row tiles of (position, head of the group) rows */
   LVB_PAGED_DECODE = 1    /* group·max_q <= 16: the cache streamed once, its key blocks dealt
                              evenly to the SMs whatever the lengths, or (few or short sequences:
-                             `cluster`) an item's blocks to the CTAs of a cluster */
+                             `cluster`) an item's blocks to the CTAs of a cluster, or (tables of at
+                             most 1,024 keys) whole items; the last two take one launch */
 } lvb_paged_kernel;
 
 typedef struct lvb_paged_plan {

@@ -233,7 +233,7 @@ int plan_paged(const lvb_paged_desc* d, const PagedRoom& room, lvb_paged_plan* o
     out->prefix_splits = paged_flash_split(d, room, kFlashPrefix, true).splits;
   const bool joined = out->prefix_splits > 0;
   if (decode) {
-    if (!joined && (out->cluster = paged_decode_cluster(d, room)) > 0) {
+    if (!joined && ((out->cluster = paged_decode_cluster(d, room)) > 0 || paged_decode_whole(d))) {
       out->launches = 1;      // no parts in memory
       return LVB_OK;
     }
@@ -420,7 +420,7 @@ int lvb_attention_paged(const lvb_paged_desc* d, const void* Q, const void* Kc, 
   mp.o_sh = lay.o[1];
   mp.lse = lse;
   uint8_t* ws = nullptr;
-  if (pl.kernel == LVB_PAGED_DECODE && pl.cluster > 0) {
+  if (pl.kernel == LVB_PAGED_DECODE && pl.launches == 1) {
     DecodeWorkspace none = {};
     return paged_decode_launch(d, lay, mp.seqs, Q, Kc, Vc, O, lse, false, false, pl.cluster, ws, &none,
                                s, dev);

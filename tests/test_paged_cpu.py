@@ -265,10 +265,13 @@ def test_plans(lvb):
                           ((1, 32, 8, 1, 1, 16, 640), 10), ((1, 32, 8, 1, 1, 16, 641), 0),
                           ((1, 32, 8, 1, 1, 16, 1), 1), ((2, 32, 8, 2, 1, 16, 512), 0),
                           ((8, 32, 8, 8, 1, 16, 64), 2), ((16, 32, 8, 16, 1, 16, 64), 1),
-                          ((32, 32, 8, 32, 1, 16, 64), 0)]:
+                          ((32, 32, 8, 32, 1, 16, 72), 0)]:
         p = lvb.attention_paged_plan(*args)
         assert p.cluster == cluster, (args, p.cluster)
         assert (p.launches, p.workspace_bytes == 0) == ((1, True) if cluster else (2, False))
+    # many short ones: whole items, the same
+    p = lvb.attention_paged_plan(32, 32, 8, 32, 1, 16, 64)
+    assert (p.cluster, p.launches, p.workspace_bytes) == (0, 1, 0)
     assert lvb.attention_paged_plan(8, 64, 8, 16, 2, 64, 256).kernel == lvb.PAGED_DECODE    # 16 rows
     assert lvb.attention_paged_plan(8, 64, 8, 24, 3, 64, 256).kernel == lvb.PAGED_FLASH     # 24 rows
     # ... behind a long prefix: its keys once for the rows of all sequences, then theirs beside them

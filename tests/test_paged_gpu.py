@@ -231,6 +231,7 @@ def run_attention(lvb, torch, c, Hq, qlens, causal=True, scale=None, cu=True, sp
     (16, 12, 4, [90, 300], [5, 5], False),                        # no causal mask
     (24, 6, 2, [20000], [2], True),                               # one long sequence: split
     (128, 4, 4, [3000, 40, 2500, 1, 900, 128, 129] * 5, [1] * 35, True),
+    (16, 8, 8, [900, 40, 0, 1, 500, 128, 129, 257] * 9, [1, 2, 1, 1, 0, 2, 1, 2] * 9, True),   # whole items
 ])
 def test_decode(lvb, torch_cuda, T, D, page, Hq, Hkv, lens, qlens, causal, wide):
     """With a table as wide as the lengths (short or few sequences: clusters of CTAs join an item in
