@@ -217,7 +217,7 @@ int device_room(DeviceState* dev, PagedRoom* out, const char* op) {
 // keys need.
 size_t prefix_bytes(const lvb_paged_desc* d, const lvb_paged_plan& pl) {
   if (!pl.prefix_splits) return 0;
-  return up256(paged_flash_workspace(d, FlashSplit{pl.prefix_splits, 1}, kFlashPrefix, true));
+  return up256(paged_flash_workspace(d, FlashSplit{pl.prefix_splits, 1, 0.0}, kFlashPrefix, true));
 }
 
 int plan_paged(const lvb_paged_desc* d, const PagedRoom& room, lvb_paged_plan* out) {
@@ -430,15 +430,17 @@ int lvb_attention_paged(const lvb_paged_desc* d, const void* Q, const void* Kc, 
   const bool bf16 = d->dtype == LVB_BF16;
   const bool joined = pl.prefix_splits > 0;
   uint8_t* own_ws = ws + prefix_bytes(d, pl);
+  const int parts = kFlashOwn | (d->prefix_len && !joined ? kFlashPrefix : 0);
+  const FlashSplit fs{pl.splits, std::max(1, pl.cluster), 0.0};
   // (before the prefix's kernel, so that nothing stands between it and the one behind it)
-  if (pl.kernel == LVB_PAGED_FLASH && pl.cluster == 0) {
+  if (pl.kernel == LVB_PAGED_FLASH && paged_flash_counts(d, fs, parts, dev->sm_count)) {
     e = cudaMemsetAsync(own_ws, 0, sizeof(int), s);
     if (e != cudaSuccess) st = fail_cuda(e, op, "work counter reset");
   }
   FlashWorkspace fw = {};
   if (joined && st == LVB_OK) {
     st = paged_flash_launch(d, lay, mp.seqs, Q, Kc, Vc, O, lse, kFlashPrefix, true,
-                            FlashSplit{pl.prefix_splits, 1}, ws, &fw, s, dev);
+                            FlashSplit{pl.prefix_splits, 1, 0.0}, ws, &fw, s, dev);
     mp.tile_o = fw.tile_o;
     mp.tile_ml = fw.tile_ml;
     mp.tile_splits = pl.prefix_splits;
@@ -458,8 +460,6 @@ int lvb_attention_paged(const lvb_paged_desc* d, const void* Q, const void* Kc, 
     // about as many pieces per item as there are CTAs for each, and one more
     pieces += dw.ctas / (int)(d->batch * d->heads_kv) + 2;
   } else {
-    const int parts = kFlashOwn | (d->prefix_len && !joined ? kFlashPrefix : 0);
-    const FlashSplit fs{pl.splits, std::max(1, pl.cluster)};
     if (st == LVB_OK)
       st = paged_flash_launch(d, lay, mp.seqs, Q, Kc, Vc, O, lse, parts, joined, fs, own_ws, &fw, s, dev);
     const int groups = fs.splits / fs.cluster;
