@@ -300,18 +300,20 @@ __device__ __forceinline__ int sequences_of(const PagedSeqs& p, int t0, int n, S
   for (; lo < p.batch; lo += 32) {
     const int k = min(lo + lane, p.batch - 1);
     const int w0 = p.cu_q[k], w1 = p.cu_q[k + 1], wl = p.lens[k];
-    for (int i = 0; i < n; ++i) {
-      const unsigned in = __ballot_sync(0xffffffffu, w0 <= t0 + i && t0 + i < w1);
-      const int src = __ffs(in) - 1;
-      const int r0 = __shfl_sync(0xffffffffu, w0, max(src, 0));
-      const int r1 = __shfl_sync(0xffffffffu, w1, max(src, 0));
-      const int l = __shfl_sync(0xffffffffu, wl, max(src, 0));
-      if (in && lane == i && b < 0) {
-        b = min(lo + src, p.batch - 1);
-        row0 = r0;
-        row1 = r1;
-        len = l;
-      }
+    int src = 0;          // the last of them that starts at or before the lane's token
+#pragma unroll
+    for (int step = 16; step > 0; step >>= 1) {
+      const int start = __shfl_sync(0xffffffffu, w0, src + step);
+      if (start <= t0 + lane) src += step;
+    }
+    const int r0 = __shfl_sync(0xffffffffu, w0, src);
+    const int r1 = __shfl_sync(0xffffffffu, w1, src);
+    const int l = __shfl_sync(0xffffffffu, wl, src);
+    if (lane < n && b < 0 && r0 <= t0 + lane && t0 + lane < r1) {
+      b = min(lo + src, p.batch - 1);
+      row0 = r0;
+      row1 = r1;
+      len = l;
     }
     if (!__any_sync(0xffffffffu, lane < n && b < 0)) break;
   }
