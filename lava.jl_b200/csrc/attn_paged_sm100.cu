@@ -1011,6 +1011,13 @@ FlashSplit paged_flash_split(const lvb_paged_desc* d, const PagedRoom& room, int
   return best;
 }
 
+size_t paged_flash_workspace(const lvb_paged_desc* d, FlashSplit fs, int parts, bool joined) {
+  const int groups = fs.splits / fs.cluster;
+  const bool store = joined || groups > 1;
+  return kCounterBytes + (store ? (size_t)paged_flash_items(d, parts) * groups * 256 *
+                                      (d->head_dim + 2) * sizeof(float) : 0);
+}
+
 // Whether the prefix is read in a pass of its own, whose tiles hold the rows of all sequences, and
 // joined with the sequences' own parts, or by every sequence's tiles in front of its own keys.
 // The first has fewer tiles where a sequence's rows do not fill one, but its parts go through
@@ -1022,18 +1029,14 @@ bool paged_flash_gathers(const lvb_paged_desc* d, const PagedRoom& room) {
   if (d->prefix_len == 0) return false;
   const FlashSplit pre = paged_flash_split(d, room, kFlashPrefix, true);
   const FlashSplit own = paged_flash_split(d, room, kFlashOwn, true);
+  // (not with parts beyond the workspace that the pool keeps: a part has all 256 rows of a pair)
+  if (paged_flash_workspace(d, pre, kFlashPrefix, true) + paged_flash_workspace(d, own, kFlashOwn, true) >
+      (size_t)512 << 20)
+    return false;
   const double rows = (double)d->batch * (double)d->max_q * (double)d->heads_q;   // of the join
-  if (rows > (double)(1 << 24)) return false;
   const double parts_us = rows * (double)(pre.splits + own.splits) * (double)(d->head_dim + 2) * 8.0 / 5e6;
   return pre.us + own.us + parts_us + kJoinUs + kPassUs <
          paged_flash_split(d, room, kFlashOwn | kFlashPrefix, false).us;
-}
-
-size_t paged_flash_workspace(const lvb_paged_desc* d, FlashSplit fs, int parts, bool joined) {
-  const int groups = fs.splits / fs.cluster;
-  const bool store = joined || groups > 1;
-  return kCounterBytes + (store ? (size_t)paged_flash_items(d, parts) * groups * 256 *
-                                      (d->head_dim + 2) * sizeof(float) : 0);
 }
 
 // Items of different length are taken from a counter, when there are more than CTAs; a prefix's are

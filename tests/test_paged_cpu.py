@@ -289,3 +289,8 @@ def test_plans(lvb):
     p = lvb.attention_paged_plan(16, 32, 8, 16384, 2048, 64, 1000, prefix_len=500)
     assert (p.kernel, p.splits, p.prefix_splits, p.launches) == (lvb.PAGED_FLASH, 1, 0, 1)
     assert lvb.attention_paged_plan(0, 32, 8, 0, 1, 64, 4).launches == 0
+    # the join's rows are counted in 32 bits; parts beyond 512 MiB are not gathered
+    with pytest.raises(lvb.LavaError, match="split the batch"):
+        lvb.attention_paged_plan(2 ** 25 + 1, 16, 1, 2 ** 25 + 1, 1, 128, 16)
+    assert lvb.attention_paged_plan(400, 64, 8, 1600, 4, 64, 5, prefix_len=16384).prefix_splits > 0
+    assert lvb.attention_paged_plan(600, 64, 8, 2400, 4, 64, 5, prefix_len=16384).prefix_splits == 0
