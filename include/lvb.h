@@ -502,7 +502,7 @@ typedef struct lvb_paged_plan {
   int32_t splits;         /* LVB_PAGED_FLASH: key-range splits per query tile pair */
   int32_t prefix_splits;  /* > 0: the prefix is read once for all query rows of a KV head, in
                              this many key ranges, and joined with the sequences' own part;
-                             0: no prefix, or (LVB_PAGED_FLASH) read by every sequence's tiles */
+                             0: no prefix, or read in front of every sequence's own keys */
   int32_t cluster;        /* CTAs of a (sequence, KV head), or of a split tile pair, that join their
                              parts in shared memory; 0: no such clusters */
   int32_t launches;       /* kernel launches per call */

@@ -229,14 +229,14 @@ int plan_paged(const lvb_paged_desc* d, const PagedRoom& room, lvb_paged_plan* o
   out->kernel = decode ? LVB_PAGED_DECODE : LVB_PAGED_FLASH;
   if (paged_flash_items(d, kFlashOwn) > INT32_MAX - 65536)
     return fail(LVB_ERR_UNSUPPORTED, op, "more than 2^31 query tiles", "split the batch");
+  if (decode && ((out->cluster = paged_decode_cluster(d, room)) > 0 || paged_decode_whole(d, room.sms))) {
+    out->launches = 1;      // no parts in memory
+    return LVB_OK;
+  }
   if (d->prefix_len && (decode || paged_flash_gathers(d, room)))
     out->prefix_splits = paged_flash_split(d, room, kFlashPrefix, true).splits;
   const bool joined = out->prefix_splits > 0;
   if (decode) {
-    if (!joined && ((out->cluster = paged_decode_cluster(d, room)) > 0 || paged_decode_whole(d))) {
-      out->launches = 1;      // no parts in memory
-      return LVB_OK;
-    }
     // (rows of the join, counted in 32 bits)
     if ((double)d->batch * (double)d->max_q * (double)d->heads_q > (double)(INT32_MAX / 4))
       return fail(LVB_ERR_UNSUPPORTED, op, "more than 2^29 query rows", "split the batch");

@@ -167,7 +167,7 @@ struct DecodeWorkspace {
 };
 // CTAs per item when its blocks are split over a cluster, 0 when they are dealt to all CTAs.
 int paged_decode_cluster(const lvb_paged_desc* d, const PagedRoom& room);
-bool paged_decode_whole(const lvb_paged_desc* d);   // no item is cut (and `ws` NULL)
+bool paged_decode_whole(const lvb_paged_desc* d, int sm_count);   // no item is cut (and `ws` NULL)
 size_t paged_decode_workspace(const lvb_paged_desc* d, int sm_count, bool keep_parts);
 // keep_parts: every item's result stays in the workspace for the join with a prefix's parts.
 // after_prefix: the kernel before it is the same call's flash kernel over the prefix.

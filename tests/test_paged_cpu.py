@@ -259,7 +259,11 @@ def test_plans(lvb):
     assert p.workspace_bytes == 64 * 16 + 2 * 148 * 16 * 130 * 4
     p = lvb.attention_paged_plan(8, 64, 8, 8, 1, 64, 256, prefix_len=16384)
     assert (p.kernel, p.prefix_splits, p.cluster, p.launches) == (lvb.PAGED_DECODE, 16, 0, 3)
-    assert lvb.attention_paged_plan(4, 32, 8, 4, 1, 16, 4, prefix_len=500).prefix_splits == 4
+    assert lvb.attention_paged_plan(64, 32, 8, 64, 1, 16, 4, prefix_len=500).prefix_splits > 0
+    # ... and few or short sequences by the decoding form, each in front of its own keys
+    for args, cluster in [((4, 32, 8, 4, 1, 16, 4), 3), ((32, 32, 8, 32, 1, 16, 4), 0)]:
+        p = lvb.attention_paged_plan(*args, prefix_len=500)
+        assert (p.kernel, p.prefix_splits, p.cluster, p.launches) == (lvb.PAGED_DECODE, 0, cluster, 1)
     # few or short sequences: clusters of CTAs, one launch, no workspace
     for args, cluster in [((1, 32, 8, 1, 1, 16, 49), 7), ((1, 32, 8, 1, 1, 16, 100), 7),
                           ((1, 32, 8, 1, 1, 16, 640), 10), ((1, 32, 8, 1, 1, 16, 641), 0),

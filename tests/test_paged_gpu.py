@@ -266,6 +266,25 @@ def test_chunks(lvb, torch_cuda, T, D, page, Hq, Hkv, lens, qlens, causal):
     run_attention(lvb, torch_cuda, c, Hq, qlens, causal, spare_rows=1)
 
 
+@pytest.mark.parametrize("T,D", [("bf16", 128), ("fp16", 128), ("bf16", 64), ("fp16", 64)])
+@pytest.mark.parametrize("page,Hq,Hkv,prefix,lens,qlens,cluster", [
+    (16, 4, 1, 1, [1], [1], True),                              # one block of each
+    (8, 8, 8, 129, [0, 7, 300, 0], [1, 2, 1, 0], True),         # none of their own; no rows
+    (48, 12, 2, 700, [500, 2, 131], [2, 1, 2], True),           # runs that pass from one to the other
+    (64, 16, 1, 2600, [900, 64], [1, 1], True),
+    (32, 8, 8, 255, [40, 0, 1, 128, 129, 257, 300] * 4, [2, 1, 1, 1, 2, 0, 2] * 4, False),   # whole items
+    (32, 16, 8, 896, [33, 1, 0] * 8, [1] * 24, False),
+])
+def test_prefix_in_front(lvb, torch_cuda, T, D, page, Hq, Hkv, prefix, lens, qlens, cluster):
+    """Few or short sequences: the decoding kernel reads the prefix in front of each one's own keys."""
+    c = Cache(torch_cuda, T, Hkv, D, page, lens, prefix=prefix, seed=prefix)
+    p = lvb.attention_paged_plan(len(lens), Hq, Hkv, sum(qlens) + 2, max(qlens), page, c.table.shape[1], D=D,
+                                 prefix_len=prefix)
+    assert (p.kernel, p.prefix_splits, p.launches, p.cluster > 0) == (lvb.PAGED_DECODE, 0, 1, cluster)
+    run_attention(lvb, torch_cuda, c, Hq, qlens, spare_rows=2)
+    run_attention(lvb, torch_cuda, c, Hq, qlens, causal=False)
+
+
 @pytest.mark.parametrize("T,D", [("bf16", 128), ("fp16", 64)])
 @pytest.mark.parametrize("page,Hq,Hkv,prefix,lens,qlens", [
     (16, 1, 1, 1, [1], [1]),
@@ -277,7 +296,11 @@ def test_chunks(lvb, torch_cuda, T, D, page, Hq, Hkv, lens, qlens, causal):
     (48, 4, 4, 128, [300], [300]),
 ])
 def test_shared_prefix(lvb, torch_cuda, T, D, page, Hq, Hkv, prefix, lens, qlens):
-    c = Cache(torch_cuda, T, Hkv, D, page, lens, prefix=prefix, seed=prefix)
+    """With a table for 100,000 keys: the prefix in a pass of its own, or by every sequence's tiles."""
+    c = Cache(torch_cuda, T, Hkv, D, page, lens, prefix=prefix, seed=prefix, width_more=100000 // page)
+    p = lvb.attention_paged_plan(len(lens), Hq, Hkv, sum(qlens) + 3, max(qlens), page, c.table.shape[1], D=D,
+                                 prefix_len=prefix)
+    assert (p.kernel == lvb.PAGED_DECODE) <= (p.prefix_splits > 0)
     run_attention(lvb, torch_cuda, c, Hq, qlens, spare_rows=3)
 
 
@@ -335,7 +358,7 @@ def test_many_sequences(lvb, torch_cuda):
 
 def test_repeatable(lvb, torch_cuda):
     torch = torch_cuda
-    for qlens, prefix in ([1] * 9, 0), ([1] * 9, 700), ([40] * 9, 0), ([9] * 9, 6000):
+    for qlens, prefix in ([1] * 9, 0), ([1] * 9, 700), ([1] * 9, 9000), ([40] * 9, 0), ([9] * 9, 6000):
         c = Cache(torch, "bf16", 2, 128, 32, [2000, 3, 900, 50, 128, 4000, 77, 1, 600], prefix=prefix, seed=3)
         if qlens[0] > 1:
             c.seq_lens = c.seq_lens.clamp(min=0)
