@@ -401,15 +401,29 @@ __global__ void __launch_bounds__(kRotThreads, kRotCtas) append_kernel(const App
 
 // Tokens per CTA and heads per CTA. As many tokens as leave about three CTAs per SM (the angles of a
 // token are worked out once for all its heads, 768 per CTA; the video clip's gradient 18.6 us with
-// 16 tokens, 20.0 with 8, 22.1 with 4); when one token per CTA is too few, its heads are
-// split too, never below one pass of the CTA's threads.
+// 16 tokens, 20.0 with 8, 22.1 with 4). Up to half more CTAs than run at once would wait for a second
+// round of few: then as many tokens as make one full round (4,900 tokens of 48 128-wide heads in 545 CTAs of
+// 9 tokens 24.8 us, in 613 of 8 29.8), or, at the most tokens and when a CTA's bytes take longer than its
+// chain of loads (3 us to the first, 1 us per kRotUnroll heads), two full rounds (10,000 such tokens in
+// 1,112 CTAs of 9 46.7, in 625 of 16 55.7; but two times 5,000 positions of eight 64-wide heads, whose
+// chain is longer, 9.1 and 7.3). When one token per CTA is too few, its heads are split too, never
+// below one pass of the CTA's threads.
 void rot_grid(long long tokens_per_row, long long rows, int heads, int tasks, int sms, int* n_tok,
               int* heads_per_cta) {
+  const long long slots = (long long)kRotCtas * sms;
   auto ctas = [&](int n) { return rows * ((tokens_per_row + n - 1) / n); };
   int n = 1;
   while (2 * n <= kRotTokens && 2 * n * tasks <= kRotThreads && ctas(2 * n) >= 3LL * sms) n *= 2;
+  if (ctas(n) > slots && 2 * ctas(n) < 3 * slots) {
+    while (ctas(n) > slots && n < kRotTokens && (n + 1) * tasks <= kRotThreads) ++n;
+    const int steps = heads * n * tasks / (kRotThreads * kRotUnroll);
+    const double bytes_us = n * heads * tasks * 64.0 * (double)slots / 6.5e6;
+    if (ctas(n) > slots && bytes_us > 3.0 + steps) {
+      while (n > 1 && ctas(n - 1) <= 2 * slots) --n;
+    }
+  }
   const int hpp = std::max(1, kRotThreads / (n * tasks));
-  const long long split = std::max<long long>(1, 4LL * sms / ctas(n));
+  const long long split = std::max<long long>(1, slots / ctas(n));
   int per = (int)((heads + split - 1) / split);
   per = std::min(heads, (per + hpp - 1) / hpp * hpp);
   *n_tok = n;
