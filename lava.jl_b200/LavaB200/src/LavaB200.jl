@@ -500,7 +500,7 @@ end
 
 Attention of packed queries `(E, Hq, T)` over a paged cache (the arguments of `kv_append!`; `seq_lens` counts
 the queries' own tokens). `prefix_table` (Int32, 0-based page numbers) and `prefix_len`: keys that
-stand before every sequence's own, read once for all. `lse` Float32 `(Hq, T)`.
+stand before every sequence's own. `lse` Float32 `(Hq, T)`.
 """
 function attention_paged!(O, Q, Kc, Vc, table, seq_lens; cu_q = nothing, max_q = nothing,
                           causal::Bool = true, scale::Real = inv(sqrt(size(Q, 1))), lse = nothing,

@@ -911,8 +911,8 @@ def attention_paged(O, Q, Kc, Vc, block_table, seq_lens, cu_q=None, max_q=None, 
     """Attention of packed queries over a paged cache: Q/O [tokens][Hq][D], the caches, the table and
     the lists as in ``kv_append`` (seq_lens counts the queries' own tokens). A query at place p
     sees places 0..p (``causal``; else all of its sequence's), and before them the ``prefix_len``
-    keys whose pages ``prefix_table`` (int32) lists, which all sequences share and the kernel reads
-    once for all when there are at most 32 query rows per KV head and sequence. Optional ``lse``
+    keys whose pages ``prefix_table`` (int32) lists, which all sequences share (read once for
+    all of them, or in front of each one's own where that takes less time). Optional ``lse``
     float32 [tokens][Hq]. Rows that see no key give O = 0 and lse = -inf; rows behind cu_q[B] are
     left as they were."""
     prepare_attention_paged(O, Q, Kc, Vc, block_table, seq_lens, cu_q, max_q, causal, scale, lse,
