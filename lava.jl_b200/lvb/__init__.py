@@ -651,12 +651,16 @@ def _refuse(op, message, status=LVB_ERR_INVALID_ARG):
 
 def _rows(op, name, t, extents):
     """Element strides of a tensor whose last dimension (head_dim) is contiguous; a dimension of
-    extent 1 gets one that any tensor could have (torch leaves it as it was)."""
+    extent 1 gets one that any tensor could have (torch leaves it as it was). Rows that share
+    elements (an expanded tensor) are refused here: in the descriptor, strides that are all 0 stand
+    for the packed layout."""
     if tuple(t.shape[:-1]) != tuple(extents):
         _refuse(op, f"{name} has shape {tuple(t.shape)}, needs {tuple(extents)} rows")
     D = t.shape[-1]
     if D > 1 and t.stride(-1) != 1:
         _refuse(op, f"{name}: head_dim must be contiguous", LVB_ERR_UNSUPPORTED)
+    if any(n > 1 and t.stride(i) < D for i, n in enumerate(extents)):
+        _refuse(op, f"{name}: stride below head_dim (an expanded tensor needs a copy)")
     return [t.stride(i) if n > 1 else D for i, n in enumerate(extents)]
 
 
