@@ -791,6 +791,8 @@ def _paged_desc(op, Kc, Vc, block_table, seq_lens, cu_q, max_q, tokens, heads_q,
             block_table.shape[1] > 1 and block_table.stride(1) != 1):
         _refuse(op, "block_table is int32 [B][pages per sequence], its rows contiguous")
     B = block_table.shape[0]
+    if B > 1 and block_table.stride(0) < block_table.shape[1]:    # (0 is "packed" in the descriptor)
+        _refuse(op, "block_table: stride below its width (an expanded table needs a copy)")
     _list_of(op, "seq_lens", seq_lens, torch.int32)
     if seq_lens.shape[0] != B:
         _refuse(op, f"seq_lens has {seq_lens.shape[0]} entries, block_table {B} rows")

@@ -68,3 +68,24 @@ def test_rows_of_extent_one_may_have_any_stride(lvb):
                 Kc=torch.empty(1, 8, 1, 128, dtype=BF), Vc=torch.empty(1, 8, 1, 128, dtype=BF),
                 block_table=torch.zeros(1, 1, dtype=I32), seq_lens=torch.zeros(1, dtype=I32))
     same(args, lvb.attention_paged, lvb)
+
+
+@pytest.mark.parametrize("call", ["attention_paged", "kv_append"])
+def test_expanded_table_is_refused(lvb, call):
+    """One row of pages expanded over the sequences: a row stride of 0 stands for packed rows in the
+    descriptor, so the entries behind the row would be read. Rows that overlap are refused too."""
+    Kc, Vc = (torch.empty(10, 16, 2, 128, dtype=BF) for _ in "kv")
+    X, Y = (torch.empty(3, 2, 128, dtype=BF) for _ in "xy")
+    names = ("O", "Q") if call == "attention_paged" else ("K", "V")
+    args = dict(zip(names, (X, Y)), Kc=Kc, Vc=Vc, seq_lens=torch.zeros(3, dtype=I32),
+                block_table=torch.zeros(3, 4, dtype=I32))
+    f = getattr(lvb, call)
+    same(args, f, lvb)
+    for table in (torch.zeros(1, 4, dtype=I32).expand(3, 4), torch.zeros(1, 1, dtype=I32).expand(3, 1),
+                  torch.zeros(12, dtype=I32).as_strided((3, 4), (2, 1))):
+        with pytest.raises(lvb.LavaError, match="block_table: stride below its width"):
+            f(**{**args, "block_table": table})
+    for table in (torch.zeros(3, 9, dtype=I32)[:, :4], torch.zeros(3, 0, dtype=I32)):
+        same({**args, "block_table": table}, f, lvb)
+    one = {k: v[:1] if k in names + ("seq_lens",) else v for k, v in args.items()}
+    same({**one, "block_table": torch.zeros(4, dtype=I32).as_strided((1, 4), (0, 1))}, f, lvb)
