@@ -405,6 +405,11 @@ function rotation(pairs::Integer, sections, layout::Symbol, inverse::Bool)
                     ntuple(i -> i <= length(s) ? Int32(s[i]) : Int32(0), 4))
 end
 
+# A descriptor names one type for all tensors of its call.
+same_eltype(op, T::Type, xs...) =
+    all(x -> x === nothing || eltype(x) === T, xs) ||
+    throw(ArgumentError("$op: the tensors must share the element type $T"))
+
 """
     rope!(Qo, Q, pos, freqs; Ko = nothing, K = nothing, sections = nothing, layout = :halves,
           inverse = false, stream = C_NULL)
@@ -423,6 +428,7 @@ function rope!(Qo, Q, pos, freqs; Ko = nothing, K = nothing, sections = nothing,
     Hkv = K === nothing ? 0 : size(K, 3)
     K === nothing || (size(Ko) == size(K) && size(K) == (E, L, Hkv, Bq)) ||
         throw(DimensionMismatch("rope!: K $(size(K)) Ko $(size(Ko))"))
+    same_eltype("rope!", eltype(Q), Qo, K, Ko)
     rot = rotation(length(freqs), sections, layout, inverse)
     (size(pos, 1), size(pos, 2), length(pos)) == (L, Bq, L * Bq * rot.n_axes) ||
         throw(DimensionMismatch("rope!: pos is (L, B) or (L, B, axes)"))
@@ -478,6 +484,9 @@ function kv_append!(Kc, Vc, K, V, table, seq_lens; cu_q = nothing, max_q = nothi
     Hq = Q === nothing ? 0 : size(Q, 2)
     Q === nothing || (size(Q) == (size(Kc, 1), Hq, T) && size(Qo) == size(Q)) ||
         throw(DimensionMismatch("kv_append!: Q $(size(Q)) Qo $(size(Qo))"))
+    same_eltype("kv_append!", eltype(Kc), Vc, K, V, Q, Qo)
+    freqs === nothing || eltype(freqs) === Float64 ||
+        throw(ArgumentError("kv_append!: freqs is Float64"))
     rot = freqs === nothing ? rotation(0, nothing, layout, false) :
           rotation(length(freqs), sections, layout, false)
     pos === nothing || (eltype(pos) === Int32 && length(pos) == T * rot.n_axes) ||
@@ -509,6 +518,7 @@ function attention_paged!(O, Q, Kc, Vc, table, seq_lens; cu_q = nothing, max_q =
     E, Hq, T = size(Q, 1), size(Q, 2), size(Q, 3)
     (size(O) == size(Q) && E == size(Kc, 1)) ||
         throw(DimensionMismatch("attention_paged!: Q $(size(Q)) O $(size(O)) cache $(size(Kc))"))
+    same_eltype("attention_paged!", eltype(Kc), O, Q, Vc)
     prefix_len == 0 || (prefix_table !== nothing && eltype(prefix_table) === Int32 &&
                         length(prefix_table) >= cld(prefix_len, size(Kc, 3))) ||
         throw(ArgumentError("attention_paged!: prefix_table must list the prefix's pages"))

@@ -31,6 +31,31 @@ using LinearAlgebra
         @test sizeof(LavaB200.PagedDesc) == 184 && sizeof(LavaB200.AppendDesc) == 256
     end
 
+    @testset "paged-cache calls refuse mixed element types (no GPU)" begin
+        h, f = Float16, Float32
+        x(T) = zeros(T, 64, 3, 2, 1)
+        pos, fr = reshape(Int32[0, 1, 2], 3, 1), ones(32)
+        @test_throws ArgumentError rope!(x(h), x(f), pos, fr)
+        @test_throws ArgumentError rope!(x(f), x(f), pos, fr; K = x(h), Ko = x(f))
+        @test_throws ArgumentError rope!(x(f), x(f), pos, fr; K = x(f), Ko = x(h))
+        @test_throws ArgumentError rope!(x(f), x(f), pos, Float32.(fr))
+        cache(T) = zeros(T, 64, 2, 16, 5)
+        new(T) = zeros(T, 64, 2, 1)
+        table, lens = reshape(Int32[4, 0, 2], 3, 1), Int32[3]
+        @test_throws ArgumentError kv_append!(cache(h), cache(f), new(h), new(h), table, lens)
+        @test_throws ArgumentError kv_append!(cache(h), cache(h), new(f), new(h), table, lens)
+        @test_throws ArgumentError kv_append!(cache(h), cache(h), new(h), new(f), table, lens)
+        for (q, qo) in ((f, h), (h, f))
+            @test_throws ArgumentError kv_append!(cache(h), cache(h), new(h), new(h), table, lens;
+                                                  Q = new(q), Qo = new(qo), freqs = fr)
+        end
+        @test_throws ArgumentError kv_append!(cache(h), cache(h), new(h), new(h), table, lens;
+                                              freqs = Float32.(fr))
+        @test_throws ArgumentError attention_paged!(new(f), new(h), cache(h), cache(h), table, lens)
+        @test_throws ArgumentError attention_paged!(new(h), new(f), cache(h), cache(h), table, lens)
+        @test_throws ArgumentError attention_paged!(new(h), new(h), cache(h), cache(f), table, lens)
+    end
+
     @testset "B200Backend is a KernelInterface.Backend (no GPU)" begin
         @test B200Backend() isa LavaB200.KI.Backend
     end
