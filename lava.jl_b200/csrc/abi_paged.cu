@@ -125,9 +125,6 @@ int check_paged(const char* op, const lvb_paged_desc* d) {
       d->batch > INT32_MAX || d->heads_q > 65535 || d->batch * d->heads_kv > INT32_MAX ||
       (d->batch > 0 && d->max_q > INT32_MAX / d->batch))
     return fail(LVB_ERR_UNSUPPORTED, op, "extent above 2^31-1", "split the batch");
-  // (key blocks of all items together: the decoding kernel counts them in 32 bits)
-  if (d->batch * d->heads_kv > INT32_MAX / 2 / (d->table_width * d->page_size / 128 + 2))
-    return fail(LVB_ERR_UNSUPPORTED, op, "more than 2^30 key blocks in the tables", "split the batch");
   const int64_t cache[3] = {d->num_pages, d->page_size, d->heads_kv};
   const int64_t rows[2] = {d->tokens, d->heads_q};
   int st;
@@ -153,6 +150,15 @@ int check_lists(const char* op, const lvb_paged_desc* d, const int32_t* table,
 // 1,000 keys, 15.8 and 10.6 over 300; at 16 rows 97 and 103, 16.3 and 20.1, 9.6 and 10.7.)
 bool use_decode(const lvb_paged_desc* d) {
   return (d->heads_q / d->heads_kv) * d->max_q <= 16;
+}
+
+// The decoding kernel deals units, an item's being its own key blocks and its cost, and counts them in
+// 32 bits: their total, and the total with one CTA's share behind it (at most half of it and a unit
+// when there are two CTAs; with one there is no second share). The prefix's blocks are not among
+// them but where paged_decode_whole bounds their number by the SMs'.
+bool units_fit(const lvb_paged_desc* d) {
+  const int64_t units = (d->table_width * d->page_size + 127) / 128 + paged_item_cost((int)d->head_dim);
+  return d->batch * d->heads_kv <= INT32_MAX / 3 * 2 / units;
 }
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
@@ -377,6 +383,9 @@ int lvb_attention_paged_check(const lvb_paged_desc* d) {
     return fail(LVB_ERR_INVALID_ARG, op, "scale must be a positive finite number");
   if (d->heads_q / d->heads_kv > 128)
     return fail(LVB_ERR_UNSUPPORTED, op, "more than 128 query heads per KV head");
+  if (use_decode(d) && !units_fit(d))
+    return fail(LVB_ERR_UNSUPPORTED, op, "more than 2^30 key blocks and items in the tables",
+                "split the batch");
   return LVB_OK;
 }
 

@@ -49,11 +49,8 @@ constexpr int kQkWarp = 10;
 constexpr int kPvWarp = 11;
 constexpr int kRows = 16;                  // rows of the products
 constexpr int kQueue = 8;                  // items published ahead
-// Blocks that an item's start and end count for when the blocks are dealt out: the time of three
-// 128-wide blocks, six 64-wide ones (measured on ragged batches: drafts over 64-wide heads 42.6 us
-// with 1, 33.7 with 4, 32.3 with 6; 61 sequences of 128-wide heads 107.3 with 1, 103.7 with 3).
 template <int D>
-constexpr int kItemCost = 384 / D;
+constexpr int kItemCost = paged_item_cost(D);   // units of an item beside its blocks
 constexpr int kChunk = 128 * 128;          // one 64-element chunk of a 128-key block
 constexpr float kLazy = 8.f;               // log2 units a score may exceed the reference maximum
 
