@@ -122,7 +122,8 @@ int check_paged(const char* op, const lvb_paged_desc* d) {
       d->prefix_len > kMostKeys)
     return fail(LVB_ERR_UNSUPPORTED, op, "more than 2^30 keys per sequence");
   if (d->num_pages >= INT32_MAX || d->tokens > INT32_MAX || d->max_q > INT32_MAX ||
-      d->batch > INT32_MAX || d->heads_q > 65535 || d->batch * d->heads_kv > INT32_MAX ||
+      d->batch > INT32_MAX || d->heads_q > 65535 || d->heads_kv > INT32_MAX / 2 ||
+      d->batch * d->heads_kv > INT32_MAX ||
       (d->batch > 0 && d->max_q > INT32_MAX / d->batch))
     return fail(LVB_ERR_UNSUPPORTED, op, "extent above 2^31-1", "split the batch");
   const int64_t cache[3] = {d->num_pages, d->page_size, d->heads_kv};

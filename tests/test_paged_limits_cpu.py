@@ -66,3 +66,14 @@ def test_other_calls_do_not_count_units(lvb):
     a.rot.n_axes = 1
     assert lvb.lib.lvb_kv_append_check(C.byref(a)) == 0
     assert attention_check(lvb, 10_000_000, 8, 64, 2, 256, max_q=17)[0] == 0
+
+
+@pytest.mark.parametrize("heads_kv", [2 ** 62, 2 ** 32 + 1, 2 ** 31])
+def test_heads_without_queries_are_bounded(lvb, heads_kv):
+    """An append without queries has no heads_q that would bound its KV heads: four sequences of 2^62
+    heads are 2^64 items, 0 in 64 bits."""
+    a = lvb.lvb_append_desc()
+    a.paged = desc(lvb, 4, heads_kv, 64, 1, 8, group=0)
+    a.rot.n_axes = 1
+    assert lvb.lib.lvb_kv_append_check(C.byref(a)) == lvb.LVB_ERR_UNSUPPORTED
+    assert "2^31" in lvb.lib.lvb_last_error().decode()
