@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr uint32_t kFmt = BF16 ? 1 : 0;
   constexpr uint32_t kIdescQK = make_idesc(1, kFmt, kFmt, 0, 0, 128, kRows);
   constexpr uint32_t kIdescPV = make_idesc(1, kFmt, kFmt, 1, 0, 128, kRows);
-  constexpr float kShift = BF16 ? 0.f : 6.f;
+  constexpr float kShift = kWeightShift<BF16>;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align_1024(smem_raw);

@@ -6,7 +6,8 @@
 // The mathematics and the inner loop are those of the dense flash kernel (attn_sm100.cu): S =
 // Q·Kᵀ per 128-key block into TMEM, softmax with thread = query row (running maximum, moved only
 // when it grows by more than 2^8, and sum in 32 bits), P in TMEM as the A operand of P·V, rounded
-// there to the inputs' type. What differs:
+// there to the inputs' type (the tensor core takes both operands in one 16-bit type). What differs:
+//   * in fp16 P is held 2^6 above its value (kWeightShift);
 //   * a tile's 128 rows are (position, head of the group): all query heads of a KV head stand in
 //     one tile, ppt = floor(128 / group) positions each, so a KV head's keys are read once for the
 //     group, and for a shared prefix once for the tokens of all sequences;
@@ -118,6 +119,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr uint32_t kFmt = BF16 ? 1 : 0;
   constexpr uint32_t kIdescQK = make_idesc(1, kFmt, kFmt, 0, 0, 128, 128);
   constexpr uint32_t kIdescPV = make_idesc(1, kFmt, kFmt, 0, 1, 128, D);
+  constexpr float kShift = kWeightShift<BF16>;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align_1024(smem_raw);
@@ -531,7 +533,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int pos = it.pos0 + t * p.ppt + row_pos;
       const bool row_ok = row_pos < p.ppt && pos < it.qlen;
       float m_ref = NEG_INF;   // running max (log2 domain, scale folded in)
-      float l = 0.f;           // running sum of p relative to m_ref
+      float l = 0.f;           // running sum of p relative to m_ref - kShift
       const int nt = t ? it.n_tile1 : it.n_tile0;
       // Keys of the sequence's own that the row sees, and that every row of the tile sees.
       const int own_keys = p.causal ? min(it.len, max(0, it.len - it.qlen + pos + 1)) : it.len;
@@ -586,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           m_ref = m_new;
           resc = true;
         }
-        const float m_use = m_ref == NEG_INF ? 0.f : m_ref;
+        const float m_use = (m_ref == NEG_INF ? 0.f : m_ref) - kShift;
         float sump[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < 64; ++c) {
@@ -634,13 +636,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int h = it.hk * p.group + row_head;
       if (p.cluster) {
         // O stays in TMEM until the CTA's products are done (below)
-        part_m = m_ref;
+        part_m = m_ref - kShift;
         part_l = l;
         part_nt = nt;
       } else if (p.store_parts) {
         const long long at = (long long)it.part * 256 + t * 128 + r;
         if (row_ok) {
-          p.tile_ml[at * 2] = m_ref;
+          p.tile_ml[at * 2] = m_ref - kShift;
           p.tile_ml[at * 2 + 1] = l;
         }
         if (nt > 0) {
@@ -689,7 +691,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc_fence_before();
         if (p.lse && row_ok) {
-          const float mu = (m_ref == NEG_INF) ? 0.f : m_ref;
+          const float mu = (m_ref == NEG_INF ? 0.f : m_ref) - kShift;
           p.lse[tok * p.Hq + h] = l == 0.f ? NEG_INF : (mu + log2f(l)) * 0.69314718055994530942f;
         }
       }

@@ -205,6 +205,13 @@ int paged_flash_launch(const lvb_paged_desc* d, const PagedLayout& lay, const Pa
                        bool joined, FlashSplit fs, void* ws, FlashWorkspace* out,
                        cudaStream_t stream, DeviceState* dev);
 
+// Log2 units that a weight of P is held above its value relative to the row's reference maximum. fp16:
+// 2^6, away from the subnormals, so that a weight is lost (in the product with V, not in the sum) below
+// 2^-31 of the reference and not below 2^-25, where a long flat tail still counts; a score may exceed
+// the reference by 2^8, and 2^14 is below the largest fp16. A part's m is lowered by as much.
+template <bool BF16>
+constexpr float kWeightShift = BF16 ? 0.f : 6.f;
+
 struct SeqInfo {
   int tok0;   // first query row
   int qlen;   // query rows (0: the sequence takes no part)
