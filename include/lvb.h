@@ -439,9 +439,11 @@ int lvb_rope(const lvb_rope_desc* d, const void* Q, const void* K, void* Qo, voi
  * reported through lvb_device_status as LVB_ERR_INVALID_ARG, with the call's effect limited:
  * site 81, a length that is negative or beyond the table's row (counts as 0); site 82, a page
  * number outside the cache (attention reads zeros, the append writes nothing); site 83, query
- * rows that do not fit in `tokens` or are more than max_q (the sequence is left out). No two tokens
- * of an append may share a place, and the first call of the library on a device is made outside
- * a capture.
+ * rows that do not fit in `tokens`, are fewer than none or more than max_q (the sequence is left
+ * out; an append takes cu_q to be in order where it looks for a token's sequence, so that tokens
+ * beside an entry that is not may be left out with it). Every sequence is checked, also one without
+ * new rows. No two tokens of an append may share a place, and the first call of the library on a
+ * device is made outside a capture.
  * ------------------------------------------------------------------------------------- */
 typedef struct lvb_paged_desc {
   int32_t dtype;          /* LVB_F16 or LVB_BF16 */

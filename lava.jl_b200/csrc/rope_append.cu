@@ -266,6 +266,7 @@ struct AppendParams {
   RotArgs rot;
   PagedSeqs seqs;
   int n_tok, tasks, T, heads_per_cta, Hq, Hkv;   // Hq 0: no queries
+  int check_chunks;                              // of kRotThreads - 32 sequences
   const uint8_t *K, *V, *Q;
   uint8_t *Kc, *Vc, *Qo;
   long long k[2], v[2], q[2], qo[2];             // byte strides of token, head
@@ -276,7 +277,8 @@ struct AppendParams {
 // the list, -1 for none. The last sequence that starts at or before t0 is found 32 at a time (two
 // rounds for 1,024), then 32 sequences from there on are held by the lanes and every token is
 // looked up among them: a few dependent loads for all tokens of the CTA (2,000 sequences of one token
-// 17.5 us when each token's warp went through the list from its start).
+// 17.5 us when each token's warp went through the list from its start). Where the offsets are not in
+// order a token may be missed; it is never taken for another sequence's.
 __device__ __forceinline__ int sequences_of(const PagedSeqs& p, int t0, int n, SeqInfo* s) {
   const int lane = (int)lane_id();
   int b = -1;
@@ -360,6 +362,13 @@ __global__ void __launch_bounds__(kRotThreads, kRotCtas) append_kernel(const App
   };
   if (threadIdx.x >= 32) {
     if (p.rot.pos) angles(threadIdx.x - 32, kRotThreads - 32);
+    // Every sequence's entries are checked by some thread, so that wrong ones are reported for a
+    // sequence without new rows too, and where the search for a token's sequence is led astray.
+    if (blockIdx.y == 0)
+      for (int c = blockIdx.x; c < p.check_chunks; c += gridDim.x) {
+        const unsigned b = (unsigned)c * (kRotThreads - 32) + threadIdx.x - 32;
+        if (b < (unsigned)p.seqs.batch) seq_info(p.seqs, (int)b);
+      }
   } else {
     const int i = threadIdx.x, n = min(p.n_tok, p.T - t0);
     SeqInfo s{0, 0, 0};
@@ -497,6 +506,7 @@ int append_launch(const lvb_append_desc* d, const PagedLayout& lay, const long l
   fill_rot(&p.rot, d->rot, pos, freqs, d->pos_stride);
   paged_seqs(&p.seqs, g, table, seq_lens, cu_q, nullptr, dev);
   p.T = (int)g.tokens;
+  p.check_chunks = (int)((g.batch + kRotThreads - 33) / (kRotThreads - 32));
   p.Hq = Q ? (int)g.heads_q : 0;
   p.Hkv = (int)g.heads_kv;
   p.tasks = (int)g.head_dim * 2 / 32;
