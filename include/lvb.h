@@ -454,7 +454,9 @@ typedef struct lvb_paged_desc {
                              many and tokens == batch·max_q */
   int64_t page_size;      /* a multiple of 8 */
   int64_t num_pages;
-  int64_t table_width;    /* entries of a row of the table that may be read */
+  int64_t table_width;    /* entries of a row of the table that may be read. The call is planned from
+                             it, the lengths being on the device: a table no wider than the longest
+                             sequence needs is the fastest */
   int64_t table_stride;   /* elements between rows (0: table_width) */
   int64_t prefix_len;     /* keys of the prefix that all sequences share (0: none): their places
                              come before place 0, every query sees all of them */
@@ -486,7 +488,8 @@ int lvb_kv_append(const lvb_append_desc* d, void* Kc, void* Vc, const void* K, c
 
 /* Attention of the packed queries over the paged cache, the same operation as lvb_attention_fwd
  * per sequence: O = softmax(scale·Q·Kᵀ + mask)·V over the prefix's keys and the sequence's own,
- * fp32 softmax, P rounded to the cache's type, GQA by head grouping; rows that see no key give
+ * fp32 softmax, P rounded to the cache's type (in fp16 a weight below 2^-31 of the row's largest may
+ * be lost from O; lse counts it), GQA by head grouping; rows that see no key give
  * O = 0 and lse = -inf. `lse` (nullable) is fp32 [token][heads_q]. What the pages hold behind a
  * sequence's last place, and the table behind its last page, plays no part, whatever it is; among
  * a sequence's own places (and the prefix's) an infinite or NaN value reaches every row of the call

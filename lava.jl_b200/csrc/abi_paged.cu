@@ -148,7 +148,9 @@ int check_lists(const char* op, const lvb_paged_desc* d, const int32_t* table,
 
 // The decoding kernel's products hold 16 rows. (More rows in wider products, with twice the softmax
 // per key, took 125 us at 24 rows over 8·8 times 16,384 keys, the flash kernel 106; 28 and 21 over
-// 1,000 keys, 15.8 and 10.6 over 300; at 16 rows 97 and 103, 16.3 and 20.1, 9.6 and 10.7.)
+// 1,000 keys, 15.8 and 10.6 over 300; at 16 rows 97 and 103, 16.3 and 20.1, 9.6 and 10.7. All of that
+// at 64 items, which the flash kernel splits in two key ranges; from 75 items on it does not, see
+// paged_flash_split, and the wider products were not measured there.)
 bool use_decode(const lvb_paged_desc* d) {
   return (d->heads_q / d->heads_kv) * d->max_q <= 16;
 }

@@ -17,9 +17,10 @@
 //   * items of at most eight blocks are not cut (paged_decode_whole): one launch, no join;
 //   * with few items, or short ones (the rule is at paged_decode_cluster), an item's blocks are split
 //     over a cluster of CTAs instead, which join their O, m and l through distributed shared memory:
-//     one launch, no workspace, no sums over the batch (a single sequence of 777 keys 9.1 us, 11.9
+//     one launch, no workspace, no sums over the batch (a single sequence of 777 keys 9.3 us, 11.6
 //     with the join kernel). In these two forms an item's blocks may begin with a prefix's, which all
-//     items share (4 sequences behind 500 keys 10.4 us, 14.7 with the prefix in a pass of its own);
+//     items share (4 sequences behind 500 keys 11.3 us, 21.0 with the prefix in a pass of its own and
+//     the items dealt and joined);
 //   * 384 threads: two softmax warpgroups take the blocks in turn, each with its own S and P
 //     buffer, maxima, sums and O accumulator (thread = key for Sᵀ, = head-dim element for Oᵀ), so
 //     one's chain of waits runs beside the other's; the one with an item's last block joins the

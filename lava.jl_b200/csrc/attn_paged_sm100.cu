@@ -311,7 +311,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       int n1 = im.pos0 + p.ppt < im.qlen
                    ? blocks_upto(p, npb, im.len, im.qlen, min(im.pos0 + rows2, im.qlen)) : 0;
       const int n = max(n0, n1);
-      // (n < 2^25 blocks, splits <= SMs: the products fit in 32 bits without a sign)
+      // (n <= 2^24 blocks, 2^23 of a prefix and as many own ones, and splits < 2^8, no more than the
+      // SMs: the products fit in 32 bits without a sign)
       im.kb0 = (int)((unsigned)n * split / p.splits);
       im.n_blocks = (int)((unsigned)n * (split + 1) / p.splits) - im.kb0;
       im.n_tile0 = min(max(n0 - im.kb0, 0), im.n_blocks);
@@ -986,7 +987,9 @@ int64_t paged_flash_items(const lvb_paged_desc* d, int parts) {
 
 // With fewer items than SMs: key ranges (of the prefix's length; of a table's row otherwise), by the
 // cost of a CTA's blocks (1.8 us each) and of a part that goes through memory (0.45 us with its
-// share of the join). Ranges meet in clusters where that spares the join kernel or most of its work
+// share of the join). With more items than half the SMs two ranges of each would not run at once, and an
+// item stays whole: 9 sequences of four drafts, 64 heads on 8, over 16,384 keys are 72 items and take 110.9 us
+// where their bytes take 92.4, 10 are 80 items and take 202.7 where theirs take 102.6. Ranges meet in clusters where that spares the join kernel or most of its work
 // (a cluster's join 1.5 us, the kernel 4 us): 64 new tokens of one sequence over 1,000, 4,000 and
 // 16,000 keys 14.8, 20.3 and 35.4 us with clusters, 21.6, 26.9 and 38.9 without. Parts that are
 // joined anyway (a prefix's and those beside it) do not: the kernel behind it fills the SMs as the

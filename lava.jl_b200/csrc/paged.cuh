@@ -199,7 +199,8 @@ bool paged_flash_gathers(const lvb_paged_desc* d, const PagedRoom& room);
 size_t paged_flash_workspace(const lvb_paged_desc* d, FlashSplit fs, int parts, bool joined);
 // Whether the first 4 bytes of `ws` are a counter, that the caller zeroes on the stream.
 bool paged_flash_counts(const lvb_paged_desc* d, FlashSplit fs, int parts, int sm_count);
-// The own pass of a joined call stands behind the prefix's and runs beside it.
+// The own pass of a joined call stands behind the prefix's: its CTAs take the SMs as the prefix's end
+// (both fill an SM's shared memory), without a gap between the two kernels.
 int paged_flash_launch(const lvb_paged_desc* d, const PagedLayout& lay, const PagedSeqs& seqs,
                        const void* Q, const void* Kc, const void* Vc, void* O, float* lse, int parts,
                        bool joined, FlashSplit fs, void* ws, FlashWorkspace* out,

@@ -22,8 +22,8 @@ constexpr int kRotThreads = 256;
 constexpr int kRotCtas = 4;           // per SM: 64 registers a thread
 constexpr int kRotTokens = 16;        // most tokens per CTA
 // Heads that a thread has under way at a time. Two, with four CTAs per SM, against one with five,
-// three or four with three: a video clip's gradient 18.6 us against 22.3, 20.9 and 22.0; prompts into
-// the cache 17.1 against 16.5, 16.3 and 16.3; 268 MB of Q and K 87.0 against 93.2, 88.5 and 86.1.
+// three or four with three: a video clip's gradient 18.3 us against 22.7, 19.8 and 19.9; prompts into
+// the cache 14.5 against 15.9, 14.5 and 14.6; 268 MB of Q and K 87.1 against 96.2, 89.0 and 88.9.
 constexpr int kRotUnroll = 2;
 
 struct RotArgs {
