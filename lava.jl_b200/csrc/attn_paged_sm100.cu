@@ -987,10 +987,11 @@ int64_t paged_flash_items(const lvb_paged_desc* d, int parts) {
 
 // With fewer items than SMs: key ranges (of the prefix's length; of a table's row otherwise), by the
 // cost of a CTA's blocks (1.8 us each) and of a part that goes through memory (0.45 us with its
-// share of the join). With more items than half the SMs two ranges of each would not run at once, and an
-// item stays whole: 9 sequences of four drafts, 64 heads on 8, over 16,384 keys are 72 items and take 110.9 us
-// where their bytes take 92.4, 10 are 80 items and take 202.7 where theirs take 102.6. Ranges meet in clusters where that spares the join kernel or most of its work
-// (a cluster's join 1.5 us, the kernel 4 us): 64 new tokens of one sequence over 1,000, 4,000 and
+// share of the join). With more items than half the SMs two ranges of each would not run at once,
+// and an item stays whole: 9 sequences of four drafts, 64 heads on 8, over 16,384 keys are 72 items
+// and take 110.9 us where their bytes take 92.4, 10 are 80 items and take 202.7 where theirs take
+// 102.6. Ranges meet in clusters where that spares the join kernel or most of its work (a
+// cluster's join 1.5 us, the kernel 4 us): 64 new tokens of one sequence over 1,000, 4,000 and
 // 16,000 keys 14.8, 20.3 and 35.4 us with clusters, 21.6, 26.9 and 38.9 without. Parts that are
 // joined anyway (a prefix's and those beside it) do not: the kernel behind it fills the SMs as the
 // CTAs end (16,384 keys before 64 sequences 87.2 us with clusters, 84.9 without), and cost a tenth
